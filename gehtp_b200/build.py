@@ -47,6 +47,7 @@ UNITS = {
     "window_attn_sm100.cu": [],
     "channel_delta.cu": [],
     "channel_chunks.cu": [],
+    "shared_attn.cu": [],
     "tp.cu": [],
     "tp_p2p.cu": [],
 }

@@ -1,0 +1,40 @@
+// Operators for a batch of sequences that go on from one prompt (shared_attn.cu, shared_attn_sm100.cu, kv_evict.cu,
+// verify_drafts.cu). All memory is the caller's: nothing is allocated, kept or remembered between calls.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace gehtp {
+
+// Attention over a shared prefix and own tails. A row is one query head of one token; the rows that meet a key head's
+// prefix together are those of p_tokens tokens (a row tile), those that meet a tail are the q_len * rep of its sequence.
+// Every (row tile, key head, slice of the prefix) and every (sequence, key head, slice of its tail) leaves a partial result per
+// row: the sum of 2^(s - m) v, the sum of 2^(s - m) and the maximum m, with s = log2(e) * scale * q.k.
+struct SharedArgs {
+    const uint16_t *q, *prefix, *tail;
+    const int32_t* n_tail;
+    const float* weights_in;
+    float* weights;
+    uint16_t* out;
+    uint32_t batch, q_len, rep, kv_heads, n_prefix, nslots;
+    size_t q_stride;
+    uint32_t p_tokens, p_tiles, p_slices, p_len;   // prefix: slices of p_len positions
+    uint32_t t_slices;                             // the tails of all sequences are cut into about so many slices
+    float sc;                                      // log2(e) * scale
+    float* part_o;                                 // [partial row][head_dim], the prefix's first
+    float2* part_ml;                               // [partial row] {m, sum}
+    float* scores;                                 // s of every tail position: [sequence][key head][row][nslots], or NULL
+    uint32_t* plan;                                // written by the first kernel: slices in front of each sequence's, batch + 1 of them
+    unsigned int* status;
+    __host__ __device__ size_t p_rows() const { return (size_t)p_tiles * kv_heads * p_slices * p_tokens * rep; }
+};
+
+// false: launch failed
+bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t row_tiles, bool prefix, bool tails);
+bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16);
+
+// true: `p` is memory of the current device (or managed); else g.last_error says which argument is not
+bool on_this_device(const void* p, const char* what);
+
+}  // namespace gehtp

@@ -1,0 +1,594 @@
+// Attention of a batch over a prefix that all its sequences share and a tail of each one's own:
+//
+//   out = sum_j p_j v_j,  p = softmax(scale q.k_j),  j over the prefix and over the tail positions the row sees
+//
+// Query t of a sequence (of q_len new tokens, the last positions of its tail) sees the tail up to its own position. The prefix is
+// read once for all sequences: its keys meet the rows of all of them, rep query heads to a key head. Rows of one tail are few
+// (q_len * rep). Positions that every row of a sequence sees go through the tensor cores without a mask; the up to
+// q_len - 1 positions behind them, each seen by some rows only, are added row by row (`zone` below), so no row's result depends
+// on a position that it does not see.
+//
+// shared_parts_kernel: CTAs that stay and walk the items (row tile, key head, slice of the prefix) and (sequence, key head, slice of
+// its tail). K and V tiles of 64 positions by cp.async in three or four stages; a warp has 16 rows and a quarter, a half or all of
+// a tile's positions; S and P stay in registers (mma.sync m16n8k16). How a batch's tails are cut follows from their lengths,
+// which lie on the device: every CTA works that out for itself.
+// shared_merge_kernel: partial results of a row together; where asked for, the weights of the tail positions.
+#include <climits>
+#include <cmath>
+#include <cstdio>
+#include "engine.h"
+#include "launchers_batch.h"
+#include "mma_bf16.cuh"
+#include "sm100_attn.cuh"
+
+namespace gehtp {
+
+namespace {
+
+constexpr uint32_t TILE = 64, MAX_BATCH = 1024, MAX_Q = 16, MAX_ROWS = 128;
+constexpr uint32_t SMS = 148;
+
+template <bool BF>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF) {
+        mma_bf16(c, a, b0, b1);
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*(const __half2*)&w);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (BF) return pack_bf2(a, b);
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&h;
+}
+
+__device__ __forceinline__ uint32_t tail_length(const SharedArgs& A, uint32_t b) { return (uint32_t)min(max(A.n_tail[b], 0), (int)A.nslots); }
+// tail positions that all rows of a sequence see
+__device__ __forceinline__ uint32_t common_length(const SharedArgs& A, uint32_t n) { return n + 1 > A.q_len ? n + 1 - A.q_len : 0; }
+
+// Slices in front of each sequence's (cum[batch]: all of them) and tiles to a slice, by one warp. Slices are as long as cuts
+// the tails together into about t_slices; a sequence with any position has one at least.
+__device__ uint32_t cut_tails(const SharedArgs& A, uint32_t* cum) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t tiles = 0;
+    for (uint32_t b = lane; b < A.batch; b += 32) tiles += (common_length(A, tail_length(A, b)) + TILE - 1) / TILE;
+    for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    const uint32_t k = max(1u, (tiles + A.t_slices - 1) / A.t_slices);
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < A.batch; b0 += 32) {
+        const uint32_t b = b0 + lane;
+        uint32_t s = 0;
+        if (b < A.batch) {
+            const uint32_t n = tail_length(A, b), t = (common_length(A, n) + TILE - 1) / TILE;
+            s = n ? max(1u, (t + k - 1) / k) : 0;
+        }
+        uint32_t x = s;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        if (b < A.batch) cum[b] = before + x - s;
+        before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) cum[A.batch] = before;
+    return k;
+}
+
+template <int HD>
+__host__ __device__ constexpr int stages() { return HD == 128 ? 3 : 4; }
+template <int HD>
+__host__ __device__ constexpr size_t ring_bytes() { return (size_t)stages<HD>() * 2 * TILE * HD * 2; }
+template <int HD, int RT>
+__host__ __device__ constexpr size_t parts_smem() { return ring_bytes<HD>() + (size_t)16 * RT * 16 * 4 + (size_t)64 * (RT == 8 ? 2 : 1) * 8 + (MAX_BATCH + 4) * 4; }
+
+// RT row tiles of 16; the warps that RT leaves share a tile's positions
+template <bool BF, int HD, int RT>
+__global__ void __launch_bounds__(RT == 8 ? 256 : 128, RT == 8 ? 1 : 2)
+shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails) {
+    constexpr int NW = RT == 8 ? 8 : 4, NT = NW * 32, PG = NW / RT, NP = TILE / PG / 16, STG = stages<HD>(), LD = HD + 8;
+    constexpr uint32_t ROW = HD * 2, HALF = TILE * ROW;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* so = (float*)smem;                                       // [PG][16 RT][LD] once the tiles are done with
+    float* zone = (float*)(smem + ring_bytes<HD>());                // [16 RT][16]
+    float2* ml = (float2*)(zone + 16 * RT * 16);                    // [PG][16 RT]
+    uint32_t* cum = (uint32_t*)(ml + PG * 16 * RT);
+    __shared__ uint32_t s_k;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
+    const uint32_t rt = warp % RT, pg = warp / RT;
+    const uint32_t ring = smem_addr(smem);
+    pdl_wait();
+    pdl_release();     // behind the wait: what starts now may read all that was there before this call
+    if (with_tails) {
+        if (warp == 0) {
+            const uint32_t k = cut_tails(A, cum);
+            if (lane == 0) s_k = k;
+        }
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (uint32_t b = threadIdx.x; b <= A.batch; b += NT) A.plan[b] = cum[b];
+    }
+    const uint32_t items = prefix_items + (with_tails ? cum[A.batch] * A.kv_heads : 0);
+    const size_t p_rows = A.p_rows();
+    for (uint32_t w = blockIdx.x; w < items; w += gridDim.x) {
+        // ---- the item: rows, keys, place of its partial results
+        const bool tail = w >= prefix_items;
+        uint32_t h, rows, token0, from, to, c = 0, n = 0, b = 0;
+        size_t pitch, v_off, part;
+        const uint16_t* kbase;
+        bool last = false;
+        if (!tail) {
+            const uint32_t tile = w % A.p_tiles, u = w / A.p_tiles, s = u / A.kv_heads;
+            h = u % A.kv_heads;
+            token0 = tile * A.p_tokens;
+            rows = min(A.p_tokens, A.batch * A.q_len - token0) * A.rep;
+            from = s * A.p_len;
+            to = min(A.n_prefix, from + A.p_len);
+            v_off = (size_t)A.kv_heads * HD;
+            kbase = A.prefix + (size_t)h * HD;
+            part = (((size_t)tile * A.kv_heads + h) * A.p_slices + s) * (A.p_tokens * A.rep);
+        } else {
+            const uint32_t u = (w - prefix_items) / A.kv_heads;
+            h = (w - prefix_items) % A.kv_heads;
+            uint32_t hi = A.batch;                                  // cum[b] <= u < cum[b + 1]
+            while (hi - b > 1) {
+                const uint32_t mid = (b + hi) / 2;
+                if (cum[mid] <= u) b = mid; else hi = mid;
+            }
+            n = tail_length(A, b);
+            c = common_length(A, n);
+            token0 = b * A.q_len;
+            rows = A.q_len * A.rep;
+            from = (u - cum[b]) * s_k * TILE;
+            to = min(c, from + s_k * TILE);
+            last = u + 1 == cum[b + 1];
+            v_off = (size_t)A.batch * A.kv_heads * HD;
+            kbase = A.tail + ((size_t)b * A.kv_heads + h) * HD;
+            part = p_rows + ((size_t)u * A.kv_heads + h) * rows;
+        }
+        pitch = 2 * v_off;
+        const uint32_t tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
+
+        auto load = [&](uint32_t i) {
+            if (i < tiles) {
+                const uint32_t st = ring + (i % STG) * 2 * HALF;
+#pragma unroll 4
+                for (uint32_t e = threadIdx.x; e < TILE * HD / 8; e += NT) {
+                    const uint32_t r = e / (HD / 8), ch = e % (HD / 8), pos = from + i * TILE + r;
+                    const bool in = pos < to;                       // rows past the end: zeros, whatever the cache holds there
+                    const uint16_t* src = kbase + (in ? (size_t)pos * pitch + ch * 8 : 0);
+                    const uint32_t dst = st + r * ROW + ((ch ^ (r & 7)) * 16);
+                    cp16(dst, src, in ? 16 : 0);
+                    cp16(dst + HALF, src + (in ? v_off : 0), in ? 16 : 0);
+                }
+            }
+            cp_commit();
+        };
+        for (int i = 0; i < STG - 1; i++) load(i);
+
+        // ---- queries of this warp's rows as A fragments
+        uint32_t qf[HD / 16][4];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t r = rt * 16 + g8 + half * 8;
+            const bool in = r < rows;
+            const uint16_t* qp = A.q + (in ? (size_t)(token0 + r / A.rep) * A.q_stride + (size_t)(h * A.rep + r % A.rep) * HD : 0) + q4 * 2;
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++) {
+                qf[k][half] = in ? *(const uint32_t*)(qp + k * 16) : 0u;
+                qf[k][half + 2] = in ? *(const uint32_t*)(qp + k * 16 + 8) : 0u;
+            }
+        }
+        float o[HD / 8][4] = {};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+        for (uint32_t i = 0; i < tiles; i++) {
+            cp_wait<STG - 2>();
+            __syncthreads();
+            load(i + STG - 1);
+            const uint32_t p0 = from + i * TILE + pg * (TILE / PG);   // this warp's first position
+            if (p0 >= to || rt * 16 >= rows) continue;                 // the same for the whole warp
+            const uint32_t kt = ring + (i % STG) * 2 * HALF, vt = kt + HALF;
+            float s[2 * NP][4];
+#pragma unroll
+            for (int t = 0; t < NP; t++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[2 * t][e] = s[2 * t + 1][e] = 0.0f;
+                const uint32_t r = pg * (TILE / PG) + t * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++) {
+                    uint32_t f[4];
+                    ldsm4(f, kt + r * ROW + (((2 * k + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+                    mma16<BF>(s[2 * t], qf[k], f[0], f[1]);
+                    mma16<BF>(s[2 * t + 1], qf[k], f[2], f[3]);
+                }
+            }
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < 2 * NP; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool in = p0 + t * 8 + q4 * 2 + (e & 1) < to;
+                    s[t][e] = in ? s[t][e] * A.sc : -INFINITY;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+                }
+            if (tail && A.scores) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const uint32_t r = rt * 16 + g8 + half * 8;
+                    float* sp = A.scores + (((size_t)b * A.kv_heads + h) * rows + r) * A.nslots;
+                    if (r < rows)
+#pragma unroll
+                        for (int t = 0; t < 2 * NP; t++) {
+                            const uint32_t p = p0 + t * 8 + q4 * 2;
+                            if (p < to) sp[p] = s[t][2 * half];
+                            if (p + 1 < to) sp[p + 1] = s[t][2 * half + 1];
+                        }
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
+            }
+            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const float mn = fmaxf(m[half], mx[half]), f = m[half] == -INFINITY ? 0.0f : sm100::ex2(m[half] - mn);
+                    if (mn > m[half]) {
+                        m[half] = mn;
+                        l[half] *= f;
+#pragma unroll
+                        for (int j = 0; j < HD / 8; j++) { o[j][2 * half] *= f; o[j][2 * half + 1] *= f; }
+                    }
+                }
+            }
+            const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+            for (int t = 0; t < NP; t++) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {                          // fragment register e: tile 2 t + e / 2, rows of half e % 2
+                    float* x = &s[2 * t + (e >> 1)][2 * (e & 1)];
+                    const float a = sm100::ex2(x[0] - off[e & 1]), c2 = sm100::ex2(x[1] - off[e & 1]);
+                    l[e & 1] += a + c2;
+                    hi[e] = pack2<BF>(a, c2);
+                    // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
+                    if (BF) {
+                        const float2 u = unpack2<BF>(hi[e]);
+                        lo[e] = pack2<BF>(a - u.x, c2 - u.y);
+                    }
+                }
+                const uint32_t r = pg * (TILE / PG) + t * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++) {
+                    uint32_t f[4];
+                    ldsm4_t(f, vt + r * ROW + (((2 * j + ((lane >> 4) & 1)) ^ (r & 7)) * 16));
+                    mma16<BF>(o[2 * j], hi, f[0], f[1]);
+                    mma16<BF>(o[2 * j + 1], hi, f[2], f[3]);
+                    if (BF) {
+                        mma16<BF>(o[2 * j], lo, f[0], f[1]);
+                        mma16<BF>(o[2 * j + 1], lo, f[2], f[3]);
+                    }
+                }
+            }
+        }
+        cp_wait<0>();
+        __syncthreads();
+        // ---- the warps' results of a row together
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t r = rt * 16 + g8 + half * 8;
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+            if (q4 == 0) ml[pg * 16 * RT + r] = make_float2(m[half], l[half]);
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) *(float2*)&so[(size_t)(pg * 16 * RT + r) * LD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+        }
+        const uint32_t nz = last ? n - c : 0;                          // positions that only some rows see
+        for (uint32_t e = warp; e < rows * nz; e += NW) {
+            const uint32_t r = e / nz, i = e % nz, t = r / A.rep;
+            float s = -INFINITY;
+            if (c + i + A.q_len < n + t + 1) {                         // position c + i < n - q_len + t + 1
+                const uint16_t* qp = A.q + (size_t)(token0 + t) * A.q_stride + (size_t)(h * A.rep + r % A.rep) * HD + lane * (HD / 32);
+                const uint16_t* kp = kbase + (size_t)(c + i) * pitch + lane * (HD / 32);
+                float d = 0.0f;
+#pragma unroll
+                for (int x = 0; x < HD / 32; x += 2) {
+                    const float2 a = unpack2<BF>(*(const uint32_t*)(qp + x)), k2 = unpack2<BF>(*(const uint32_t*)(kp + x));
+                    d = fmaf(a.x, k2.x, fmaf(a.y, k2.y, d));
+                }
+                s = warp_sum(d) * A.sc;
+            }
+            if (lane == 0) {
+                zone[r * 16 + i] = s;
+                if (A.scores) A.scores[(((size_t)b * A.kv_heads + h) * rows + r) * A.nslots + c + i] = s;
+            }
+        }
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < rows * (HD / 4); e += NT) {
+            const uint32_t r = e / (HD / 4), c4 = e % (HD / 4);
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int p = 0; p < PG; p++) M = fmaxf(M, ml[p * 16 * RT + r].x);
+            for (uint32_t i = 0; i < nz; i++) M = fmaxf(M, zone[r * 16 + i]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int p = 0; p < PG; p++) {
+                const float2 x = ml[p * 16 * RT + r];
+                const float f = x.x == -INFINITY ? (x.y == 0.0f ? 0.0f : 1.0f) : sm100::ex2(x.x - M);   // a sum without a maximum is no number and stays one
+                const float4 v = *(const float4*)&so[(size_t)(p * 16 * RT + r) * LD + c4 * 4];
+                acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+                L = fmaf(x.y, f, L);
+            }
+            const uint32_t t = r / A.rep;
+            for (uint32_t i = 0; i < nz && c + i + A.q_len < n + t + 1; i++) {
+                const float p = sm100::ex2(zone[r * 16 + i] - (M == -INFINITY ? 0.0f : M));
+                const uint2 vw = *(const uint2*)(kbase + (size_t)(c + i) * pitch + v_off + c4 * 4);
+                const float2 va = unpack2<BF>(vw.x), vb = unpack2<BF>(vw.y);
+                acc.x = fmaf(p, va.x, acc.x); acc.y = fmaf(p, va.y, acc.y); acc.z = fmaf(p, vb.x, acc.z); acc.w = fmaf(p, vb.y, acc.w);
+                L += p;
+            }
+            *(float4*)&A.part_o[(part + r) * HD + c4 * 4] = acc;
+            if (c4 == 0) A.part_ml[part + r] = make_float2(M, L);
+        }
+        __syncthreads();
+    }
+}
+
+// Places of a row's partial results: `first` + i * step for i < count, of the prefix and of the tail.
+struct RowParts { size_t p_first, p_step, t_first, t_step; uint32_t p_count, t_count; };
+
+__device__ __forceinline__ RowParts row_parts(const SharedArgs& A, uint32_t token, uint32_t head) {
+    RowParts x;
+    const uint32_t h = head / A.rep, g = head % A.rep;
+    x.p_step = (size_t)A.p_tokens * A.rep;
+    x.p_count = A.n_prefix ? A.p_slices : 0;
+    x.p_first = x.p_count ? ((size_t)(token / A.p_tokens) * A.kv_heads + h) * A.p_slices * x.p_step + (token % A.p_tokens) * A.rep + g : 0;
+    const uint32_t b = token / A.q_len, rows = A.q_len * A.rep;
+    x.t_step = (size_t)A.kv_heads * rows;
+    x.t_count = 0; x.t_first = 0;
+    if (A.nslots) {
+        const uint32_t c0 = A.plan[b];
+        x.t_count = A.plan[b + 1] - c0;
+        x.t_first = A.p_rows() + ((size_t)c0 * A.kv_heads + h) * rows + (token % A.q_len) * A.rep + g;
+    }
+    return x;
+}
+__device__ __forceinline__ size_t part_at(const RowParts& x, uint32_t i) {
+    return i < x.p_count ? x.p_first + i * x.p_step : x.t_first + (i - x.p_count) * x.t_step;
+}
+__device__ __forceinline__ float part_factor(float2 ml, float M) { return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : sm100::ex2(ml.x - M); }
+
+constexpr uint32_t W_CHUNK = 512;
+
+// The first `row_blocks` CTAs: a warp to a row of the result. The others: 512 tail positions of a (sequence, key head) each.
+template <bool BF, int HD>
+__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, uint32_t row_blocks, uint32_t chunks) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_release();
+    if (blockIdx.x < row_blocks) {
+        const uint32_t heads = A.kv_heads * A.rep, row = blockIdx.x * 8 + warp;
+        if (row >= A.batch * A.q_len * heads) return;
+        const RowParts x = row_parts(A, row / heads, row % heads);
+        const uint32_t count = x.p_count + x.t_count;
+        float M = -INFINITY, L = 0.0f;
+        for (uint32_t i = lane; i < count; i += 32) M = fmaxf(M, __ldcg(&A.part_ml[part_at(x, i)]).x);
+        M = warp_max(M);
+        constexpr int V = HD / 32;
+        float acc[V] = {};
+        for (uint32_t i0 = 0; i0 < count; i0 += 32) {
+            const uint32_t mine = i0 + lane;
+            const float2 ml = mine < count ? __ldcg(&A.part_ml[part_at(x, mine)]) : make_float2(-INFINITY, 0.0f);
+            const float f = part_factor(ml, M);
+            L = fmaf(ml.y, f, L);
+            const uint32_t here = min(32u, count - i0);
+#pragma unroll 4
+            for (uint32_t i = 0; i < here; i++) {
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+                const float* p = A.part_o + part_at(x, i0 + i) * HD + lane * V;
+                if (V == 4) {
+                    const float4 v = __ldcg((const float4*)p);
+                    acc[0] = fmaf(v.x, fi, acc[0]); acc[1] = fmaf(v.y, fi, acc[1]); acc[V - 2] = fmaf(v.z, fi, acc[V - 2]); acc[V - 1] = fmaf(v.w, fi, acc[V - 1]);
+                } else {
+                    const float2 v = __ldcg((const float2*)p);
+                    acc[0] = fmaf(v.x, fi, acc[0]); acc[1] = fmaf(v.y, fi, acc[1]);
+                }
+            }
+        }
+        L = warp_sum(L);
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;      // a row that sees nothing: zeros
+        uint32_t* out = (uint32_t*)(A.out + (size_t)row * HD + lane * V);
+        if (V == 4) *(uint2*)out = make_uint2(pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[V - 2] * inv, acc[V - 1] * inv));
+        else *out = pack2<BF>(acc[0] * inv, acc[1] * inv);
+        return;
+    }
+    __shared__ float2 norm[MAX_ROWS];       // {maximum, 1 / sum} of the rows of the key head
+    const uint32_t u = blockIdx.x - row_blocks, p0 = (u % chunks) * W_CHUNK, h = (u / chunks) % A.kv_heads, b = u / chunks / A.kv_heads;
+    const uint32_t n = tail_length(A, b), rows = A.q_len * A.rep;
+    if (p0 >= n) return;
+    for (uint32_t r = warp; r < rows; r += 8) {
+        const RowParts x = row_parts(A, b * A.q_len + r / A.rep, h * A.rep + r % A.rep);
+        const uint32_t count = x.p_count + x.t_count;
+        float M = -INFINITY, L = 0.0f;
+        for (uint32_t i = lane; i < count; i += 32) M = fmaxf(M, __ldcg(&A.part_ml[part_at(x, i)]).x);
+        M = warp_max(M);
+        for (uint32_t i = lane; i < count; i += 32) {
+            const float2 ml = __ldcg(&A.part_ml[part_at(x, i)]);
+            L = fmaf(ml.y, part_factor(ml, M), L);
+        }
+        L = warp_sum(L);
+        if (lane == 0) norm[r] = make_float2(M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L);
+    }
+    __syncthreads();
+    const size_t head = (size_t)b * A.kv_heads + h;
+    for (uint32_t p = p0 + threadIdx.x; p < min(n, p0 + W_CHUNK); p += 256) {
+        float sum = A.weights_in ? A.weights_in[head * A.nslots + p] : 0.0f;
+        float add = 0.0f;
+        for (uint32_t r = 0; r < rows; r++) add = fmaf(sm100::ex2(__ldcg(&A.scores[(head * rows + r) * A.nslots + p]) - norm[r].x), norm[r].y, add);
+        A.weights[head * A.nslots + p] = sum + add;
+    }
+}
+
+template <bool BF, int HD, int RT>
+bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, bool tails) {
+    static int have[64] = {};
+    const size_t smem = parts_smem<HD, RT>();
+    if (!ensure_dyn_smem(shared_parts_kernel<BF, HD, RT>, smem, have)) return false;
+    const uint32_t fit = RT == 8 ? 1 : HD == 128 ? 2 : 3;
+    const size_t items = prefix_items + (tails ? ((size_t)a.t_slices + a.batch) * a.kv_heads : 0);
+    if (!items) return true;
+    g_launches++;
+    return launch_pdl(shared_parts_kernel<BF, HD, RT>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * fit)), dim3(RT == 8 ? 256 : 128), smem, st, a,
+                      prefix_items, tails ? 1u : 0u) == cudaSuccess;
+}
+template <bool BF, int HD>
+bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t prefix_items, bool tails) {
+    switch (rt) {
+        case 1: return launch_parts<BF, HD, 1>(st, a, prefix_items, tails);
+        case 2: return launch_parts<BF, HD, 2>(st, a, prefix_items, tails);
+        case 4: return launch_parts<BF, HD, 4>(st, a, prefix_items, tails);
+        default: return launch_parts<BF, HD, 8>(st, a, prefix_items, tails);
+    }
+}
+template <bool BF, int HD>
+bool launch_merge(cudaStream_t st, const SharedArgs& a) {
+    const size_t rows = (size_t)a.batch * a.q_len * a.kv_heads * a.rep;
+    const uint32_t chunks = (a.nslots + W_CHUNK - 1) / W_CHUNK;
+    const size_t blocks = (rows + 7) / 8, more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
+    g_launches++;
+    return launch_pdl(shared_merge_kernel<BF, HD>, dim3((uint32_t)(blocks + more)), dim3(256), 0, st, a, (uint32_t)blocks, std::max(1u, chunks)) == cudaSuccess;
+}
+
+uint32_t row_tiles(size_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
+
+struct Layout { size_t ml, o, scores, total; uint32_t t_rt, p_rt; };
+
+// How a call's work is cut and where its partial results lie. false: sizes the kernels do not take.
+bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, Layout& l, const char** why) {
+    *why = "attn shared: bad shape";
+    if (!a.batch || !a.q_len || !n_heads || !a.kv_heads || n_heads % a.kv_heads) return false;
+    *why = "attn shared: head_dim is 64 or 128";
+    if (hd != 64 && hd != 128) return false;
+    a.rep = n_heads / a.kv_heads;
+    *why = "attn shared: up to 1024 sequences, 16 new tokens and 128 rows (q_len * n_heads / kv_heads) to a key head, 65536 (sequence, key head) pairs";
+    if (a.batch > MAX_BATCH || a.q_len > MAX_Q || (size_t)a.q_len * a.rep > MAX_ROWS || (size_t)a.batch * a.kv_heads > 65536) return false;
+    *why = "attn shared: up to 2^30 prefix positions and 2^24 slots";
+    if (a.n_prefix > (1u << 30) || a.nslots > (1u << 24)) return false;
+    *why = "attn shared: weights of tails that have no slots";
+    if (with_weights && !a.nslots) return false;
+    const size_t tokens = (size_t)a.batch * a.q_len, rows = tokens * a.rep;
+    l.t_rt = row_tiles((size_t)a.q_len * a.rep);
+    l.p_rt = std::max(l.t_rt, row_tiles(rows));
+    a.p_tokens = (uint32_t)std::min<size_t>(tokens, l.p_rt * 16 / a.rep);
+    a.p_tiles = (uint32_t)((tokens + a.p_tokens - 1) / a.p_tokens);
+    const uint32_t fit = SMS * (l.p_rt == 8 ? 1 : 2), groups = a.p_tiles * a.kv_heads;
+    const uint32_t tiles = (a.n_prefix + TILE - 1) / TILE;
+    a.p_slices = a.p_len = 0;
+    if (tiles) {
+        const uint32_t want = std::min(tiles, std::max(1u, fit / groups));
+        a.p_len = (tiles + want - 1) / want * TILE;
+        a.p_slices = (a.n_prefix + a.p_len - 1) / a.p_len;
+    }
+    a.t_slices = std::max(1u, 6 * SMS / a.kv_heads);
+    const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    l.ml = up((size_t)(a.batch + 1) * 4);
+    l.o = l.ml + up(parts * 8);
+    l.scores = l.o + up(parts * hd * 4);
+    l.total = l.scores + (with_weights ? up((size_t)a.batch * a.kv_heads * a.q_len * a.rep * a.nslots * 4) : 0);
+    return true;
+}
+
+}  // namespace
+
+bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t rt, bool prefix, bool tails) {
+    const uint32_t items = prefix ? a.p_tiles * a.kv_heads * a.p_slices : 0;
+    if (hd == 128) return bf16 ? launch_parts_rt<true, 128>(st, a, rt, items, tails) : launch_parts_rt<false, 128>(st, a, rt, items, tails);
+    return bf16 ? launch_parts_rt<true, 64>(st, a, rt, items, tails) : launch_parts_rt<false, 64>(st, a, rt, items, tails);
+}
+bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16) {
+    if (hd == 128) return bf16 ? launch_merge<true, 128>(st, a) : launch_merge<false, 128>(st, a);
+    return bf16 ? launch_merge<true, 64>(st, a) : launch_merge<false, 64>(st, a);
+}
+
+bool on_this_device(const void* p, const char* what) {
+    int dev = -1;
+    cudaPointerAttributes at;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaPointerGetAttributes(&at, p) == cudaSuccess &&
+        (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev)))
+        return true;
+    cudaGetLastError();
+    g.last_error = std::string(what) + " is no memory of the current device";
+    return false;
+}
+
+}  // namespace gehtp
+
+using namespace gehtp;
+
+extern "C" size_t gehtp_attn_shared_workspace(uint32_t batch, uint32_t q_len, uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim,
+                                              uint32_t n_prefix, uint32_t nslots, int with_weights) {
+    SharedArgs a{};
+    a.batch = batch; a.q_len = q_len; a.kv_heads = kv_heads; a.n_prefix = n_prefix; a.nslots = nslots;
+    Layout l;
+    const char* why;
+    if (!lay_out(a, n_heads, head_dim, with_weights != 0, l, &why)) { g.last_error = why; return 0; }
+    return l.total;
+}
+
+extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, const void* tail_dev, const int32_t* n_tail_dev,
+                                 const float* weights_in_dev, float* weights_dev, void* out_dev, uint32_t batch, uint32_t q_len,
+                                 uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_stride, uint32_t n_prefix,
+                                 uint32_t nslots, uint32_t dtype, float scale, void* workspace_dev, size_t workspace_bytes, void* stream) {
+    auto fail = [](const char* m) { g.last_error = m; return -1; };
+    SharedArgs a{};
+    a.batch = batch; a.q_len = q_len; a.kv_heads = kv_heads; a.n_prefix = n_prefix; a.nslots = nslots;
+    Layout l;
+    const char* why;
+    if (!lay_out(a, n_heads, head_dim, weights_dev != nullptr, l, &why)) return fail(why);
+    if (dtype != GEHTP_DT_F16 && dtype != GEHTP_DT_BF16) return fail("attn shared: element type is GEHTP_DT_F16 or GEHTP_DT_BF16");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail("attn shared: scale is a positive number");
+    if (!q_dev || !out_dev || !workspace_dev || (n_prefix && !prefix_dev) || (nslots && (!tail_dev || !n_tail_dev))) return fail("attn shared: null pointer");
+    if (weights_in_dev && !weights_dev) return fail("attn shared: weights_in without weights");
+    if (q_stride < (size_t)n_heads * head_dim || q_stride % 8) return fail("attn shared: q_stride is a multiple of 8, n_heads * head_dim at least");
+    if ((((uintptr_t)q_dev) | ((uintptr_t)(n_prefix ? prefix_dev : nullptr)) | ((uintptr_t)(nslots ? tail_dev : nullptr)) | ((uintptr_t)out_dev)) & 15u)
+        return fail("attn shared: q, prefix, tail and out lie on 16-byte boundaries");
+    if ((uintptr_t)workspace_dev & 255u) return fail("attn shared: the workspace lies on a 256-byte boundary");
+    if ((((uintptr_t)n_tail_dev) | ((uintptr_t)weights_in_dev) | ((uintptr_t)weights_dev)) & 3u) return fail("attn shared: n_tail and weights lie on 4-byte boundaries");
+    if (workspace_bytes < l.total) {
+        char m[128];
+        std::snprintf(m, sizeof m, "attn shared: needs %zu bytes of workspace, got %zu", l.total, workspace_bytes);
+        return fail(m);
+    }
+    if (!on_this_device(q_dev, "attn shared: q") || !on_this_device(out_dev, "attn shared: out") || !on_this_device(workspace_dev, "attn shared: workspace") ||
+        (n_prefix && !on_this_device(prefix_dev, "attn shared: prefix")) ||
+        (nslots && (!on_this_device(tail_dev, "attn shared: tail") || !on_this_device(n_tail_dev, "attn shared: n_tail"))) ||
+        (weights_dev && !on_this_device(weights_dev, "attn shared: weights")) || (weights_in_dev && !on_this_device(weights_in_dev, "attn shared: weights_in")))
+        return -1;
+    a.q = (const uint16_t*)q_dev; a.prefix = (const uint16_t*)prefix_dev; a.tail = (const uint16_t*)tail_dev; a.n_tail = n_tail_dev;
+    a.weights_in = weights_in_dev; a.weights = weights_dev; a.out = (uint16_t*)out_dev; a.q_stride = q_stride;
+    a.sc = scale * 1.4426950408889634f;
+    unsigned char* ws = (unsigned char*)workspace_dev;
+    a.plan = (uint32_t*)ws; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
+    a.scores = weights_dev ? (float*)(ws + l.scores) : nullptr;
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool bf = dtype == GEHTP_DT_BF16, one = l.p_rt == l.t_rt;
+    bool ok = true;
+    if (n_prefix && !one) ok = k_shared_parts(st, a, head_dim, bf, l.p_rt, true, false);
+    if (ok && (nslots || (n_prefix && one))) ok = k_shared_parts(st, a, head_dim, bf, l.t_rt, n_prefix && one, nslots != 0);
+    if (ok) ok = k_shared_merge(st, a, head_dim, bf);
+    if (!ok) {
+        const cudaError_t e = cudaGetLastError();
+        return fail(e == cudaSuccess ? "attn shared: launch refused" : cudaGetErrorString(e));
+    }
+    return 0;
+}

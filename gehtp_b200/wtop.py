@@ -16,7 +16,7 @@ SLOT_EXT_IN, SLOT_EXT_OUT, SLOT_TEMPOFF = 0xFFFFFFFF, 0xFFFFFFFE, 0xFFFFFFFD
 SLOT_EXT_WGT, SLOT_STATE, KV_POS_AUTO = 0xFFFFFFFC, 0xFFFFFFFB, 0xFFFFFFFA
 # row-count runlists (this executor's own): limits slot, and the row arguments that follow the run
 SLOT_ROWS, ROWS_AUTO, SEL_AUTO = 0xFFFFFFF7, 0xFFFFFFF9, 0xFFFFFFF8
-DT_F32, DT_BF16 = 0, 1
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 LIN_X_BF16, LIN_Y_BF16, LIN_RELU2, LIN_GELU_GATE = 1, 2, 16, 32
 COL_ALIGN = 8
 
@@ -256,6 +256,9 @@ def bind(lib):
         lib.gehtp_dev_w4a16_swiglu.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32, u32]
         lib.gehtp_dev_rmsnorm.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32]
         lib.gehtp_cuda_capture_end_replay.argtypes = [c.c_int, P(c.c_float)]
+        lib.gehtp_attn_shared_workspace.argtypes = [u32] * 7 + [c.c_int]
+        lib.gehtp_attn_shared_workspace.restype = c.c_size_t
+        lib.gehtp_attn_shared.argtypes = [vp] * 7 + [u32] * 9 + [c.c_float, vp, c.c_size_t, vp]
         lib.gehtp_attn_decode_noalloc.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_void_p, c.c_uint32, c.c_uint32,
                                                   c.c_uint32, c.c_uint32, c.c_uint32, c.c_float, c.c_void_p]
     return lib

@@ -330,6 +330,45 @@ int gehtp_attn_decode_noalloc(const uint16_t* q_dev, const uint16_t* ring_dev, c
  * -1 = the copy failed. Call it after synchronising the stream the calls were queued on. */
 int gehtp_attn_decode_noalloc_status(void);
 
+/* ------------------------------------- several sequences from one prompt
+ * No counterparts in the reference. Operators for a batch of sequences that go on from one prompt: attention over the
+ * prompt's cache, held once for all, and a cache of each sequence's own; eviction from those own caches; verification of drafted
+ * tokens. As gehtp_attn_decode_noalloc they take device pointers of the caller, queue their work on `stream` (a cudaStream_t, NULL =
+ * default stream) of the current device and wait for nothing. They allocate nothing and keep nothing between calls: partial
+ * results go to a workspace of the caller, on a 256-byte boundary, of the size that the _workspace function gives for the
+ * same sizes (0: sizes the operator does not take, gehtp_cuda_last_error says why). What is in it before a call does not
+ * matter and nothing has to be kept of it. Calls that may overlap on the GPU need a workspace each, and so do captured graphs that
+ * may be replayed at the same time. Return value: 0, or -1 with gehtp_cuda_last_error; after -1 nothing has been queued unless the
+ * message is one of the CUDA runtime's. */
+
+/* Element types: WT_DT_F32, WT_DT_BF16 and fp16. */
+#define GEHTP_DT_F32   0u
+#define GEHTP_DT_BF16  1u
+#define GEHTP_DT_F16   2u
+
+/* out = softmax(q . K * scale) . V over the n_prefix positions that all sequences share and over the tail of each one's own.
+ *   q        [batch][q_len] rows, q_stride elements apart (a multiple of 8), of n_heads * head_dim elements: q_len new tokens each;
+ *            head h reads key head h / (n_heads / kv_heads)
+ *   prefix   [n_prefix][K: kv_heads * head_dim | V: the same], a KV ring of one sequence that has not wrapped (NULL with n_prefix = 0)
+ *   tail     [nslots][K: batch * kv_heads * head_dim | V: the same], the KV ring of a decode batch; position p of a sequence's tail lies
+ *            in slot p (NULL with nslots = 0: no tails)
+ *   n_tail   [batch] positions in each tail, the new tokens' own included (appended before the call); read on the device, values outside
+ *            0 .. nslots count as the nearer of the two. New token t sees the tail's first n_tail - q_len + t + 1 positions.
+ *            What lies in slots from n_tail on is never read.
+ *   weights  NULL, or fp32 [batch][kv_heads][nslots]: position p < n_tail gets weights_in[p] + the softmax weight that the key head's
+ *            q_len * n_heads / kv_heads rows give it, positions from n_tail on are left as they are. weights_in: NULL stands for zeros;
+ *            may be `weights` itself, but not overlap it otherwise
+ *   out      [batch][q_len][n_heads][head_dim]; a row that sees no position at all is zeros
+ * q, prefix, tail and out are of type `dtype` (GEHTP_DT_F16 or GEHTP_DT_BF16), on 16-byte boundaries; out and weights overlap no input
+ * otherwise. Scores, softmax and sums are fp32. head_dim 64 or 128, batch up to 1024, q_len up to 16, q_len * n_heads / kv_heads up to
+ * 128, scale > 0. */
+size_t gehtp_attn_shared_workspace(uint32_t batch, uint32_t q_len, uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim,
+                                   uint32_t n_prefix, uint32_t nslots, int with_weights);
+int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, const void* tail_dev, const int32_t* n_tail_dev,
+                      const float* weights_in_dev, float* weights_dev, void* out_dev, uint32_t batch, uint32_t q_len,
+                      uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_stride, uint32_t n_prefix,
+                      uint32_t nslots, uint32_t dtype, float scale, void* workspace_dev, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

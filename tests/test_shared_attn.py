@@ -1,0 +1,237 @@
+"""Attention over a shared prefix and own tails (gehtp_attn_shared) against the formula in 64 bits.
+
+Tolerance of an output component, from the roundings on the way to it, with A = sum p |v| of that component:
+  eps/2 |out|                 the result's own rounding
+  eps_p A                     the weights as matrix operands: fp16 2^-11; bf16 in two terms 2^-16
+  2 e_s A                     the scores, once in the weight and once in the sum: head_dim fp32 additions of products whose magnitudes
+                              sum up to S = scale * max_j sum |q k_j|, each off by 2^-23 of that at most, and the product with the scale
+  2^-19 A                     the exponentials (2^-22) and the sums of weights and of partial results
+  N 2^-24 max|v|              weights that fp16 holds with fewer bits (below 2^-14), N positions, against a sum of at least 1
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+from gehtp_b200.wtop import DT_BF16, DT_F16, DT_F32
+
+P = ctypes.c_void_p
+
+
+def formula(q, prefix, tail, n_tail, scale):
+    """q [b][t][h][d], prefix [P][2][kvh][d], tail [n][2][b * kvh][d] in 64 bits: out, its tolerance base A, S, weights of the tails."""
+    import torch
+    b, t, h, d = q.shape
+    kvh = prefix.shape[2]
+    rep = h // kvh
+    out, mag = torch.zeros(b, t, h, d, dtype=torch.float64), torch.zeros(b, t, h, d, dtype=torch.float64)
+    weights = torch.zeros(b, kvh, tail.shape[0], dtype=torch.float64)
+    top = torch.zeros(b, t, h, 1, dtype=torch.float64)
+    for i in range(b):
+        for x in range(h):
+            k = x // rep
+            for y in range(t):
+                n = max(0, int(n_tail[i]) - t + y + 1)
+                keys = torch.cat([prefix[:, 0, k], tail[:n, 0, i * kvh + k]])
+                values = torch.cat([prefix[:, 1, k], tail[:n, 1, i * kvh + k]])
+                if not len(keys):
+                    continue
+                p = torch.softmax(keys @ q[i, y, x] * scale, 0)
+                out[i, y, x], mag[i, y, x] = p @ values, p @ values.abs()
+                top[i, y, x] = (keys.abs() @ q[i, y, x].abs()).max() * scale
+                weights[i, k, :n] += p[len(prefix):]
+    return out, mag, top, weights
+
+
+def tolerance(out, mag, top, values, positions, dtype, d):
+    import torch
+    half, eps_p = (2.0 ** -11, 2.0 ** -11) if dtype == torch.float16 else (2.0 ** -8, 2.0 ** -16)
+    tol = half * out.abs() + mag * (eps_p + 2 * top * (d + 2) * 2.0 ** -23 + 2.0 ** -19)
+    return tol + (positions * 2.0 ** -24 * values.abs().max() + 2.0 ** -25 if dtype == torch.float16 else 1e-30)
+
+
+class Call:
+    """Operands of a call on the GPU; slots behind a tail's end hold NaN."""
+
+    def __init__(self, batch, q_len, heads, kv_heads, d, prefix, slots, n_tail, dtype, weights=False, pad=0, seed=0):
+        import torch
+        g = torch.Generator().manual_seed(seed)
+        self.shape, self.slots, self.n_prefix, self.dtype, self.scale = (batch, q_len, heads, kv_heads, d), slots, prefix, dtype, 1.0 / np.sqrt(d)
+        r = lambda *s: torch.randn(*s, generator=g)
+        self.stride = heads * d + pad
+        rows = r(batch * q_len, self.stride)
+        keys = torch.exp(0.7 * r(prefix + slots, 1, 1, 1))
+        pre, tail = r(prefix, 2, kv_heads, d), r(slots, 2, batch * kv_heads, d)
+        pre[:, 0] *= keys[:prefix, 0]
+        tail[:, 0] *= keys[prefix:, 0]
+        self.n = torch.tensor(n_tail, dtype=torch.int32)
+        real = self.n.clamp(0, slots)
+        for b in range(batch):
+            tail.view(slots, 2, batch, kv_heads, d)[real[b]:, :, b] = float("nan")
+        self.rows, self.prefix, self.tail = (x.to(dtype).cuda() for x in (rows, pre, tail))
+        self.n_dev = self.n.cuda()
+        self.out = torch.full((batch, q_len, heads, d), 7.0, dtype=dtype, device="cuda")
+        self.w_in = torch.rand(batch, kv_heads, slots, generator=g).cuda() if weights else None
+        self.w = torch.full_like(self.w_in, -5.0) if weights else None
+
+    def size(self, lib):
+        return lib.gehtp_attn_shared_workspace(*self.shape, self.n_prefix, self.slots, int(self.w is not None))
+
+    def workspace(self, lib):
+        import torch
+        self.ws = torch.full((self.size(lib),), 255, dtype=torch.uint8, device="cuda")      # 255: every float in it NaN
+
+    def run(self, lib, stream=None, w_in="own"):
+        import torch
+        a = lambda t: t.data_ptr() if t is not None and t.numel() else None
+        if not hasattr(self, "ws"):
+            self.workspace(lib)
+        dt = DT_F16 if self.dtype == torch.float16 else DT_BF16
+        rc = lib.gehtp_attn_shared(a(self.rows), a(self.prefix), a(self.tail), a(self.n_dev) if self.slots else None, a(self.w_in) if w_in == "own" else w_in,
+                                   a(self.w), a(self.out), *self.shape, self.stride, self.n_prefix, self.slots, dt, self.scale, a(self.ws), self.ws.numel(),
+                                   stream if stream is not None else torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, lib.gehtp_cuda_last_error()
+
+    def check(self):
+        import torch
+        torch.cuda.synchronize()
+        b, t, h, kvh, d = self.shape
+        q = self.rows.cpu().double()[:, :h * d].reshape(b, t, h, d)
+        n = self.n.clamp(0, self.slots)
+        tail = torch.nan_to_num(self.tail.cpu().double())
+        want, mag, top, weights = formula(q, self.prefix.cpu().double(), tail, n, self.scale)
+        values = torch.cat([self.prefix.cpu()[:, 1].reshape(-1), tail[:, 1].reshape(-1).to(self.dtype), torch.zeros(1, dtype=self.dtype)]).double()
+        tol = tolerance(want, mag, top, values, self.n_prefix + self.slots, self.dtype, d)
+        got = self.out.cpu().double()
+        assert torch.isfinite(got).all()
+        off = (got - want).abs() - tol
+        assert (off <= 0).all(), "%g over the tolerance at %s" % (off.max(), np.unravel_index(int(off.argmax()), off.shape))
+        if self.w is not None:
+            for i in range(b):
+                assert (self.w[i, :, int(n[i]):] == -5.0).all()
+                w, x = self.w[i, :, :int(n[i])].cpu().double(), self.w_in[i, :, :int(n[i])].cpu().double()
+                rel = 2 * top[i].max() * (d + 2) * 2.0 ** -23 + 2.0 ** -19
+                assert ((w - x - weights[i, :, :int(n[i])]).abs() <= weights[i, :, :int(n[i])] * rel + w.abs() * 2.0 ** -23 + 1e-30).all()
+
+
+CASES = [
+    # batch, q_len, heads, kv_heads, d, prefix, slots, n_tail
+    (1, 1, 1, 1, 64, 1, 0, [0]),
+    (1, 1, 4, 4, 128, 1, 1, [1]),
+    (2, 1, 4, 2, 128, 0, 5, [0, 5]),                        # a sequence that sees nothing
+    (3, 4, 14, 2, 64, 65, 70, [0, 3, 70]),                  # fewer positions than new tokens, groups of seven
+    (3, 4, 14, 2, 64, 0, 70, [2, 3, 64]),                   # rows that see nothing
+    (2, 1, 16, 1, 128, 63, 64, [64, 63]),
+    (2, 16, 8, 1, 128, 130, 200, [16, 200]),                # 128 rows to a key head
+    (1, 1, 71, 1, 64, 129, 129, [129]),
+    (5, 2, 20, 4, 64, 1000, 333, [1, 64, 65, 128, 333]),
+    (40, 1, 8, 1, 128, 300, 20, [i % 21 for i in range(40)]),
+    (70, 5, 6, 2, 64, 127, 9, [i % 10 for i in range(70)]),
+    (4, 1, 32, 8, 128, 2049, 3000, [3000, 1, 64, 1777]),
+    (9, 8, 12, 4, 128, 513, 100, [-3, 1000, 8, 7, 9, 100, 64, 72, 71]),      # lengths outside the cache count as its ends
+    (130, 1, 2, 2, 64, 40, 300, [300 if i == 77 else 2 for i in range(130)]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c[:7])))
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_against_the_formula(cuda, case, dtype):
+    import torch
+    call = Call(*case, dtype=getattr(torch, dtype), weights=case[6] > 0, pad=24, seed=len(case[7]) + case[5])
+    call.run(cuda)
+    call.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix,rows", [(96, 1), (1500, 40)])
+def test_again_and_without_given_weights(cuda, prefix, rows):
+    """The same bits every time; weights_in NULL stands for zeros; in place adds up."""
+    import torch
+    call = Call(rows, 3, 8, 2, 128, prefix, 150, [(37 * i) % 151 for i in range(rows)], torch.bfloat16, weights=True)
+    call.run(cuda, w_in=None)
+    torch.cuda.synchronize()
+    first = call.out.clone(), call.w.clone()
+    for _ in range(5):
+        call.ws.fill_(255)
+        call.run(cuda, w_in=None)
+        torch.cuda.synchronize()
+        assert torch.equal(first[0].view(torch.int16), call.out.view(torch.int16)) and torch.equal(first[1], call.w)
+    call.run(cuda, w_in=call.w.data_ptr())
+    torch.cuda.synchronize()
+    live = first[1] != -5.0
+    assert torch.equal(call.w[live], 2 * first[1][live]) and (call.w[~live] == -5.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_a_position_that_is_no_number(cuda, dtype):
+    """It makes no number of the rows that see it and of no others: not of earlier tokens, not of other sequences."""
+    import torch
+    call = Call(3, 5, 8, 2, 128, 100, 90, [80, 70, 90], getattr(torch, dtype), weights=True)
+    call.run(cuda)
+    torch.cuda.synchronize()
+    clean = call.out.clone()
+    call.tail.view(90, 2, 3, 2, 128)[72, :, 0] = float("nan")        # the last but seven of the first sequence: seen by all its rows
+    call.tail.view(90, 2, 3, 2, 128)[68, 1, 1, 0, 5] = float("inf")  # the second's last but one, a value: rows of the last two tokens
+    call.tail.view(90, 2, 3, 2, 128)[88, 0, 2] = float("nan")        # the third's last but one, its key
+    call.run(cuda)
+    torch.cuda.synchronize()
+    assert not torch.isfinite(call.out[0]).any()
+    assert torch.equal(call.out[1, :3], clean[1, :3]) and torch.equal(call.out[2, :3], clean[2, :3])
+    assert not torch.isfinite(call.out[1, 3:, :4, 5]).any() and torch.equal(call.out[1, 3:, 4:], clean[1, 3:, 4:])
+    assert not torch.isfinite(call.out[2, 3:]).any()
+
+
+@pytest.mark.gpu
+def test_captured_replayed_and_on_two_streams(cuda):
+    """Lengths are read when the graph runs; calls on two streams with a workspace each."""
+    import torch
+    a = Call(6, 2, 8, 4, 128, 700, 200, [200, 1, 2, 64, 90, 3], torch.float16, weights=True)
+    b = Call(33, 1, 16, 2, 64, 1200, 80, [(7 * i) % 81 for i in range(33)], torch.bfloat16, seed=4)
+    a.run(cuda), b.run(cuda)
+    torch.cuda.synchronize()
+    want = a.out.clone(), a.w.clone(), b.out.clone()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for call, s in zip((a, b), streams):
+            call.run(cuda, s.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(a.out, want[0]) and torch.equal(a.w, want[1]) and torch.equal(b.out, want[2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        a.run(cuda, streams[0].cuda_stream)
+    for seed in range(3):
+        a.n = torch.tensor([(50 * seed + 31 * i) % 201 for i in range(6)], dtype=torch.int32)
+        c = Call(6, 2, 8, 4, 128, 700, 200, a.n.tolist(), torch.float16, weights=True, seed=10 + seed)
+        for x, y in ((a.rows, c.rows), (a.prefix, c.prefix), (a.tail, c.tail), (a.n_dev, c.n_dev), (a.w_in, c.w_in), (a.w, c.w)):
+            x.copy_(y)
+        graph.replay()
+        a.check()
+
+
+def test_workspace_refuses_what_the_call_refuses(cuda):
+    ws = lambda *s: cuda.gehtp_attn_shared_workspace(*s)
+    assert ws(2, 1, 16, 8, 128, 512, 64, 1) > ws(2, 1, 16, 8, 128, 512, 64, 0) > 0
+    for bad in ((0, 1, 16, 8, 128, 512, 64, 0), (2, 0, 16, 8, 128, 512, 64, 0), (2, 1, 15, 8, 128, 512, 64, 0), (2, 1, 16, 0, 128, 512, 64, 0),
+                (2, 1, 16, 8, 96, 512, 64, 0), (1025, 1, 16, 8, 128, 512, 64, 0), (2, 17, 16, 8, 128, 512, 64, 0), (2, 16, 9, 1, 128, 512, 64, 0),
+                (2, 1, 16, 8, 128, 512, 0, 1), (2, 1, 16, 8, 128, (1 << 30) + 1, 64, 0), (2, 1, 16, 8, 128, 0, (1 << 24) + 1, 0), (1024, 1, 65, 65, 64, 1, 0, 0)):
+        assert ws(*bad) == 0 and b"attn shared" in cuda.gehtp_cuda_last_error()
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(ws=None), b"null"), (dict(prefix=None), b"null"), (dict(tail=None), b"null"),
+    (dict(n_tail=None), b"null"), (dict(w=None), b"weights_in"), (dict(q=8), b"16-byte"), (dict(tail=8), b"16-byte"), (dict(ws=64), b"256-byte"),
+    (dict(n_tail=2), b"4-byte"), (dict(stride=1024), b"q_stride"), (dict(stride=2052), b"q_stride"), (dict(dt=DT_F32), b"element type"),
+    (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"),
+    (dict(size=1000), b"workspace"), (dict(heads=24, kv=16), b"shape"), (dict(), b"no memory of the current device"),
+])
+def test_refusals(cuda, change, message):
+    """Host memory in every place: a call that got as far as its pointers says so, and nothing is queued."""
+    buf = np.zeros(1 << 16, np.uint8)
+    base = (buf.ctypes.data + 255) // 256 * 256
+    at = lambda k: None if k in change and change[k] is None else base + change.get(k, 0)
+    heads, kv = change.get("heads", 16), change.get("kv", 8)
+    rc = cuda.gehtp_attn_shared(at("q"), at("prefix"), at("tail"), at("n_tail"), base, at("w"), at("out"), 2, 1, heads, kv, 128, change.get("stride", 2048), 512, 64,
+                                change.get("dt", DT_F16), change.get("scale", 0.1), at("ws"), change.get("size", 1 << 40), None)
+    assert rc == -1 and message in cuda.gehtp_cuda_last_error()
