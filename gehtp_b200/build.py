@@ -48,6 +48,8 @@ UNITS = {
     "channel_delta.cu": [],
     "channel_chunks.cu": [],
     "shared_attn.cu": [],
+    "kv_evict.cu": [],
+    "verify_drafts.cu": [],
     "tp.cu": [],
     "tp_p2p.cu": [],
 }

@@ -259,6 +259,12 @@ def bind(lib):
         lib.gehtp_attn_shared_workspace.argtypes = [u32] * 7 + [c.c_int]
         lib.gehtp_attn_shared_workspace.restype = c.c_size_t
         lib.gehtp_attn_shared.argtypes = [vp] * 7 + [u32] * 9 + [c.c_float, vp, c.c_size_t, vp]
+        lib.gehtp_kv_evict_workspace.argtypes = [u32] * 7
+        lib.gehtp_kv_evict_workspace.restype = c.c_size_t
+        lib.gehtp_kv_evict.argtypes = [vp] * 7 + [u32] * 7 + [vp, c.c_size_t, vp]
+        lib.gehtp_verify_drafts_workspace.argtypes = [u32] * 3
+        lib.gehtp_verify_drafts_workspace.restype = c.c_size_t
+        lib.gehtp_verify_drafts.argtypes = [vp] * 7 + [u32] * 6 + [c.c_double, vp, c.c_size_t, vp]
         lib.gehtp_attn_decode_noalloc.argtypes = [c.c_void_p, c.c_void_p, c.c_void_p, c.c_void_p, c.c_uint32, c.c_uint32,
                                                   c.c_uint32, c.c_uint32, c.c_uint32, c.c_float, c.c_void_p]
     return lib

@@ -369,6 +369,48 @@ int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, const void* tai
                       uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_stride, uint32_t n_prefix,
                       uint32_t nslots, uint32_t dtype, float scale, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* Cuts caches down to their positions of greatest weight. A sequence with more than `keep` positions keeps, for every key head on its
+ * own, its first `sinks` positions, its last `recent` and, of those between, the ones of greatest weight (of equal weights the lower
+ * position; a weight that is no number counts as less than any other); they move up in their order to slots 0 .. keep - 1. Rotary
+ * embedding is part of the cached keys, so what stays keeps the angle of its old position. A sequence with no more than
+ * `keep` keeps them all.
+ *   ring     [nslots][K: batch * kv_heads * head_dim | V: the same], 16-bit elements, position p in slot p; ring_out the same: `ring` itself
+ *            (in place) or memory that does not overlap it. Slots of ring_out behind a sequence's new length are left as they are.
+ *   weights  fp32 [batch][kv_heads][nslots], moved with the positions; weights_out: `weights` itself or memory apart from it. Behind
+ *            the new length it is left as it is; in place, zeros are written from there to the old length, so that slots filled
+ *            again begin without weight.
+ *   n, n_out [batch] lengths before and after (n_out may be n); read on the device, values outside 0 .. nslots count as the nearer one
+ *   kept     NULL, or int32 [batch][kv_heads][keep]: the old positions of what stayed, -1 behind them
+ * head_dim is a multiple of 8 up to 512. */
+size_t gehtp_kv_evict_workspace(uint32_t batch, uint32_t kv_heads, uint32_t head_dim, uint32_t nslots, uint32_t keep,
+                                uint32_t sinks, uint32_t recent);
+int gehtp_kv_evict(const void* ring_dev, void* ring_out_dev, const float* weights_dev, float* weights_out_dev,
+                   const int32_t* n_dev, int32_t* n_out_dev, int32_t* kept_dev, uint32_t batch, uint32_t kv_heads,
+                   uint32_t head_dim, uint32_t nslots, uint32_t keep, uint32_t sinks, uint32_t recent,
+                   void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* Holds drafted tokens against the target's probabilities and draws the token behind the accepted ones, from given random numbers.
+ * p_i = softmax(target_i / temperature), q_i = softmax(draft_i / temperature). Draft i of a sequence is accepted while
+ * uniforms[i] * q_i(token_i) < p_i(token_i). At the first place that is not accepted the token is drawn from max(p_i - q_i, 0) (from p_i
+ * where its sum is below 1e-12: rows that are alike), behind n accepted ones from p_n: the first token whose cumulated share is above
+ * uniforms[n_drafts]. temperature 0: draft i is accepted while it is the lowest place of target_i's largest logit, and the token behind
+ * the accepted ones is that place; draft and uniforms are not read.
+ *   target   [batch][n_drafts + 1] rows of `vocab` logits, target_stride elements apart: row i is what follows draft i - 1
+ *   draft    [batch][n_drafts] rows, draft_stride apart, or NULL: drafts without probabilities (found by lookup, or chosen greedily),
+ *            for which q_i is 1 at the drafted token
+ *   tokens   int32 [batch][n_drafts]; an id outside the vocabulary is not accepted
+ *   n_drafts_dev  NULL, or int32 [batch]: drafts of each sequence, read on the device, values outside 0 .. n_drafts count as the nearer one
+ *   uniforms fp32 [batch][n_drafts + 1] in [0, 1): one for each draft, the last for the draw, whatever the number of drafts
+ *   accepted int32 [batch]; out int32 [batch][n_drafts + 1]: the accepted drafts, the token behind them, -1 in the rest
+ * A target row without a distribution (a logit that is no number or +inf, -inf throughout) accepts nothing and yields the token -1; a
+ * draft row without one is not accepted and takes nothing away from p. Logits of type `dtype`; -inf stands for a token that is ruled out.
+ * n_drafts 0 (no tokens, no draft) draws a token per sequence. Up to 64 drafts and 4096 sequences; temperature 0 or 1e-4 to 1e4. */
+size_t gehtp_verify_drafts_workspace(uint32_t batch, uint32_t n_drafts, uint32_t vocab);
+int gehtp_verify_drafts(const void* target_dev, const void* draft_dev, const int32_t* tokens_dev, const int32_t* n_drafts_dev,
+                        const float* uniforms_dev, int32_t* accepted_dev, int32_t* out_dev, uint32_t batch, uint32_t n_drafts,
+                        uint32_t vocab, uint32_t target_stride, uint32_t draft_stride, uint32_t dtype, double temperature,
+                        void* workspace_dev, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
