@@ -48,6 +48,7 @@ UNITS = {
     "channel_delta.cu": [],
     "channel_chunks.cu": [],
     "shared_attn.cu": [],
+    "shared_attn_sm100.cu": [],
     "kv_evict.cu": [],
     "verify_drafts.cu": [],
     "tp.cu": [],

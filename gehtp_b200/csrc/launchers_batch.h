@@ -26,12 +26,13 @@ struct SharedArgs {
     float2* part_ml;                               // [partial row] {m, sum}
     float* scores;                                 // s of every tail position: [sequence][key head][row][nslots], or NULL
     uint32_t* plan;                                // written by the first kernel: slices in front of each sequence's, batch + 1 of them
-    unsigned int* status;
     __host__ __device__ size_t p_rows() const { return (size_t)p_tiles * kv_heads * p_slices * p_tokens * rep; }
 };
 
 // false: launch failed
-bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t row_tiles, bool prefix, bool tails);
+bool k_shared_prefix_sm100(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16);
+// beside: behind the prefix's kernel in the stream, at the same time as it
+bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t row_tiles, bool prefix, bool tails, bool beside);
 bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16);
 
 // true: `p` is memory of the current device (or managed); else g.last_error says which argument is not

@@ -92,7 +92,7 @@ __host__ __device__ constexpr size_t parts_smem() { return ring_bytes<HD>() + (s
 // RT row tiles of 16; the warps that RT leaves share a tile's positions
 template <bool BF, int HD, int RT>
 __global__ void __launch_bounds__(RT == 8 ? 256 : 128, RT == 8 ? 1 : 2)
-shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails) {
+shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
     constexpr int NW = RT == 8 ? 8 : 4, NT = NW * 32, PG = NW / RT, NP = TILE / PG / 16, STG = stages<HD>(), LD = HD + 8;
     constexpr uint32_t ROW = HD * 2, HALF = TILE * ROW;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -104,8 +104,10 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
     const uint32_t rt = warp % RT, pg = warp / RT;
     const uint32_t ring = smem_addr(smem);
-    pdl_wait();
-    pdl_release();     // behind the wait: what starts now may read all that was there before this call
+    // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait: all that was there before the
+    // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
+    if (!beside) pdl_wait();
+    pdl_release();
     if (with_tails) {
         if (warp == 0) {
             const uint32_t k = cut_tails(A, cum);
@@ -341,6 +343,7 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
         }
         __syncthreads();
     }
+    if (beside) pdl_wait();
 }
 
 // Places of a row's partial results: `first` + i * step for i < count, of the prefix and of the tail.
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, u
 }
 
 template <bool BF, int HD, int RT>
-bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, bool tails) {
+bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, bool tails, bool beside) {
     static int have[64] = {};
     const size_t smem = parts_smem<HD, RT>();
     if (!ensure_dyn_smem(shared_parts_kernel<BF, HD, RT>, smem, have)) return false;
@@ -448,15 +451,15 @@ bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, b
     if (!items) return true;
     g_launches++;
     return launch_pdl(shared_parts_kernel<BF, HD, RT>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * fit)), dim3(RT == 8 ? 256 : 128), smem, st, a,
-                      prefix_items, tails ? 1u : 0u) == cudaSuccess;
+                      prefix_items, tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
 }
 template <bool BF, int HD>
-bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t prefix_items, bool tails) {
+bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t prefix_items, bool tails, bool beside) {
     switch (rt) {
-        case 1: return launch_parts<BF, HD, 1>(st, a, prefix_items, tails);
-        case 2: return launch_parts<BF, HD, 2>(st, a, prefix_items, tails);
-        case 4: return launch_parts<BF, HD, 4>(st, a, prefix_items, tails);
-        default: return launch_parts<BF, HD, 8>(st, a, prefix_items, tails);
+        case 1: return launch_parts<BF, HD, 1>(st, a, prefix_items, tails, beside);
+        case 2: return launch_parts<BF, HD, 2>(st, a, prefix_items, tails, beside);
+        case 4: return launch_parts<BF, HD, 4>(st, a, prefix_items, tails, beside);
+        default: return launch_parts<BF, HD, 8>(st, a, prefix_items, tails, beside);
     }
 }
 template <bool BF, int HD>
@@ -470,7 +473,7 @@ bool launch_merge(cudaStream_t st, const SharedArgs& a) {
 
 uint32_t row_tiles(size_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 
-struct Layout { size_t ml, o, scores, total; uint32_t t_rt, p_rt; };
+struct Layout { size_t ml, o, scores, total; uint32_t t_rt; bool umma; };
 
 // How a call's work is cut and where its partial results lie. false: sizes the kernels do not take.
 bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, Layout& l, const char** why) {
@@ -487,15 +490,22 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     if (with_weights && !a.nslots) return false;
     const size_t tokens = (size_t)a.batch * a.q_len, rows = tokens * a.rep;
     l.t_rt = row_tiles((size_t)a.q_len * a.rep);
-    l.p_rt = std::max(l.t_rt, row_tiles(rows));
-    a.p_tokens = (uint32_t)std::min<size_t>(tokens, l.p_rt * 16 / a.rep);
+    // the prefix goes with the tails while its rows fit into their row tiles, else on tcgen05
+    l.umma = rows > l.t_rt * 16;
+    a.p_tokens = (uint32_t)std::min<size_t>(tokens, (l.umma ? 128 : l.t_rt * 16) / a.rep);
     a.p_tiles = (uint32_t)((tokens + a.p_tokens - 1) / a.p_tokens);
-    const uint32_t fit = SMS * (l.p_rt == 8 ? 1 : 2), groups = a.p_tiles * a.kv_heads;
-    const uint32_t tiles = (a.n_prefix + TILE - 1) / TILE;
+    const uint32_t unit = l.umma ? 128 : TILE, tiles = (a.n_prefix + unit - 1) / unit;
     a.p_slices = a.p_len = 0;
     if (tiles) {
-        const uint32_t want = std::min(tiles, std::max(1u, fit / groups));
-        a.p_len = (tiles + want - 1) / want * TILE;
+        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * (l.t_rt == 8 ? 1 : 2);
+        uint32_t best = 1;
+        size_t least = SIZE_MAX;
+        // rounds over the SMs of slices and about three tiles' time to begin and end one
+        for (uint32_t s = 1; s <= std::min(tiles, fit); s++) {
+            const size_t cost = ((size_t)groups * s + fit - 1) / fit * ((tiles + s - 1) / s + 3);
+            if (cost < least) { least = cost; best = s; }
+        }
+        a.p_len = (tiles + best - 1) / best * unit;
         a.p_slices = (a.n_prefix + a.p_len - 1) / a.p_len;
     }
     a.t_slices = std::max(1u, 6 * SMS / a.kv_heads);
@@ -510,10 +520,10 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
 
 }  // namespace
 
-bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t rt, bool prefix, bool tails) {
+bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t rt, bool prefix, bool tails, bool beside) {
     const uint32_t items = prefix ? a.p_tiles * a.kv_heads * a.p_slices : 0;
-    if (hd == 128) return bf16 ? launch_parts_rt<true, 128>(st, a, rt, items, tails) : launch_parts_rt<false, 128>(st, a, rt, items, tails);
-    return bf16 ? launch_parts_rt<true, 64>(st, a, rt, items, tails) : launch_parts_rt<false, 64>(st, a, rt, items, tails);
+    if (hd == 128) return bf16 ? launch_parts_rt<true, 128>(st, a, rt, items, tails, beside) : launch_parts_rt<false, 128>(st, a, rt, items, tails, beside);
+    return bf16 ? launch_parts_rt<true, 64>(st, a, rt, items, tails, beside) : launch_parts_rt<false, 64>(st, a, rt, items, tails, beside);
 }
 bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16) {
     if (hd == 128) return bf16 ? launch_merge<true, 128>(st, a) : launch_merge<false, 128>(st, a);
@@ -581,10 +591,10 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
     a.plan = (uint32_t*)ws; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
     a.scores = weights_dev ? (float*)(ws + l.scores) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool bf = dtype == GEHTP_DT_BF16, one = l.p_rt == l.t_rt;
+    const bool bf = dtype == GEHTP_DT_BF16, umma = n_prefix && l.umma;
     bool ok = true;
-    if (n_prefix && !one) ok = k_shared_parts(st, a, head_dim, bf, l.p_rt, true, false);
-    if (ok && (nslots || (n_prefix && one))) ok = k_shared_parts(st, a, head_dim, bf, l.t_rt, n_prefix && one, nslots != 0);
+    if (umma) ok = k_shared_prefix_sm100(st, a, head_dim, bf);
+    if (ok && (nslots || (n_prefix && !umma))) ok = k_shared_parts(st, a, head_dim, bf, l.t_rt, n_prefix && !umma, nslots != 0, umma);
     if (ok) ok = k_shared_merge(st, a, head_dim, bf);
     if (!ok) {
         const cudaError_t e = cudaGetLastError();

@@ -1,0 +1,400 @@
+// The shared prefix on tcgen05 / TMEM: the rows that all sequences have on a key head against the prefix's keys and values.
+//
+// One CTA = one key head, one slice of the prefix and two tiles of 128 rows (PAIR), or one tile where a key head has no more rows.
+// K / V tiles of 128 positions by TMA straight from the prefix's ring, zeros past its end. Two groups of four softmax warps:
+// of a PAIR each has a row tile, and the two share every K / V tile (a CTA with one row tile would need 64 KB of L2 for 32 KB
+// worth of work: 119 bytes a cycle and SM, where L2 gives about 64); of a single tile each has every other K / V tile, with an S, an O,
+// maxima and sums of its own, and the halves are added at the end.
+//
+//   S = Q K^T       tcgen05.mma into TMEM
+//   P               one thread per row: maximum, 2^(s - m) written over S as matrix operand: fp16, or bf16 as hi + lo pairs (bf16's 8 bits
+//                   are fewer than a result of that type has)
+//   O += P V        tcgen05.mma with P as the A operand from TMEM, V as it lies in memory (MN-major B operand)
+// The maximum a row is referred to is raised - and its O rescaled - only when a tile exceeds it by more than 2^8.
+//
+// Rows of a tile: p_tokens tokens of rep heads, heads fastest (a three-dimensional TMA box over [head_dim][heads][tokens]). Where rep does
+// not divide 128 the last rows of a tile are left over: what lies in their shared memory never reaches another row.
+//
+//   warp 0     TMA: Q once, K and V tiles in stages
+//   warp 1     one lane issues tcgen05.mma / tcgen05.commit
+//   warp 2     owns the TMEM allocation (512 columns)
+//   warps 4-11 softmax and output
+// Every mbarrier wait is bounded; on a timeout the CTA raises the status word and winds down.
+#include <cuda.h>
+#include "engine.h"
+#include "launchers_batch.h"
+#include "sm100_attn.cuh"
+
+namespace gehtp {
+
+using namespace sm100;
+
+// what a wait that ran out leaves for gehtp_attn_shared_status
+__device__ unsigned int g_shared_status;
+
+namespace {
+
+constexpr uint32_t BKV = 128;
+constexpr int NTHREADS = 384;
+constexpr float kRaise = 8.0f;
+
+// stages of K and of V tiles: as many as 227 KB hold behind the rows' tiles
+template <int DB, bool PAIR>
+__host__ __device__ constexpr int kv_stages() { return DB == 2 ? (PAIR ? 2 : 3) : 4; }
+
+template <int ST>
+struct __align__(8) PBars {
+    uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full, merge;
+    uint32_t tmem_base, abort_flag;
+};
+
+// V boxes of 128 positions x 64 values: 8-position groups 1024 bytes apart, the second 64 values 16384 bytes further
+__device__ __forceinline__ uint64_t desc_v128(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(16384 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// 2^(s sc + off) of 32 scores (EDGE: 0 where the bit is not set), as 16 words of fp16 pairs; adds the values to l
+template <bool EDGE>
+__device__ __forceinline__ void probs32_h(const uint32_t (&v)[32], uint32_t (&w)[32], float sc, float off, uint32_t see, float2 (&l)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), make_float2(sc, sc), make_float2(off, off));
+        float2 e = make_float2(ex2(x.x), ex2(x.y));
+        if (EDGE) {
+            e.x = (see >> (2 * i)) & 1u ? e.x : 0.0f;
+            e.y = (see >> (2 * i + 1)) & 1u ? e.y : 0.0f;
+        }
+        l[i & 1] = add2(l[i & 1], e);
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(e.y), "f"(e.x));
+    }
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr) : "memory");
+}
+
+// BF: bf16. DB: head_dim in units of 64
+template <bool BF, int DB, bool PAIR>
+__global__ void __launch_bounds__(NTHREADS, 1)
+shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const SharedArgs A) {
+    extern __shared__ unsigned char smem_raw[];
+    constexpr int ST = kv_stages<DB, PAIR>();
+    constexpr uint32_t BOX = 128 * 64 * 2, TILE = DB * BOX, NQ = PAIR ? 2 : 1, FMT = BF ? IDESC_BF16 : 0u;
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* sQ = smem;
+    unsigned char* sK = sQ + NQ * TILE;
+    unsigned char* sV = sK + ST * TILE;
+    PBars<ST>* bars = (PBars<ST>*)(sV + ST * TILE);
+    volatile uint32_t* abort_flag = &bars->abort_flag;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t h = blockIdx.y, slice = blockIdx.z, tile0 = blockIdx.x * NQ;
+    const uint32_t from = slice * A.p_len, to = min(A.n_prefix, from + A.p_len), n_kt = (to - from + BKV - 1) / BKV;
+    const uint32_t heads = A.kv_heads * A.rep;
+    const bool two = PAIR && tile0 + 1 < A.p_tiles;               // an odd number of row tiles leaves the last CTA one
+    const uint32_t box_rows = A.p_tokens * A.rep;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bars->q_full, 1); mbar_init(&bars->o_full, 1); mbar_init(&bars->merge, 8);
+        for (int s = 0; s < ST; s++) {
+            mbar_init(&bars->k_full[s], 1); mbar_init(&bars->k_empty[s], 1);
+            mbar_init(&bars->v_full[s], 1); mbar_init(&bars->v_empty[s], 1);
+        }
+        for (int s = 0; s < 2; s++) { mbar_init(&bars->s_full[s], 1); mbar_init(&bars->p_full[s], 4); }
+        bars->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = bars->tmem_base;
+    pdl_wait();
+    pdl_release();     // behind the wait: the tails' kernel starts beside this one and may read all that was there before the call
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            mbar_expect_tx(&bars->q_full, (two ? 2 : 1) * DB * box_rows * 128);
+            for (uint32_t t = 0; t < (two ? 2u : 1u); t++)
+#pragma unroll
+                for (uint32_t d = 0; d < DB; d++)
+                    tma_load_3d(sQ + t * TILE + d * BOX, &tmap_q, (int)(d * 64), (int)(h * A.rep), (int)((tile0 + t) * A.p_tokens), &bars->q_full);
+            uint32_t kn = 0, vn = 0;
+            for (uint32_t j = 0; j < n_kt && !*abort_flag; j++) {
+                const uint32_t s = j % ST, ph = (j / ST) & 1;
+                const int y = (int)(from + j * BKV);
+                if (!mbar_wait_or_abort(&bars->k_empty[s], ph ^ 1, abort_flag)) { *abort_flag = 1; break; }
+                mbar_expect_tx(&bars->k_full[s], TILE);
+#pragma unroll
+                for (uint32_t d = 0; d < DB; d++) tma_load_2d(sK + s * TILE + d * BOX, &tmap_kv, (int)((h * DB + d) * 64), y, &bars->k_full[s]);
+                kn++;
+                if (!mbar_wait_or_abort(&bars->v_empty[s], ph ^ 1, abort_flag)) { *abort_flag = 1; break; }
+                mbar_expect_tx(&bars->v_full[s], TILE);
+#pragma unroll
+                for (uint32_t d = 0; d < DB; d++) tma_load_2d(sV + s * TILE + d * BOX, &tmap_kv, (int)(((A.kv_heads + h) * DB + d) * 64), y, &bars->v_full[s]);
+                vn++;
+            }
+            if (*abort_flag) {   // copies already requested must land before the CTA may go away
+                mbar_wait(&bars->q_full, 0);
+                for (uint32_t j = kn > ST ? kn - ST : 0; j < kn; j++) mbar_wait(&bars->k_full[j % ST], (j / ST) & 1);
+                for (uint32_t j = vn > ST ? vn - ST : 0; j < vn; j++) mbar_wait(&bars->v_full[j % ST], (j / ST) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            const uint32_t q_base = smem_u32(sQ), k_base = smem_u32(sK), v_base = smem_u32(sV);
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                if (ok) ok = mbar_wait_or_abort(bar, parity, abort_flag);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                return ok;
+            };
+            // S of group t: row tile `q` against K tile j
+            auto issue_s = [&](uint32_t t, uint32_t q, uint32_t j) {
+#pragma unroll
+                for (uint32_t d = 0; d < DB; d++)
+#pragma unroll
+                    for (uint32_t k4 = 0; k4 < 4; k4++)
+                        umma_f16(tmem + t * 128, umma_desc(q_base + q * TILE + d * BOX) + (uint64_t)(k4 * 2),
+                                 umma_desc(k_base + (j % ST) * TILE + d * BOX) + (uint64_t)(k4 * 2), idesc_f16(128) | FMT, (d | k4) ? 1u : 0u);
+                umma_commit(&bars->s_full[t]);
+            };
+            auto issue_o = [&](uint32_t t, uint32_t j, bool first) {
+#pragma unroll
+                for (uint32_t part = 0; part < (BF ? 2u : 1u); part++)
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; k++)             // 16 positions = two 8-position groups = 2048 bytes; bit 16: B is MN-major
+                        umma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8,
+                                    desc_v128(v_base + (j % ST) * TILE + k * 2048), idesc_f16(DB * 64) | FMT | (1u << 16), (!first || part || k) ? 1u : 0u);
+            };
+            if (PAIR) {
+                if (wait(&bars->q_full, 0) && wait(&bars->k_full[0], 0)) {
+                    issue_s(0, 0, 0);
+                    if (two) issue_s(1, 1, 0);
+                    umma_commit(&bars->k_empty[0]);
+                }
+                for (uint32_t j = 0; ok && j < n_kt; j++) {
+                    const uint32_t s = j % ST, s1 = (j + 1) % ST, ph1 = ((j + 1) / ST) & 1;
+                    const bool more = j + 1 < n_kt;
+                    if (!wait(&bars->v_full[s], (j / ST) & 1) || !wait(&bars->p_full[0], j & 1)) break;
+                    issue_o(0, j, j == 0);
+                    if (more) {
+                        if (!wait(&bars->k_full[s1], ph1)) break;
+                        issue_s(0, 0, j + 1);
+                    }
+                    if (two) {
+                        if (!wait(&bars->p_full[1], j & 1)) break;
+                        issue_o(1, j, j == 0);
+                    }
+                    umma_commit(&bars->v_empty[s]);
+                    if (more) {
+                        if (two) issue_s(1, 1, j + 1);
+                        umma_commit(&bars->k_empty[s1]);
+                    }
+                }
+            } else {
+                auto next_s = [&](uint32_t j) {
+                    if (!wait(&bars->k_full[j % ST], (j / ST) & 1)) return;
+                    issue_s(j & 1, 0, j);
+                    umma_commit(&bars->k_empty[j % ST]);
+                };
+                if (wait(&bars->q_full, 0)) {
+                    next_s(0);
+                    if (n_kt > 1) next_s(1);
+                }
+                for (uint32_t j = 0; ok && j < n_kt; j++) {
+                    if (!wait(&bars->v_full[j % ST], (j / ST) & 1) || !wait(&bars->p_full[j & 1], (j >> 1) & 1)) break;
+                    issue_o(j & 1, j, j < 2);
+                    umma_commit(&bars->v_empty[j % ST]);
+                    if (j + 2 < n_kt) next_s(j + 2);             // over the P just read: products run in the order they are issued
+                }
+            }
+            if (ok) umma_commit(&bars->o_full);
+            else *abort_flag = 1;
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ softmax and output: one thread per row and group
+        const uint32_t t = (warp - 4) >> 2, quarter = warp & 3;
+        const uint32_t ts = tmem + ((quarter * 32) << 16) + t * 128, to_ = ts + 256;
+        float m = -INFINITY;
+        float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        bool ok = true;
+        const bool works = t == 0 || (PAIR ? two : n_kt > 1);
+        uint32_t round = 0;
+#pragma unroll 1
+        for (uint32_t j = PAIR ? 0 : t; works && j < n_kt; j += PAIR ? 1 : 2, round++) {
+            ok = !__any_sync(0xffffffffu, *abort_flag != 0) && __all_sync(0xffffffffu, mbar_wait_or_abort(&bars->s_full[t], round & 1, abort_flag));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int hi = (int)(A.n_prefix - 1 - (from + j * BKV));       // last column of the tile that is a position of the prefix
+            const bool edge = hi < (int)BKV - 1;
+            float mt = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 2; c++) {
+                uint32_t va[32], vb[32];
+                tmem_ld32(ts + c * 64, va);
+                tmem_ld32(ts + c * 64 + 32, vb);
+                tmem_ld_wait(va);
+                tmem_ld_wait(vb);
+                if (edge) mt = fmaxf(mt, fmaxf(max32<true>(va, visible32(c * 64, 0, hi)), max32<true>(vb, visible32(c * 64 + 32, 0, hi))));
+                else mt = fmaxf(mt, fmaxf(max32<false>(va, 0u), max32<false>(vb, 0u)));
+            }
+            mt *= A.sc;
+            // s_full of this tile came after the group's products of the tile before: its O is at rest
+            const bool raise = mt > m + kRaise;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float f = raise ? (m == -INFINITY ? 0.0f : ex2(m - mt)) : 1.0f;
+                if (raise) m = mt;
+#pragma unroll
+                for (int i = 0; i < 2; i++) { l2[i].x *= f; l2[i].y *= f; }
+                if (round) {
+#pragma unroll 1
+                    for (int c = 0; c < DB * 2; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(to_ + c * 32, v);
+                        tmem_ld_wait(v);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tmem_st32(to_ + c * 32, v);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            const float off = m == -INFINITY ? 0.0f : -m;
+            auto probs = [&](const uint32_t (&v)[32], uint32_t col) {
+                uint32_t w[32];
+                if (BF) {
+                    if (edge) probs32<true>(v, w, A.sc, off, visible32((int)col, 0, hi), l2);
+                    else probs32<false>(v, w, A.sc, off, 0u, l2);
+                    tmem_st32(ts + col, w);
+                } else {
+                    if (edge) probs32_h<true>(v, w, A.sc, off, visible32((int)col, 0, hi), l2);
+                    else probs32_h<false>(v, w, A.sc, off, 0u, l2);
+                    tmem_st16(ts + col, w);
+                }
+            };
+#pragma unroll 1
+            for (int c = 0; c < 2; c++) {
+                uint32_t va[32], vb[32];
+                tmem_ld32(ts + c * 64, va);
+                tmem_ld_wait(va);
+                tmem_ld32(ts + c * 64 + 32, vb);
+                probs(va, c * 64);
+                tmem_ld_wait(vb);
+                probs(vb, c * 64 + 32);
+            }
+            tmem_st_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->p_full[t]);
+        }
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&bars->o_full, 0, abort_flag));      // all operands have been read
+        float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y), f0 = 1.0f, f1 = 0.0f;
+        float2* halves = (float2*)sQ;                                     // of a single row tile: {m, l} of [group][row]
+        if (!PAIR && ok) {
+            halves[t * 128 + quarter * 32 + lane] = make_float2(m, l);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->merge);
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&bars->merge, 0, abort_flag));
+            const float2 a = halves[quarter * 32 + lane], b = halves[128 + quarter * 32 + lane];
+            m = fmaxf(a.x, b.x);
+            // a group without a maximum has no sum either, or one that is no number and stays
+            f0 = a.x == -INFINITY ? (a.y == 0.0f ? 0.0f : 1.0f) : ex2(a.x - m);
+            f1 = b.x == -INFINITY ? (b.y == 0.0f ? 0.0f : 1.0f) : ex2(b.x - m);
+            l = a.y * f0 + b.y * f1;
+        }
+        const uint32_t tile = tile0 + (PAIR ? t : 0), row0 = quarter * 32;
+        if (ok && tile < A.p_tiles) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t rows = min(A.p_tokens, A.batch * A.q_len - tile * A.p_tokens) * A.rep;
+            const size_t part = (((size_t)tile * A.kv_heads + h) * A.p_slices + slice) * box_rows;
+            // The warp's 32 rows by way of shared memory, so that a request touches whole rows. Of a single tile each group takes half the columns.
+            constexpr uint32_t COLS = PAIR ? DB * 64 : DB * 32, CH = COLS / 4;
+            float4* stage = (float4*)sK + (warp - 4) * (32 * CH);
+            const uint32_t ta = tmem + ((quarter * 32) << 16) + 256 + (PAIR ? t * 128 : t * COLS);
+#pragma unroll 1
+            for (uint32_t c = 0; c < COLS / 16; c++) {
+                uint32_t v[16], u[16];
+                tmem_ld16(ta + c * 16, v);
+                if (!PAIR && n_kt > 1) tmem_ld16(ta + 128 + c * 16, u);
+                tmem_ld_wait(v);
+                if (!PAIR && n_kt > 1) tmem_ld_wait(u);
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    x[i] = __uint_as_float(v[i]);
+                    if (!PAIR) x[i] = n_kt > 1 ? fmaf(__uint_as_float(u[i]), f1, x[i] * f0) : x[i] * f0;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) stage[lane * CH + ((c * 4 + i) ^ (lane & 7))] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            }
+            __syncwarp();
+#pragma unroll 4
+            for (uint32_t i = lane; i < 32 * CH; i += 32) {
+                const uint32_t r = i / CH, p = i % CH;
+                if (row0 + r < rows) ((float4*)(A.part_o + (part + row0 + r) * (DB * 64) + (PAIR ? 0 : t * COLS)))[p] = stage[r * CH + (p ^ (r & 7))];
+            }
+            if ((PAIR || t == 0) && row0 + lane < rows) A.part_ml[part + row0 + lane] = make_float2(m, l);
+        }
+        if (!ok) *abort_flag = 1;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 2) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        if (lane == 0 && *abort_flag) raise_status(&g_shared_status, kStatusAttnTimeout);
+    }
+}
+
+template <bool BF, int DB, bool PAIR>
+bool launch(cudaStream_t st, const SharedArgs& a) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const CUtensorMapDataType type = BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t hd = DB * 64, heads = (cuuint64_t)a.kv_heads * a.rep, tokens = (cuuint64_t)a.batch * a.q_len;
+    CUtensorMap tq, tkv;
+    cuuint64_t qd[3] = {hd, heads, tokens}, qs[2] = {hd * 2, a.q_stride * 2}, kd[2] = {2 * a.kv_heads * hd, a.n_prefix}, ks[1] = {4 * a.kv_heads * hd};
+    cuuint32_t qb[3] = {64, a.rep, a.p_tokens}, kb[2] = {64, BKV}, one[3] = {1, 1, 1};
+    if (enc(&tq, type, 3, (void*)a.q, qd, qs, qb, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+        enc(&tkv, type, 2, (void*)a.prefix, kd, ks, kb, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    constexpr int ST = kv_stages<DB, PAIR>();
+    const size_t smem = 1024 + (size_t)((PAIR ? 2 : 1) + 2 * ST) * DB * 16384 + sizeof(PBars<ST>);
+    static int have[64] = {};
+    if (!ensure_dyn_smem(shared_prefix_sm100_kernel<BF, DB, PAIR>, smem, have)) return false;
+    const dim3 grid(PAIR ? (a.p_tiles + 1) / 2 : a.p_tiles, a.kv_heads, a.p_slices);
+    g_launches++;
+    return launch_pdl(shared_prefix_sm100_kernel<BF, DB, PAIR>, grid, dim3(NTHREADS), smem, st, tq, tkv, a) == cudaSuccess;
+}
+template <bool BF, int DB>
+bool launch_pair(cudaStream_t st, const SharedArgs& a) { return a.p_tiles > 1 ? launch<BF, DB, true>(st, a) : launch<BF, DB, false>(st, a); }
+
+}  // namespace
+
+bool k_shared_prefix_sm100(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16) {
+    if (hd == 128) return bf16 ? launch_pair<true, 2>(st, a) : launch_pair<false, 2>(st, a);
+    return bf16 ? launch_pair<true, 1>(st, a) : launch_pair<false, 1>(st, a);
+}
+
+}  // namespace gehtp
+
+// 0 when no bounded wait of gehtp_attn_shared's kernels on the current device has run out since the last query, else the code it
+// left (and the word is cleared)
+extern "C" int gehtp_attn_shared_status(void) {
+    unsigned int v = 0;
+    if (cudaMemcpyFromSymbol(&v, gehtp::g_shared_status, sizeof v) != cudaSuccess) { cudaGetLastError(); return -1; }
+    if (v) {
+        const unsigned int zero = 0;
+        cudaMemcpyToSymbol(gehtp::g_shared_status, &zero, sizeof zero);
+        gehtp::g.last_error = "attn shared: a K/V tile copy or a product never arrived (bounded wait ran out); the output is incomplete";
+    }
+    return (int)(v & 0x7fffffffu);
+}

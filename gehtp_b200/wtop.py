@@ -259,6 +259,7 @@ def bind(lib):
         lib.gehtp_attn_shared_workspace.argtypes = [u32] * 7 + [c.c_int]
         lib.gehtp_attn_shared_workspace.restype = c.c_size_t
         lib.gehtp_attn_shared.argtypes = [vp] * 7 + [u32] * 9 + [c.c_float, vp, c.c_size_t, vp]
+        lib.gehtp_attn_shared_status.restype = c.c_int
         lib.gehtp_kv_evict_workspace.argtypes = [u32] * 7
         lib.gehtp_kv_evict_workspace.restype = c.c_size_t
         lib.gehtp_kv_evict.argtypes = [vp] * 7 + [u32] * 7 + [vp, c.c_size_t, vp]

@@ -369,6 +369,11 @@ int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, const void* tai
                       uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_stride, uint32_t n_prefix,
                       uint32_t nslots, uint32_t dtype, float scale, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* Kernels of gehtp_attn_shared wait for their copies and products with a bounded poll. 0: every call on the current device since the last
+ * query completed; > 0: a wait ran out and that call's output is incomplete; -1: the copy of the word failed. Reads and
+ * clears the word; call it after synchronising the stream. */
+int gehtp_attn_shared_status(void);
+
 /* Cuts caches down to their positions of greatest weight. A sequence with more than `keep` positions keeps, for every key head on its
  * own, its first `sinks` positions, its last `recent` and, of those between, the ones of greatest weight (of equal weights the lower
  * position; a weight that is no number counts as less than any other); they move up in their order to slots 0 .. keep - 1. Rotary
