@@ -4,9 +4,7 @@
 //
 // Query t of a sequence (of q_len new tokens, the last positions of its tail) sees the tail up to its own position. The prefix is
 // read once for all sequences: its keys meet the rows of all of them, rep query heads to a key head. Rows of one tail are few
-// (q_len * rep). Positions that every row of a sequence sees go through the tensor cores without a mask; the up to
-// q_len - 1 positions behind them, each seen by some rows only, are added row by row (`zone` below), so no row's result depends
-// on a position that it does not see.
+// (q_len * rep). No row's result depends on a position that it does not see, whatever is cached there.
 //
 // shared_parts_kernel: CTAs that stay and walk the items (row tile, key head, slice of the prefix) and (sequence, key head, slice of
 // its tail). K and V tiles of 64 positions by cp.async in three or four stages; a warp has 16 rows and a quarter, a half or all of
@@ -149,14 +147,14 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             token0 = b * A.q_len;
             rows = A.q_len * A.rep;
             from = (u - cum[b]) * s_k * TILE;
-            to = min(c, from + s_k * TILE);
             last = u + 1 == cum[b + 1];
+            to = last ? n : from + s_k * TILE;
             v_off = (size_t)A.batch * A.kv_heads * HD;
             kbase = A.tail + ((size_t)b * A.kv_heads + h) * HD;
             part = p_rows + ((size_t)u * A.kv_heads + h) * rows;
         }
         pitch = 2 * v_off;
-        const uint32_t tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
+        uint32_t tiles = (to - from + TILE - 1) / TILE;
 
         auto load = [&](uint32_t i) {
             if (i < tiles) {
@@ -174,13 +172,35 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             cp_commit();
         };
         for (int i = 0; i < STG - 1; i++) load(i);
+        // Positions that only some rows see carry weight 0 for the others, which is 0 times their values: where one of those is no number,
+        // the positions are left to the code behind the tiles, which adds them row by row.
+        uint32_t nz = last ? n - c : 0;
+        if (nz) {
+            bool odd = false;
+            for (uint32_t e = threadIdx.x; e < nz * (HD / 8); e += NT) {
+                const uint4 v = *(const uint4*)(kbase + (size_t)(c + e / (HD / 8)) * pitch + v_off + e % (HD / 8) * 8);
+                constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
+                for (uint32_t x : {v.x, v.y, v.z, v.w}) odd |= (x & EXP & 0xffffu) == (EXP & 0xffffu) || (x & EXP & 0xffff0000u) == (EXP & 0xffff0000u);
+            }
+            if (__syncthreads_or(odd)) {
+                cp_wait<0>();
+                __syncthreads();
+                to = max(c, from);
+                tiles = (to - from + TILE - 1) / TILE;
+                for (int i = 0; i < STG - 1; i++) load(i);
+            } else {
+                nz = 0;
+            }
+        }
 
         // ---- queries of this warp's rows as A fragments
         uint32_t qf[HD / 16][4];
+        int lim[2];                                                   // the first position that a row does not see
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint32_t r = rt * 16 + g8 + half * 8;
             const bool in = r < rows;
+            lim[half] = last ? min((int)to, (int)(n + r / A.rep + 1) - (int)A.q_len) : (int)to;
             const uint16_t* qp = A.q + (in ? (size_t)(token0 + r / A.rep) * A.q_stride + (size_t)(h * A.rep + r % A.rep) * HD : 0) + q4 * 2;
 #pragma unroll
             for (int k = 0; k < HD / 16; k++) {
@@ -217,7 +237,7 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             for (int t = 0; t < 2 * NP; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const bool in = p0 + t * 8 + q4 * 2 + (e & 1) < to;
+                    const bool in = (int)(p0 + t * 8 + q4 * 2 + (e & 1)) < lim[e >> 1];
                     s[t][e] = in ? s[t][e] * A.sc : -INFINITY;
                     mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
                 }
@@ -294,7 +314,6 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
 #pragma unroll
             for (int j = 0; j < HD / 8; j++) *(float2*)&so[(size_t)(pg * 16 * RT + r) * LD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
         }
-        const uint32_t nz = last ? n - c : 0;                          // positions that only some rows see
         for (uint32_t e = warp; e < rows * nz; e += NW) {
             const uint32_t r = e / nz, i = e % nz, t = r / A.rep;
             float s = -INFINITY;
@@ -372,22 +391,25 @@ __device__ __forceinline__ float part_factor(float2 ml, float M) { return ml.x =
 
 constexpr uint32_t W_CHUNK = 512;
 
-// The first `row_blocks` CTAs: a warp to a row of the result. The others: 512 tail positions of a (sequence, key head) each.
-template <bool BF, int HD>
+// The first `row_blocks` CTAs: WR warps to a row of the result. The others: 512 tail positions of a (sequence, key head) each.
+template <bool BF, int HD, int WR>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, uint32_t row_blocks, uint32_t chunks) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_release();
     if (blockIdx.x < row_blocks) {
-        const uint32_t heads = A.kv_heads * A.rep, row = blockIdx.x * 8 + warp;
-        if (row >= A.batch * A.q_len * heads) return;
+        const uint32_t heads = A.kv_heads * A.rep, row = blockIdx.x * (8 / WR) + warp / WR, wr = warp % WR;
+        const bool there = row < A.batch * A.q_len * heads;
+        if (WR == 1 && !there) return;
+        constexpr int V = HD / 32;
+        float acc[V] = {};
+        float inv = 0.0f;
+        if (there) {
         const RowParts x = row_parts(A, row / heads, row % heads);
         const uint32_t count = x.p_count + x.t_count;
         float M = -INFINITY, L = 0.0f;
         for (uint32_t i = lane; i < count; i += 32) M = fmaxf(M, __ldcg(&A.part_ml[part_at(x, i)]).x);
         M = warp_max(M);
-        constexpr int V = HD / 32;
-        float acc[V] = {};
         for (uint32_t i0 = 0; i0 < count; i0 += 32) {
             const uint32_t mine = i0 + lane;
             const float2 ml = mine < count ? __ldcg(&A.part_ml[part_at(x, mine)]) : make_float2(-INFINITY, 0.0f);
@@ -395,7 +417,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, u
             L = fmaf(ml.y, f, L);
             const uint32_t here = min(32u, count - i0);
 #pragma unroll 4
-            for (uint32_t i = 0; i < here; i++) {
+            for (uint32_t i = wr; i < here; i += WR) {
                 const float fi = __shfl_sync(0xffffffffu, f, i);
                 const float* p = A.part_o + part_at(x, i0 + i) * HD + lane * V;
                 if (V == 4) {
@@ -408,7 +430,19 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, u
             }
         }
         L = warp_sum(L);
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;      // a row that sees nothing: zeros
+        inv = L == 0.0f ? 0.0f : 1.0f / L;                  // a row that sees nothing: zeros
+        }
+        if (WR > 1) {
+            __shared__ float sums[8][HD];
+#pragma unroll
+            for (int v = 0; v < V; v++) sums[warp][v * 32 + lane] = acc[v];
+            __syncthreads();
+            if (wr || !there) return;
+#pragma unroll
+            for (int w = 1; w < WR; w++)
+#pragma unroll
+                for (int v = 0; v < V; v++) acc[v] += sums[warp + w][v * 32 + lane];
+        }
         uint32_t* out = (uint32_t*)(A.out + (size_t)row * HD + lane * V);
         if (V == 4) *(uint2*)out = make_uint2(pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[V - 2] * inv, acc[V - 1] * inv));
         else *out = pack2<BF>(acc[0] * inv, acc[1] * inv);
@@ -466,9 +500,12 @@ template <bool BF, int HD>
 bool launch_merge(cudaStream_t st, const SharedArgs& a) {
     const size_t rows = (size_t)a.batch * a.q_len * a.kv_heads * a.rep;
     const uint32_t chunks = (a.nslots + W_CHUNK - 1) / W_CHUNK;
-    const size_t blocks = (rows + 7) / 8, more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
+    // four warps to a row while a warp each would leave the SMs room
+    const bool wide = rows <= 8 * SMS;
+    const size_t blocks = wide ? (rows + 1) / 2 : (rows + 7) / 8, more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
     g_launches++;
-    return launch_pdl(shared_merge_kernel<BF, HD>, dim3((uint32_t)(blocks + more)), dim3(256), 0, st, a, (uint32_t)blocks, std::max(1u, chunks)) == cudaSuccess;
+    return launch_pdl(wide ? shared_merge_kernel<BF, HD, 4> : shared_merge_kernel<BF, HD, 1>, dim3((uint32_t)(blocks + more)), dim3(256), 0, st, a, (uint32_t)blocks,
+                      std::max(1u, chunks)) == cudaSuccess;
 }
 
 uint32_t row_tiles(size_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }

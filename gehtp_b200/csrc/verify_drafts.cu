@@ -6,11 +6,15 @@
 //   r = max(p_i - q_i, 0) at the first place i that was not accepted (p_i where the rows are alike: a sum below 1e-12), r = p_n when all were
 //   T = 0: x_i is accepted while it is the lowest place of the largest logit, and the token behind is that place
 //
-// verify_rows_kernel: maximum and sum of 2^(x - maximum) of pieces of the rows, one pass over the logits in fp32: what the tests of
-// acceptance need. A probability is then some 2^-22 off, and so is a test's border.
-// verify_choose_kernel: a cluster of eight CTAs per sequence decides how many are accepted and draws the token behind them. A draw that a
-// border of two tokens is next to has to go to the right one, and the borders are as many as there are tokens: this one row is taken
+// verify_rows_kernel: maximum and sum of 2^((x - maximum) k), k = log2(e) / T, of pieces of the rows, a warp to a piece, in fp32: within some
+// 2^-20, which is what the tests of acceptance go by.
+// verify_choose_kernel: a cluster of eight CTAs per sequence decides how many are accepted and draws the token behind them. A draw that ends
+// next to the border of two tokens has to go to the right one, and there are as many borders as tokens: this one row is taken
 // in 64 bits. Every warp has a stretch of the vocabulary; its sum says in which stretch the draw ends, and that warp walks it.
+// r needs the sums of p and q, which are not known in 64 bits before the row has been read: with c0 = sum q / sum p in fp32 in the place of the
+// true c, one pass gives sum(e_p - c0 e_q) and sum(e_q) over the tokens where e_p > c0 e_q, and so sum(e_p - c e_q) = the first -
+// (c - c0) times the second; tokens whose e_p / e_q lies between c0 and c (some 2^-22 wide) are off by no more than that width
+// squared. Where p and q are so alike that this could show (a sum below 2^-10) the row is read once more with the true c.
 #include <cooperative_groups.h>
 #include <cmath>
 #include <cstdio>
@@ -44,21 +48,24 @@ struct El32 { typedef float T; static constexpr int V = 4; static __device__ flo
 struct ElBf { typedef uint16_t T; static constexpr int V = 8; static __device__ float f(uint16_t x) { return bf2f(x); } };
 struct ElHf { typedef uint16_t T; static constexpr int V = 8; static __device__ float f(uint16_t x) { return h2f(x); } };
 
-// V logits from place e on (a multiple of V off the row's first 16-byte boundary, or in front of it): in one load where they lie in the row
-// and on a boundary; places outside the row are -inf
+// V logits from a 16-byte boundary on
+template <class E>
+__device__ __forceinline__ void unpack_logits(const uint4& v, float (&x)[E::V]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (E::V == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { x[2 * i] = E::f((typename E::T)(w[i] & 0xffffu)); x[2 * i + 1] = E::f((typename E::T)(w[i] >> 16)); }
+    }
+}
+// V logits from place e on: in one load where they lie in the row and on a boundary; places outside the row are -inf
 template <class E>
 __device__ __forceinline__ void load_logits(const typename E::T* row, int64_t e, int64_t end, float (&x)[E::V]) {
     const typename E::T* p = row + e;
     if (e >= 0 && e + E::V <= end && ((uintptr_t)p & 15u) == 0) {
-        const uint4 v = __ldg((const uint4*)p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        if constexpr (E::V == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) { x[2 * i] = E::f((typename E::T)(w[i] & 0xffffu)); x[2 * i + 1] = E::f((typename E::T)(w[i] >> 16)); }
-        }
+        unpack_logits<E>(__ldg((const uint4*)p), x);
     } else {
 #pragma unroll
         for (int i = 0; i < E::V; i++) x[i] = e + i >= 0 && e + i < end ? E::f(p[i]) : -INFINITY;
@@ -67,6 +74,29 @@ __device__ __forceinline__ void load_logits(const typename E::T* row, int64_t e,
 // logits between the row's start and the last 16-byte boundary at or in front of it
 template <class E>
 __device__ __forceinline__ int lead(const typename E::T* row) { return (int)(((uintptr_t)row & 15u) / sizeof(typename E::T)); }
+
+// 2^((x - m) k) in 64 bits: x k - m k split into a whole number and at most a half, 2^that by the interpolation of degree 9 at the Chebyshev
+// points of [-1/2, 1/2] (within 2^-45). 0 below 2^-1000 and for -inf.
+struct Power64 {
+    double k, mk;
+    float floor;
+    __device__ __forceinline__ Power64(double k_, float m) : k(k_), mk(-(double)m * k_), floor((float)((double)m - 1000.0 / k_)) {}
+    __device__ __forceinline__ double operator()(float x) const {
+        const double t = fma((double)fmaxf(x, floor), k, mk), magic = 6755399441055744.0, n = t + magic, f = t - (n - magic);
+        double v = 1.0205905413765595e-07;
+        v = fma(v, f, 1.325964524488711e-06);
+        v = fma(v, f, 1.5252672924850737e-05);
+        v = fma(v, f, 0.0001540343375125101);
+        v = fma(v, f, 0.0013333558200794592);
+        v = fma(v, f, 0.009618129193934313);
+        v = fma(v, f, 0.05550410866465167);
+        v = fma(v, f, 0.2402265069564034);
+        v = fma(v, f, 0.6931471805599462);
+        v = fma(v, f, 1.0000000000000135);
+        const double e = __hiloint2double(__double2hiint(v) + (__double2loint(n) << 20), __double2loint(v));
+        return x >= floor ? e : 0.0;
+    }
+};
 
 __device__ __forceinline__ uint32_t drafts_of(const VerifyArgs& A, uint32_t b) {
     return A.n_drafts ? (uint32_t)min(max(A.n_drafts[b], 0), (int)A.n) : A.n;
@@ -84,62 +114,95 @@ __device__ __forceinline__ bool ahead(float a, int pa, float b, int pb) {
     return a > b || ((a == b || na) && pa < pb);
 }
 
+constexpr int AHEAD = 4;                    // loads of a thread in flight
+
+// A warp to a piece of a row, CTAs that stay. Rows in the order of their drafts, so that all CTAs have like shares of the ones that are there.
 template <class E, bool GREEDY>
 __global__ void __launch_bounds__(RT) verify_rows_kernel(const VerifyArgs A) {
-    __shared__ float2 parts[RT / 32];
+    const uint32_t lane = threadIdx.x & 31;
     pdl_wait();
     pdl_release();
-    const uint32_t t_rows = A.batch * (A.n + 1), row = blockIdx.y + blockIdx.z * gridDim.y;
-    if (row >= t_rows + (A.draft ? A.batch * A.n : 0)) return;
-    const bool target = row < t_rows;
-    const uint32_t r = target ? row : row - t_rows, per = target ? A.n + 1 : A.n, b = r / per, i = r % per;
-    if (i >= drafts_of(A, b) + (target ? 1 : 0)) return;
-    const typename E::T* p = target ? (const typename E::T*)A.target + r * A.t_stride : (const typename E::T*)A.draft + r * A.d_stride;
-    const int64_t first = (int64_t)blockIdx.x * A.piece - lead<E>(p), end = blockIdx.x + 1 == A.pieces ? (int64_t)A.vocab : min((int64_t)A.vocab, first + A.piece);
+    const uint32_t kinds = A.draft ? 2 : 1, rows = A.batch * (A.n * kinds + 1);
+    const uint64_t items = (uint64_t)rows * A.pieces;
     const float k = (float)(A.inv * 1.4426950408889634);
-    float2 best = make_float2(-INFINITY, 0.0f);
-    int place = 0x7fffffff;
-    for (int64_t e = first + threadIdx.x * E::V; e < end; e += RT * E::V) {
-        float x[E::V];
-        load_logits<E>(p, e, end, x);
-        if (GREEDY) {
+    for (uint64_t it = (uint64_t)blockIdx.x * (RT / 32) + threadIdx.x / 32; it < items; it += (uint64_t)gridDim.x * (RT / 32)) {
+        const uint32_t piece = (uint32_t)(it % A.pieces), u = (uint32_t)(it / A.pieces), i = u / (A.batch * kinds), v = u % (A.batch * kinds), b = v % A.batch;
+        const bool target = v < A.batch;
+        if (i >= drafts_of(A, b) + (target ? 1 : 0)) continue;
+        const size_t row = target ? (size_t)b * (A.n + 1) + i : (size_t)b * A.n + i;
+        const typename E::T* p = target ? (const typename E::T*)A.target + row * A.t_stride : (const typename E::T*)A.draft + row * A.d_stride;
+        const int64_t first = (int64_t)piece * A.piece - lead<E>(p), end = piece + 1 == A.pieces ? (int64_t)A.vocab : min((int64_t)A.vocab, first + A.piece);
+        float2 best = make_float2(-INFINITY, 0.0f);
+        int place = 0x7fffffff;
+        bool odd = false;                                            // T = 0: some logit is no number
+        // N vectors of places e, e + STEP, ... together: one look at the maximum
+        constexpr int64_t STEP = 32 * E::V;
+        auto take = [&](const auto& x, int64_t e) {
+            constexpr int N = sizeof(x) / sizeof(float);
+            if (GREEDY) {
 #pragma unroll
-            for (int j = 0; j < E::V; j++)
-                if (e + j >= 0 && e + j < end && ahead(x[j], (int)(e + j), best.x, place)) { best.x = x[j]; place = (int)(e + j); }
-        } else {
-            float m = x[0];
+                for (int j = 0; j < N; j++) {                        // a lane's places ascend: the first of equal ones stays
+                    odd |= x[j] != x[j];
+                    if (x[j] > best.x) { best.x = x[j]; place = (int)(e + (j / E::V) * STEP + j % E::V); }
+                }
+            } else {
+                float m[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int j = 1; j < E::V; j++) m = fmaxf(m, x[j]);
-            if (m > best.x) {
-                best.y = best.x == -INFINITY ? best.y : best.y * sm100::ex2((best.x - m) * k);
-                best.x = m;
+                for (int j = 4; j < N; j++) m[j & 3] = fmaxf(m[j & 3], x[j]);
+                m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                if (m[0] > best.x) {
+                    best.y = best.x == -INFINITY ? best.y : best.y * sm100::ex2((best.x - m[0]) * k);
+                    best.x = m[0];
+                }
+                const float off = best.x == -INFINITY ? 0.0f : best.x;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < N; j++) sum[j & 3] += sm100::ex2((x[j] - off) * k);
+                best.y += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            const float off = best.x == -INFINITY ? 0.0f : best.x;
+        };
+        int64_t e = first + lane * E::V;
+        if (e < 0) {                                                 // in front of the row's first boundary
+            float x[E::V];
+            load_logits<E>(p, e, end, x);
+            take(x, e);
+            e += STEP;
+        }
+        for (; e + (AHEAD - 1) * STEP + E::V <= end; e += AHEAD * STEP) {
+            uint4 w[AHEAD];
+            float x[AHEAD * E::V];
 #pragma unroll
-            for (int j = 0; j < E::V; j++) best.y += sm100::ex2((x[j] - off) * k);
+            for (int u2 = 0; u2 < AHEAD; u2++) w[u2] = __ldg((const uint4*)(p + e + u2 * STEP));
+#pragma unroll
+            for (int u2 = 0; u2 < AHEAD; u2++) {
+                float y[E::V];
+                unpack_logits<E>(w[u2], y);
+#pragma unroll
+                for (int j = 0; j < E::V; j++) x[u2 * E::V + j] = y[j];
+            }
+            take(x, e);
         }
-    }
-    if (GREEDY) {
-        for (int o = 16; o; o >>= 1) {
-            const float y = __shfl_xor_sync(0xffffffffu, best.x, o);
-            const int q = __shfl_xor_sync(0xffffffffu, place, o);
-            if (ahead(y, q, best.x, place)) { best.x = y; place = q; }
+        for (; e < end; e += STEP) {
+            float x[E::V];
+            load_logits<E>(p, e, end, x);
+            take(x, e);
         }
-        best.y = __int_as_float(place);
-    } else {
-        for (int o = 16; o; o >>= 1) {
-            const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.y, o));
-            best = join(best, y, k);
+        __syncwarp();
+        if (GREEDY) {
+            if (odd) { best.x = NAN; place = 0; }
+            for (int o = 16; o; o >>= 1) {
+                const float y = __shfl_xor_sync(0xffffffffu, best.x, o);
+                const int q = __shfl_xor_sync(0xffffffffu, place, o);
+                if (ahead(y, q, best.x, place)) { best.x = y; place = q; }
+            }
+            best.y = __int_as_float(place);
+        } else {
+            for (int o = 16; o; o >>= 1) {
+                const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.y, o));
+                best = join(best, y, k);
+            }
         }
-    }
-    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < RT / 32; w++) {
-            if (GREEDY) { if (ahead(parts[w].x, __float_as_int(parts[w].y), best.x, __float_as_int(best.y))) best = parts[w]; }
-            else best = join(best, parts[w], k);
-        }
-        A.part[(size_t)row * A.pieces + blockIdx.x] = best;
+        if (lane == 0) A.part[(row + (target ? 0 : (size_t)A.batch * (A.n + 1))) * A.pieces + piece] = best;
     }
 }
 
@@ -162,17 +225,183 @@ __device__ __forceinline__ float2 whole_row(const VerifyArgs& A, size_t row) {
 }
 __device__ __forceinline__ bool sound(float2 x) { return x.y > 0.0f && isfinite(x.y) && isfinite(x.x); }
 
+constexpr int WARPS = CT / 32, EACH = STRETCHES / 32;
+
+struct DrawShared {
+    double mine[4][WARPS], all[4][STRETCHES], goal, upto, c;
+    int where, less;
+};
+
+// The sums of four values over the stretches: of all of them in order, for every CTA of the cluster.
+__device__ __forceinline__ void share_sums(cg::cluster_group& cluster, DrawShared& S, double (&v)[4]) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[i] = warp_sum_d(v[i]);
+        if (lane == 0) S.mine[i][warp] = v[i];
+    }
+    cluster.sync();
+    for (uint32_t i = threadIdx.x; i < 4 * STRETCHES; i += CT)
+        S.all[i / STRETCHES][i % STRETCHES] = cluster.map_shared_rank(&S.mine[0][0], i % STRETCHES / WARPS)[i / STRETCHES * WARPS + i % WARPS];
+    cluster.sync();                                           // all have read: `mine` may be written again, CTAs may leave
+}
+
+// The token that a draw from r = max(p - q, 0) (from p without q, or where they are alike) ends in; `away` is never drawn. -1: none has a
+// weight (S.where). The CTA that finds it writes it to `to_`.
+template <class E>
+__device__ void draw(const typename E::T* p, const typename E::T* q, float2 rp, float2 rq, double k, double u, int64_t vocab, int away, DrawShared& S, int32_t* to_) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = cluster.block_rank() * WARPS + warp;
+    const int64_t p_lead = lead<E>(p), vecs = (vocab + p_lead + E::V - 1) / E::V, from = vecs * mine / STRETCHES, to = vecs * (mine + 1) / STRETCHES;
+    const Power64 ep(k, rp.x), eq(k, rq.x);
+    const double c0 = q ? (double)(rp.y / rq.y) : 0.0;
+    double v[4] = {0.0, 0.0, 0.0, 0.0};                       // sums of e_p, e_q; e_p - c0 e_q and e_q where the former is positive
+    for (int64_t j = from + lane; j < to; j += 32) {
+        const int64_t e = j * E::V - p_lead;
+        float x[E::V], y[E::V];
+        load_logits<E>(p, e, vocab, x);
+        if (q) load_logits<E>(q, e, vocab, y);
+#pragma unroll
+        for (int i = 0; i < E::V; i++) {
+            const double a = e + i == away ? 0.0 : ep(x[i]);
+            v[0] += a;
+            if (q) {
+                const double b = eq(y[i]), r = fma(-c0, b, a);
+                v[1] += b;
+                v[2] += r > 0.0 ? r : 0.0;
+                v[3] += r > 0.0 ? b : 0.0;
+            }
+        }
+    }
+    share_sums(cluster, S, v);
+    // one warp: which weights, and where they end the draw
+    if (warp == 0) {
+        double w[EACH], tp = 0.0, tq = 0.0, t = 0.0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) { tp += S.all[0][lane * EACH + i]; tq += S.all[1][lane * EACH + i]; }
+        tp = warp_sum_d(tp);
+        tq = warp_sum_d(tq);
+        const double c = q ? tp / tq : 0.0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) t += fma(c0 - c, S.all[3][lane * EACH + i], S.all[2][lane * EACH + i]);
+        t = warp_sum_d(t);
+        if (lane == 0) { S.c = c; S.less = !q ? 0 : t > 0x1p-10 * tp ? 1 : 2; }
+    }
+    __syncthreads();
+    const double c = S.c;
+    int less = S.less;
+    // e_p - c e_q with the product rounded on its own: equal rows leave 0
+    auto rest = [&](float x, float y) { return fmax(ep(x) - __dmul_rn(c, eq(y)), 0.0); };
+    if (less == 2) {                                          // the same for the whole cluster
+        double r[4] = {0.0, 0.0, 0.0, 0.0};
+        for (int64_t j = from + lane; j < to; j += 32) {
+            const int64_t e = j * E::V - p_lead;
+            float x[E::V], y[E::V];
+            load_logits<E>(p, e, vocab, x);
+            load_logits<E>(q, e, vocab, y);
+#pragma unroll
+            for (int i = 0; i < E::V; i++) r[2] += rest(x[i], y[i]);
+        }
+        r[0] = lane == 0 ? S.mine[0][warp] : 0.0;
+        __syncwarp();
+        share_sums(cluster, S, r);
+    }
+    if (warp == 0) {
+        double w[EACH], tp = 0.0, t = 0.0, sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int at = lane * EACH + i;
+            tp += S.all[0][at];
+            w[i] = less == 1 ? fmax(fma(c0 - c, S.all[3][at], S.all[2][at]), 0.0) : less == 2 ? S.all[2][at] : S.all[0][at];
+            t += w[i];
+        }
+        if (less == 2) {
+            // below: what the roundings of two sums leave of equal rows
+            if (warp_sum_d(t) <= 1e-12 * warp_sum_d(tp)) {
+                less = 0;
+#pragma unroll
+                for (int i = 0; i < EACH; i++) w[i] = S.all[0][lane * EACH + i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++) sum += w[i];
+        double before = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double z = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= (uint32_t)o) before += z;
+        }
+        const double total = __shfl_sync(0xffffffffu, before, 31), goal = fmax(u * total, 0.0);
+        double upto = before - sum, front = 0.0;
+        int hit = -1, some = -1;                              // the first stretch whose end is above the goal, the last with a weight
+        double some_front = 0.0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            if (w[i] > 0.0) {
+                some = lane * EACH + i; some_front = upto;
+                if (hit < 0 && upto + w[i] > goal) { hit = some; front = upto; }
+            }
+            upto += w[i];
+        }
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
+        const int l = hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : 0;   // a draw of 1 and above ends in the last
+        const int where = __shfl_sync(0xffffffffu, hits ? hit : some, l);
+        const double at = __shfl_sync(0xffffffffu, hits ? front : some_front, l);
+        if (lane == 0) { S.where = where; S.goal = goal; S.upto = at; S.less = less; }
+    }
+    __syncthreads();
+    less = S.less;
+    if (S.where < 0 || (uint32_t)S.where != mine) return;
+    const double goal = S.goal;
+    double upto = S.upto;
+    int64_t found = -1, last = -1;
+    for (int64_t j0 = from; j0 < to && found < 0; j0 += 32) {
+        const int64_t j = j0 + lane, e = j * E::V - p_lead;
+        float x[E::V], y[E::V];
+        double r[E::V], sum = 0.0;
+        if (j < to) {
+            load_logits<E>(p, e, vocab, x);
+            if (less) load_logits<E>(q, e, vocab, y);
+        }
+#pragma unroll
+        for (int i = 0; i < E::V; i++) {
+            r[i] = j >= to || e + i == away ? 0.0 : less ? rest(x[i], y[i]) : ep(x[i]);
+            sum += r[i];
+        }
+        double before = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double z = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= (uint32_t)o) before += z;
+        }
+        const double end = upto + __shfl_sync(0xffffffffu, before, 31);
+        double s = upto + (before - sum);
+        int64_t here = -1, some = -1;
+#pragma unroll
+        for (int i = 0; i < E::V; i++) {
+            s += r[i];
+            if (r[i] > 0.0) {
+                some = e + i;
+                if (here < 0 && s > goal) here = e + i;
+            }
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, here >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
+        if (any) last = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
+        if (hit) found = __shfl_sync(0xffffffffu, here, __ffs(hit) - 1);
+        upto = end;
+    }
+    if (lane == 0) *to_ = (int)(found >= 0 ? found : last);   // the stretch's sum was above the goal: its last possible token at the latest
+}
+
 template <class E, bool GREEDY>
 __global__ void __launch_bounds__(CT) verify_choose_kernel(const VerifyArgs A) {
-    __shared__ double sum_p[CT / 32], sum_q[CT / 32], sum_r[CT / 32], all[STRETCHES], s_total[2], s_goal, s_upto;
+    __shared__ DrawShared shared;
     __shared__ uint8_t pass[MAX_DRAFTS];
-    __shared__ float s_max[2];
-    __shared__ int s_where, s_drawn;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x / CL, rank = blockIdx.x % CL;
+    __shared__ float2 s_row[2];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x / (GREEDY ? 1 : CL), rank = blockIdx.x % (GREEDY ? 1 : CL);
     pdl_wait();
     pdl_release();
     const uint32_t nd = drafts_of(A, b);
     const typename E::T *target = (const typename E::T*)A.target + (size_t)b * (A.n + 1) * A.t_stride, *draft = (const typename E::T*)A.draft + (size_t)b * A.n * A.d_stride;
+    const double k = A.inv * 1.4426950408889634;
     // ---- which drafts pass
     for (uint32_t i = warp; i < nd; i += CT / 32) {
         const int x = A.tokens[(size_t)b * A.n + i];
@@ -182,14 +411,13 @@ __global__ void __launch_bounds__(CT) verify_choose_kernel(const VerifyArgs A) {
             ok = isfinite(p.x) && x == __float_as_int(p.y);
         } else {
             const bool in = x >= 0 && (uint32_t)x < A.vocab;
-            const double l2 = A.inv * 1.4426950408889634;
             double px = 0.0, qx = 1.0;
             ok = sound(p);
-            if (ok && in) px = exp2(((double)E::f(target[i * A.t_stride + x]) - p.x) * l2) / p.y;
+            if (ok && in) px = exp2(((double)E::f(target[i * A.t_stride + x]) - p.x) * k) / p.y;
             if (A.draft) {
                 const float2 q = whole_row<false>(A, (size_t)A.batch * (A.n + 1) + (size_t)b * A.n + i);
                 ok = ok && sound(q);
-                qx = ok && in ? exp2(((double)E::f(draft[i * A.d_stride + x]) - q.x) * l2) / q.y : 0.0;
+                qx = ok && in ? exp2(((double)E::f(draft[i * A.d_stride + x]) - q.x) * k) / q.y : 0.0;
             }
             ok = ok && (double)A.uniforms[(size_t)b * (A.n + 1) + i] * qx < px;
         }
@@ -206,156 +434,25 @@ __global__ void __launch_bounds__(CT) verify_choose_kernel(const VerifyArgs A) {
             if (i != a) out[i] = i < a ? A.tokens[(size_t)b * A.n + i] : -1;
     }
     // ---- the row behind the accepted ones
-    if (GREEDY) {
-        if (rank == 0 && warp == 0) {
-            const float2 p = whole_row<true>(A, (size_t)b * (A.n + 1) + a);
-            if (lane == 0) out[a] = isfinite(p.x) ? __float_as_int(p.y) : -1;
-        }
-        return;
-    }
-    cg::cluster_group cluster = cg::this_cluster();
-    const bool with_q = rejected && A.draft;
-    if (warp == 0) {
-        const float2 p = whole_row<false>(A, (size_t)b * (A.n + 1) + a);
-        if (lane == 0) s_max[0] = sound(p) ? p.x : NAN;
-    }
-    if (warp == 1 && with_q) {
-        const float2 q = whole_row<false>(A, (size_t)A.batch * (A.n + 1) + (size_t)b * A.n + a);
-        if (lane == 0) s_max[1] = sound(q) ? q.x : NAN;
+    if (warp < 2) {
+        float2 x = make_float2(NAN, NAN);
+        if (warp == 0) x = whole_row<GREEDY>(A, (size_t)b * (A.n + 1) + a);
+        else if (!GREEDY && rejected && A.draft) x = whole_row<false>(A, (size_t)A.batch * (A.n + 1) + (size_t)b * A.n + a);
+        if (lane == 0) s_row[warp] = x;
     }
     __syncthreads();
-    const double mp = s_max[0], mq = with_q ? s_max[1] : NAN, l2 = A.inv * 1.4426950408889634;
-    if (mp != mp) {                                           // a row without a distribution (the same for the whole cluster)
-        if (rank == 0 && threadIdx.x == 0) out[a] = -1;
-        return;
+    if constexpr (GREEDY) {
+        if (threadIdx.x == 0) out[a] = isfinite(s_row[0].x) ? __float_as_int(s_row[0].y) : -1;
+    } else {
+        if (!sound(s_row[0])) {                                   // a row without a distribution, for the whole cluster
+            if (rank == 0 && threadIdx.x == 0) out[a] = -1;
+            return;
+        }
+        const int away = rejected && !A.draft ? A.tokens[(size_t)b * A.n + a] : -1;
+        const typename E::T *p = target + a * A.t_stride, *q = sound(s_row[1]) ? draft + a * A.d_stride : nullptr;   // a draft row without one takes nothing away
+        draw<E>(p, q, s_row[0], s_row[1], k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], A.vocab, away, shared, out + a);
+        if (rank == 0 && threadIdx.x == 0 && shared.where < 0) out[a] = away;                    // all of p lay on the rejected token
     }
-    const bool use_q = mq == mq;                              // a draft row without one takes nothing away
-    const int away = rejected && !A.draft ? A.tokens[(size_t)b * A.n + a] : -1;
-    const typename E::T *p = target + a * A.t_stride, *q = use_q ? draft + a * A.d_stride : nullptr;
-    const int64_t vocab = A.vocab, p_lead = lead<E>(p), vecs = (vocab + p_lead + E::V - 1) / E::V;
-    const uint32_t mine = rank * (CT / 32) + warp;
-    const int64_t from = vecs * mine / STRETCHES, to = vecs * (mine + 1) / STRETCHES;      // the warp's stretch
-    auto chance = [](float x, double l2, double m) { return exp2(((double)x - m) * l2); };
-    // p - q of two such values, both products rounded on their own: equal ones leave 0
-    double sp = 1.0, sq = 1.0;
-    auto excess = [&](float x, float y) { return fmax(__dmul_rn(chance(x, l2, mp), sp) - __dmul_rn(chance(y, l2, mq), sq), 0.0); };
-    auto block_sums = [&](double v, double* to_smem) {
-        v = warp_sum_d(v);
-        if (lane == 0) to_smem[warp] = v;
-    };
-    double tp = 0.0, tq = 0.0;
-    for (int64_t j = from + lane; j < to; j += 32) {
-        const int64_t e = j * E::V - p_lead;
-        float x[E::V];
-        load_logits<E>(p, e, vocab, x);
-#pragma unroll
-        for (int i = 0; i < E::V; i++) tp += e + i == away ? 0.0 : chance(x[i], l2, mp);
-        if (use_q) {
-            load_logits<E>(q, e, vocab, x);
-#pragma unroll
-            for (int i = 0; i < E::V; i++) tq += chance(x[i], l2, mq);
-        }
-    }
-    block_sums(tp, sum_p);
-    block_sums(tq, sum_q);
-    cluster.sync();
-    // all stretches' sums in order; every CTA for itself
-    auto gather = [&](double* of) {
-        for (uint32_t i = threadIdx.x; i < STRETCHES; i += CT) all[i] = cluster.map_shared_rank(of, i / (CT / 32))[i % (CT / 32)];
-        __syncthreads();
-    };
-    bool less = false;                                        // r = p - q
-    if (use_q) {
-        for (int w = 0; w < 2; w++) {
-            gather(w ? sum_q : sum_p);
-            if (threadIdx.x == 0) {
-                double t = 0.0;
-                for (int i = 0; i < STRETCHES; i++) t += all[i];
-                s_total[w] = t;
-            }
-            __syncthreads();
-        }
-        sp = 1.0 / s_total[0]; sq = 1.0 / s_total[1];
-        double tr = 0.0;
-        for (int64_t j = from + lane; j < to; j += 32) {
-            const int64_t e = j * E::V - p_lead;
-            float x[E::V], y[E::V];
-            load_logits<E>(p, e, vocab, x);
-            load_logits<E>(q, e, vocab, y);
-#pragma unroll
-            for (int i = 0; i < E::V; i++) tr += excess(x[i], y[i]);
-        }
-        block_sums(tr, sum_r);
-        cluster.sync();
-        gather(sum_r);
-        if (threadIdx.x == 0) {
-            double t = 0.0;
-            for (int i = 0; i < STRETCHES; i++) t += all[i];
-            s_total[0] = t;
-        }
-        __syncthreads();
-        less = s_total[0] > 1e-12;                            // below: what the roundings of two sums leave of equal rows
-    }
-    if (!less) gather(sum_p);
-    // p and q alike: of p, whose sums are not normalised. The drafted token alone was possible: of p with it
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < STRETCHES; i++) t += all[i];
-        const double goal = fmax((double)A.uniforms[(size_t)b * (A.n + 1) + A.n] * t, 0.0);
-        double upto = 0.0, front = 0.0;
-        int where = -1;
-        for (int i = 0; i < STRETCHES; i++) {
-            if (all[i] > 0.0) { where = i; front = upto; }    // a draw of 1 and above ends in the last stretch with any
-            if (upto + all[i] > goal) break;
-            upto += all[i];
-        }
-        s_where = t > 0.0 ? where : -1;
-        s_goal = goal; s_upto = front;
-    }
-    __syncthreads();
-    if (s_where < 0) {                                        // all of p lay on the rejected token
-        if (rank == 0 && threadIdx.x == 0) out[a] = away;
-    } else if ((uint32_t)s_where == mine) {
-        const double goal = s_goal;
-        double upto = s_upto;
-        int64_t found = -1, last = -1;
-        for (int64_t j0 = from; j0 < to && found < 0; j0 += 32) {
-            const int64_t j = j0 + lane, e = j * E::V - p_lead;
-            float x[E::V], y[E::V];
-            double r[E::V], sum = 0.0;
-            if (j < to) {
-                load_logits<E>(p, e, vocab, x);
-                if (less) load_logits<E>(q, e, vocab, y);
-            }
-#pragma unroll
-            for (int i = 0; i < E::V; i++) {
-                r[i] = j >= to || e + i == away ? 0.0 : less ? excess(x[i], y[i]) : chance(x[i], l2, mp);
-                sum += r[i];
-            }
-            double before = sum;
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y2 = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= (uint32_t)o) before += y2;
-            }
-            const double end = upto + __shfl_sync(0xffffffffu, before, 31);
-            double c = upto + (before - sum);
-            int64_t here = -1, some = -1;
-#pragma unroll
-            for (int i = 0; i < E::V; i++) {
-                c += r[i];
-                if (r[i] > 0.0) {
-                    some = e + i;
-                    if (here < 0 && c > goal) here = e + i;
-                }
-            }
-            const uint32_t hit = __ballot_sync(0xffffffffu, here >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
-            if (any) last = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
-            if (hit) found = __shfl_sync(0xffffffffu, here, __ffs(hit) - 1);
-            upto = end;
-        }
-        if (lane == 0) out[a] = (int)(found >= 0 ? found : last);   // the stretch's sum was above the goal: its last possible token at the latest
-    }
-    cluster.sync();                                           // others may still read this CTA's sums
 }
 
 const char* verify_refuses(uint32_t batch, uint32_t n, uint32_t vocab) {
@@ -365,25 +462,24 @@ const char* verify_refuses(uint32_t batch, uint32_t n, uint32_t vocab) {
     return nullptr;
 }
 
-// Pieces of a row: about eight CTAs an SM over all rows, of 2048 to 16384 logits
+// Pieces of a row, a warp's each: of 1024 to 8192 logits, some 64 warps an SM over all rows
 void cut_rows(uint32_t batch, uint32_t n, uint32_t vocab, uint32_t* piece, uint32_t* pieces) {
     const size_t total = (size_t)batch * (2 * n + 1) * vocab;
-    uint32_t p = 2048;
-    while (p < 16384 && (size_t)p * 148 * 8 < total) p *= 2;
-    while (((size_t)vocab + 7 + p - 1) / p > 65535) p *= 2;
+    uint32_t p = 1024;
+    while (p < 8192 && (size_t)p * 148 * 64 < total) p *= 2;
     *piece = p;
     *pieces = (uint32_t)(((size_t)vocab + 7 + p - 1) / p);    // up to seven logits in front of the first boundary
 }
 
 template <class E, bool GREEDY>
 bool launch_verify(cudaStream_t st, const VerifyArgs& a) {
-    const size_t rows = (size_t)a.batch * (a.n + 1) + (a.draft ? (size_t)a.batch * a.n : 0);
-    const uint32_t y = (uint32_t)std::min<size_t>(rows, 32768), z = (uint32_t)((rows + y - 1) / y);
+    const uint64_t items = ((uint64_t)a.batch * (a.n * (a.draft ? 2 : 1) + 1)) * a.pieces;
     g_launches += 2;
-    if (launch_pdl(verify_rows_kernel<E, GREEDY>, dim3(a.pieces, y, z), dim3(RT), 0, st, a) != cudaSuccess) return false;
+    if (launch_pdl(verify_rows_kernel<E, GREEDY>, dim3((uint32_t)std::min<uint64_t>((items + RT / 32 - 1) / (RT / 32), 148 * 6)), dim3(RT), 0, st, a) != cudaSuccess) return false;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.batch * CL); cfg.blockDim = dim3(CT); cfg.stream = st;
-    return launch_pdl_cluster(verify_choose_kernel<E, GREEDY>, cfg, dim3(CL, 1, 1), a) == cudaSuccess;
+    const uint32_t cl = GREEDY ? 1 : CL;
+    cfg.gridDim = dim3(a.batch * cl); cfg.blockDim = dim3(CT); cfg.stream = st;
+    return launch_pdl_cluster(verify_choose_kernel<E, GREEDY>, cfg, dim3(cl, 1, 1), a) == cudaSuccess;
 }
 
 }  // namespace

@@ -92,16 +92,23 @@ class Call:
                                    stream if stream is not None else torch.cuda.current_stream().cuda_stream)
         assert rc == 0, lib.gehtp_cuda_last_error()
 
-    def check(self):
+    def expected(self):
+        """Of the operands as they are: result, weights, scores' sizes and the tolerance."""
         import torch
-        torch.cuda.synchronize()
         b, t, h, kvh, d = self.shape
         q = self.rows.cpu().double()[:, :h * d].reshape(b, t, h, d)
         n = self.n.clamp(0, self.slots)
         tail = torch.nan_to_num(self.tail.cpu().double())
         want, mag, top, weights = formula(q, self.prefix.cpu().double(), tail, n, self.scale)
         values = torch.cat([self.prefix.cpu()[:, 1].reshape(-1), tail[:, 1].reshape(-1).to(self.dtype), torch.zeros(1, dtype=self.dtype)]).double()
-        tol = tolerance(want, mag, top, values, self.n_prefix + self.slots, self.dtype, d)
+        return want, weights, top, tolerance(want, mag, top, values, self.n_prefix + self.slots, self.dtype, d)
+
+    def check(self):
+        import torch
+        torch.cuda.synchronize()
+        b, t, h, kvh, d = self.shape
+        n = self.n.clamp(0, self.slots)
+        want, weights, top, tol = self.expected()
         got = self.out.cpu().double()
         assert torch.isfinite(got).all()
         off = (got - want).abs() - tol
@@ -166,20 +173,20 @@ def test_again_and_without_given_weights(cuda, prefix, rows):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 def test_a_position_that_is_no_number(cuda, dtype):
-    """It makes no number of the rows that see it and of no others: not of earlier tokens, not of other sequences."""
+    """It makes no number of the rows that see it and of no others: not of earlier tokens, not of other sequences. Those may come by another
+    order of sums, and are held to the formula."""
     import torch
     call = Call(3, 5, 8, 2, 128, 100, 90, [80, 70, 90], getattr(torch, dtype), weights=True)
-    call.run(cuda)
-    torch.cuda.synchronize()
-    clean = call.out.clone()
+    want, _, _, tol = call.expected()
     call.tail.view(90, 2, 3, 2, 128)[72, :, 0] = float("nan")        # the last but seven of the first sequence: seen by all its rows
     call.tail.view(90, 2, 3, 2, 128)[68, 1, 1, 0, 5] = float("inf")  # the second's last but one, a value: rows of the last two tokens
     call.tail.view(90, 2, 3, 2, 128)[88, 0, 2] = float("nan")        # the third's last but one, its key
     call.run(cuda)
     torch.cuda.synchronize()
     assert not torch.isfinite(call.out[0]).any()
-    assert torch.equal(call.out[1, :3], clean[1, :3]) and torch.equal(call.out[2, :3], clean[2, :3])
-    assert not torch.isfinite(call.out[1, 3:, :4, 5]).any() and torch.equal(call.out[1, 3:, 4:], clean[1, 3:, 4:])
+    fine = (call.out.cpu().double() - want).abs() <= tol
+    assert fine[1, :3].all() and fine[2, :3].all()
+    assert not torch.isfinite(call.out[1, 3:, :4, 5]).any() and fine[1, 3:, 4:].all() and fine[1, 3:, :4, :5].all() and fine[1, 3:, :4, 6:].all()
     assert not torch.isfinite(call.out[2, 3:]).any()
 
 
