@@ -8,14 +8,15 @@
 //
 // verify_rows_kernel: maximum and sum of 2^((x - maximum) k), k = log2(e) / T, of pieces of the rows, a warp to a piece, in fp32: within some
 // 2^-20, which is what the tests of acceptance go by.
-// verify_choose_kernel: a cluster of eight CTAs per sequence decides how many are accepted and draws the token behind them. A draw that ends
-// next to the border of two tokens has to go to the right one, and there are as many borders as tokens: this one row is taken
-// in 64 bits. Every warp has a stretch of the vocabulary; its sum says in which stretch the draw ends, and that warp walks it.
+// verify_choose_kernel: several CTAs per sequence decide, each for itself, how many are accepted, and draw the token behind them. A draw
+// that ends next to the border of two tokens has to go to the right one, and there are as many borders as tokens: this one row
+// is taken in 64 bits. Every warp has a stretch of the vocabulary; the CTA that comes last sees from the stretches' sums in which
+// one the draw ends, and walks it.
 // r needs the sums of p and q, which are not known in 64 bits before the row has been read: with c0 = sum q / sum p in fp32 in the place of the
 // true c, one pass gives sum(e_p - c0 e_q) and sum(e_q) over the tokens where e_p > c0 e_q, and so sum(e_p - c e_q) = the first -
 // (c - c0) times the second; tokens whose e_p / e_q lies between c0 and c (some 2^-22 wide) are off by no more than that width
 // squared. Where p and q are so alike that this could show (a sum below 2^-10) the row is read once more with the true c.
-#include <cooperative_groups.h>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <algorithm>
@@ -28,10 +29,8 @@ namespace gehtp {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr uint32_t MAX_DRAFTS = 64;
-constexpr int RT = 256, CT = 512, CL = 8, STRETCHES = CL * CT / 32;
+constexpr uint32_t MAX_DRAFTS = 64, MAX_SPLITS = 64;
+constexpr int RT = 256, CT = 256, WARPS = CT / 32;
 
 struct VerifyArgs {
     const void *target, *draft;             // draft NULL: drafts without probabilities (and always with T = 0)
@@ -41,6 +40,9 @@ struct VerifyArgs {
     uint32_t batch, n, vocab, pieces, piece;        // pieces of `piece` logits to a row
     size_t t_stride, d_stride;
     double inv;                             // 1 / T
+    uint32_t splits;                        // CTAs that share a sequence's draw
+    uint32_t* done;                         // [batch] of them that are through; zeros when the second kernel starts
+    double4* sums;                          // [batch][splits * WARPS] of the stretches
     float2* part;                           // [target rows | draft rows][pieces] {maximum, sum}; T = 0: {maximum, its place}
 };
 
@@ -125,6 +127,8 @@ __global__ void __launch_bounds__(RT) verify_rows_kernel(const VerifyArgs A) {
     const uint32_t kinds = A.draft ? 2 : 1, rows = A.batch * (A.n * kinds + 1);
     const uint64_t items = (uint64_t)rows * A.pieces;
     const float k = (float)(A.inv * 1.4426950408889634);
+    if (!GREEDY && blockIdx.x == 0)
+        for (uint32_t b = threadIdx.x; b < A.batch; b += RT) A.done[b] = 0;
     for (uint64_t it = (uint64_t)blockIdx.x * (RT / 32) + threadIdx.x / 32; it < items; it += (uint64_t)gridDim.x * (RT / 32)) {
         const uint32_t piece = (uint32_t)(it % A.pieces), u = (uint32_t)(it / A.pieces), i = u / (A.batch * kinds), v = u % (A.batch * kinds), b = v % A.batch;
         const bool target = v < A.batch;
@@ -225,139 +229,169 @@ __device__ __forceinline__ float2 whole_row(const VerifyArgs& A, size_t row) {
 }
 __device__ __forceinline__ bool sound(float2 x) { return x.y > 0.0f && isfinite(x.y) && isfinite(x.x); }
 
-constexpr int WARPS = CT / 32, EACH = STRETCHES / 32;
-
-struct DrawShared {
-    double mine[4][WARPS], all[4][STRETCHES], goal, upto, c;
-    int where, less;
+// Sums over the CTA: of all threads, and of those in front of each.
+struct BlockScan {
+    double warp[WARPS];
+    __device__ __forceinline__ double sum(double v) {
+        v = warp_sum_d(v);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) warp[threadIdx.x >> 5] = v;
+        __syncthreads();
+        double t = 0.0;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) t += warp[i];
+        return t;
+    }
+    __device__ __forceinline__ double before(double v, double* total) {
+        double x = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double z = __shfl_up_sync(0xffffffffu, x, o);
+            if ((threadIdx.x & 31) >= (uint32_t)o) x += z;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 31) warp[threadIdx.x >> 5] = x;
+        __syncthreads();
+        double t = 0.0, front = 0.0;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) { if (i == (int)(threadIdx.x >> 5)) front = t; t += warp[i]; }
+        *total = t;
+        return front + (x - v);
+    }
 };
 
-// The sums of four values over the stretches: of all of them in order, for every CTA of the cluster.
-__device__ __forceinline__ void share_sums(cg::cluster_group& cluster, DrawShared& S, double (&v)[4]) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[i] = warp_sum_d(v[i]);
-        if (lane == 0) S.mine[i][warp] = v[i];
-    }
-    cluster.sync();
-    for (uint32_t i = threadIdx.x; i < 4 * STRETCHES; i += CT)
-        S.all[i / STRETCHES][i % STRETCHES] = cluster.map_shared_rank(&S.mine[0][0], i % STRETCHES / WARPS)[i / STRETCHES * WARPS + i % WARPS];
-    cluster.sync();                                           // all have read: `mine` may be written again, CTAs may leave
+struct DrawShared {
+    BlockScan scan;
+    int first, last, is_last;
+    double front;
+};
+
+// The lowest place of `hit` (a place or INT_MAX) over the CTA, and the sum in front of it.
+__device__ __forceinline__ void lowest(DrawShared& S, int hit, double front) {
+    if (threadIdx.x == 0) S.first = INT_MAX;
+    __syncthreads();
+    if (hit != INT_MAX) atomicMin(&S.first, hit);
+    __syncthreads();
+    if (hit != INT_MAX && S.first == hit) S.front = front;
+    __syncthreads();
 }
 
-// The token that a draw from r = max(p - q, 0) (from p without q, or where they are alike) ends in; `away` is never drawn. -1: none has a
-// weight (S.where). The CTA that finds it writes it to `to_`.
+// The token that a draw from r = max(p - q, 0) (from p without q, or where they are alike) ends in; `away` is never drawn, and comes back
+// where nothing else has a weight. The last CTA of a sequence writes it.
 template <class E>
-__device__ void draw(const typename E::T* p, const typename E::T* q, float2 rp, float2 rq, double k, double u, int64_t vocab, int away, DrawShared& S, int32_t* to_) {
-    cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = cluster.block_rank() * WARPS + warp;
-    const int64_t p_lead = lead<E>(p), vecs = (vocab + p_lead + E::V - 1) / E::V, from = vecs * mine / STRETCHES, to = vecs * (mine + 1) / STRETCHES;
+__device__ __forceinline__ void draw(const VerifyArgs& A, uint32_t b, const typename E::T* p, const typename E::T* q, float2 rp, float2 rq, double k, double u, int away,
+                                     DrawShared& S, int32_t* to_) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stretches = A.splits * WARPS;
+    const int64_t vocab = A.vocab, p_lead = lead<E>(p), vecs = (vocab + p_lead + E::V - 1) / E::V;
     const Power64 ep(k, rp.x), eq(k, rq.x);
     const double c0 = q ? (double)(rp.y / rq.y) : 0.0;
-    double v[4] = {0.0, 0.0, 0.0, 0.0};                       // sums of e_p, e_q; e_p - c0 e_q and e_q where the former is positive
-    for (int64_t j = from + lane; j < to; j += 32) {
-        const int64_t e = j * E::V - p_lead;
-        float x[E::V], y[E::V];
-        load_logits<E>(p, e, vocab, x);
-        if (q) load_logits<E>(q, e, vocab, y);
-#pragma unroll
-        for (int i = 0; i < E::V; i++) {
-            const double a = e + i == away ? 0.0 : ep(x[i]);
-            v[0] += a;
-            if (q) {
-                const double b = eq(y[i]), r = fma(-c0, b, a);
-                v[1] += b;
-                v[2] += r > 0.0 ? r : 0.0;
-                v[3] += r > 0.0 ? b : 0.0;
-            }
-        }
-    }
-    share_sums(cluster, S, v);
-    // one warp: which weights, and where they end the draw
-    if (warp == 0) {
-        double w[EACH], tp = 0.0, tq = 0.0, t = 0.0;
-#pragma unroll
-        for (int i = 0; i < EACH; i++) { tp += S.all[0][lane * EACH + i]; tq += S.all[1][lane * EACH + i]; }
-        tp = warp_sum_d(tp);
-        tq = warp_sum_d(tq);
-        const double c = q ? tp / tq : 0.0;
-#pragma unroll
-        for (int i = 0; i < EACH; i++) t += fma(c0 - c, S.all[3][lane * EACH + i], S.all[2][lane * EACH + i]);
-        t = warp_sum_d(t);
-        if (lane == 0) { S.c = c; S.less = !q ? 0 : t > 0x1p-10 * tp ? 1 : 2; }
-    }
-    __syncthreads();
-    const double c = S.c;
-    int less = S.less;
-    // e_p - c e_q with the product rounded on its own: equal rows leave 0
-    auto rest = [&](float x, float y) { return fmax(ep(x) - __dmul_rn(c, eq(y)), 0.0); };
-    if (less == 2) {                                          // the same for the whole cluster
-        double r[4] = {0.0, 0.0, 0.0, 0.0};
+    {
+        const int64_t mine = blockIdx.x * WARPS + warp, from = vecs * mine / stretches, to = vecs * (mine + 1) / stretches;
+        double4 v = make_double4(0.0, 0.0, 0.0, 0.0);         // sums of e_p, e_q; e_p - c0 e_q and e_q where the former is positive
         for (int64_t j = from + lane; j < to; j += 32) {
             const int64_t e = j * E::V - p_lead;
             float x[E::V], y[E::V];
             load_logits<E>(p, e, vocab, x);
-            load_logits<E>(q, e, vocab, y);
+            if (q) {
+                load_logits<E>(q, e, vocab, y);
 #pragma unroll
-            for (int i = 0; i < E::V; i++) r[2] += rest(x[i], y[i]);
-        }
-        r[0] = lane == 0 ? S.mine[0][warp] : 0.0;
-        __syncwarp();
-        share_sums(cluster, S, r);
-    }
-    if (warp == 0) {
-        double w[EACH], tp = 0.0, t = 0.0, sum = 0.0;
+                for (int i = 0; i < E::V; i++) {
+                    const double a = ep(x[i]), d = eq(y[i]), r = fma(-c0, d, a);
+                    const bool more = __double2hiint(r) > 0;
+                    v.x += a;
+                    v.y += d;
+                    v.z += more ? r : 0.0;
+                    v.w += more ? d : 0.0;
+                }
+            } else {
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int at = lane * EACH + i;
-            tp += S.all[0][at];
-            w[i] = less == 1 ? fmax(fma(c0 - c, S.all[3][at], S.all[2][at]), 0.0) : less == 2 ? S.all[2][at] : S.all[0][at];
-            t += w[i];
-        }
-        if (less == 2) {
-            // below: what the roundings of two sums leave of equal rows
-            if (warp_sum_d(t) <= 1e-12 * warp_sum_d(tp)) {
-                less = 0;
-#pragma unroll
-                for (int i = 0; i < EACH; i++) w[i] = S.all[0][lane * EACH + i];
+                for (int i = 0; i < E::V; i++) v.x += e + i == away ? 0.0 : ep(x[i]);
             }
         }
-#pragma unroll
-        for (int i = 0; i < EACH; i++) sum += w[i];
-        double before = sum;
-        for (int o = 1; o < 32; o <<= 1) {
-            const double z = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= (uint32_t)o) before += z;
+        v.x = warp_sum_d(v.x);
+        if (q) { v.y = warp_sum_d(v.y); v.z = warp_sum_d(v.z); v.w = warp_sum_d(v.w); }
+        if (lane == 0) {
+            A.sums[(size_t)b * stretches + mine] = v;
+            __threadfence();
         }
-        const double total = __shfl_sync(0xffffffffu, before, 31), goal = fmax(u * total, 0.0);
-        double upto = before - sum, front = 0.0;
-        int hit = -1, some = -1;                              // the first stretch whose end is above the goal, the last with a weight
-        double some_front = 0.0;
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            if (w[i] > 0.0) {
-                some = lane * EACH + i; some_front = upto;
-                if (hit < 0 && upto + w[i] > goal) { hit = some; front = upto; }
-            }
-            upto += w[i];
-        }
-        const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
-        const int l = hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : 0;   // a draw of 1 and above ends in the last
-        const int where = __shfl_sync(0xffffffffu, hits ? hit : some, l);
-        const double at = __shfl_sync(0xffffffffu, hits ? front : some_front, l);
-        if (lane == 0) { S.where = where; S.goal = goal; S.upto = at; S.less = less; }
     }
     __syncthreads();
-    less = S.less;
-    if (S.where < 0 || (uint32_t)S.where != mine) return;
-    const double goal = S.goal;
-    double upto = S.upto;
-    int64_t found = -1, last = -1;
-    for (int64_t j0 = from; j0 < to && found < 0; j0 += 32) {
-        const int64_t j = j0 + lane, e = j * E::V - p_lead;
+    if (threadIdx.x == 0) S.is_last = atomicAdd(&A.done[b], 1u) + 1 == A.splits;
+    __syncthreads();
+    if (!S.is_last) return;
+    __threadfence();
+    // ---- the last: weights of the stretches, two to a thread
+    static_assert(MAX_SPLITS * WARPS <= 2 * CT, "two stretches to a thread");
+    const double4* sums = A.sums + (size_t)b * stretches;
+    double4 v[2];
+    double w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t at = threadIdx.x * 2 + i;
+        v[i] = make_double4(0.0, 0.0, 0.0, 0.0);
+        if (at < stretches) { const double2 *x = (const double2*)(sums + at), lo = __ldcg(x), hi = __ldcg(x + 1); v[i] = make_double4(lo.x, lo.y, hi.x, hi.y); }
+        w[i] = v[i].x;
+    }
+    double c = 0.0;
+    bool less = q != nullptr;                                 // the weights are p - q
+    // e_p - c e_q with the product rounded on its own: equal rows leave 0
+    auto rest = [&](float x, float y) { return fmax(ep(x) - __dmul_rn(c, eq(y)), 0.0); };
+    if (less) {
+        const double tp = S.scan.sum(v[0].x + v[1].x), tq = S.scan.sum(v[0].y + v[1].y);
+        c = tp / tq;
+#pragma unroll
+        for (int i = 0; i < 2; i++) w[i] = fmax(fma(c0 - c, v[i].w, v[i].z), 0.0);
+        if (S.scan.sum(w[0] + w[1]) < 0x1p-10 * tp) {         // p and q nearly alike: once more with the true c
+            __shared__ double again[MAX_SPLITS * WARPS];
+            for (uint32_t at = warp; at < stretches; at += WARPS) {
+                const int64_t from = vecs * at / stretches, to = vecs * (at + 1) / stretches;
+                double r = 0.0;
+                for (int64_t j = from + lane; j < to; j += 32) {
+                    const int64_t e = j * E::V - p_lead;
+                    float x[E::V], y[E::V];
+                    load_logits<E>(p, e, vocab, x);
+                    load_logits<E>(q, e, vocab, y);
+#pragma unroll
+                    for (int i = 0; i < E::V; i++) r += rest(x[i], y[i]);
+                }
+                r = warp_sum_d(r);
+                if (lane == 0) again[at] = r;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 2; i++) w[i] = threadIdx.x * 2 + i < stretches ? again[threadIdx.x * 2 + i] : 0.0;
+            // below: what the roundings of two sums leave of equal rows
+            if (S.scan.sum(w[0] + w[1]) <= 1e-12 * tp) {
+                less = false;
+                w[0] = v[0].x; w[1] = v[1].x;
+            }
+        }
+    }
+    double total;
+    const double front = S.scan.before(w[0] + w[1], &total), goal = fmax(u * total, 0.0);
+    // the first stretch whose end is above the goal; a draw of 1 and above ends in the last that has a weight
+    if (threadIdx.x == 0) S.last = -1;
+    __syncthreads();
+    if (w[0] > 0.0 || w[1] > 0.0) atomicMax(&S.last, (int)threadIdx.x * 2 + (w[1] > 0.0 ? 1 : 0));
+    int hit = INT_MAX;
+    if (w[0] > 0.0 && front + w[0] > goal) hit = threadIdx.x * 2;
+    else if (w[1] > 0.0 && front + w[0] + w[1] > goal) hit = threadIdx.x * 2 + 1;
+    lowest(S, hit, hit & 1 ? front + w[0] : front);
+    if (S.first == INT_MAX) {
+        if (S.last < 0) {
+            if (threadIdx.x == 0) *to_ = away;                // all of p lay on the rejected token
+            return;
+        }
+        lowest(S, (int)threadIdx.x == S.last / 2 ? S.last : INT_MAX, S.last & 1 ? front + w[0] : front);
+    }
+    const int at = S.first;
+    const int64_t from = vecs * at / stretches, to = vecs * (at + 1) / stretches;
+    double upto = S.front;
+    __syncthreads();
+    if (threadIdx.x == 0) S.last = -1;
+    for (int64_t j0 = from; j0 < to; j0 += CT) {
+        const int64_t j = j0 + threadIdx.x, e = j * E::V - p_lead;
         float x[E::V], y[E::V];
-        double r[E::V], sum = 0.0;
+        double r[E::V], sum = 0.0, all;
         if (j < to) {
             load_logits<E>(p, e, vocab, x);
             if (less) load_logits<E>(q, e, vocab, y);
@@ -367,57 +401,54 @@ __device__ void draw(const typename E::T* p, const typename E::T* q, float2 rp, 
             r[i] = j >= to || e + i == away ? 0.0 : less ? rest(x[i], y[i]) : ep(x[i]);
             sum += r[i];
         }
-        double before = sum;
-        for (int o = 1; o < 32; o <<= 1) {
-            const double z = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= (uint32_t)o) before += z;
-        }
-        const double end = upto + __shfl_sync(0xffffffffu, before, 31);
-        double s = upto + (before - sum);
-        int64_t here = -1, some = -1;
+        double s = upto + S.scan.before(sum, &all);
+        int here = INT_MAX, some = -1;
 #pragma unroll
         for (int i = 0; i < E::V; i++) {
             s += r[i];
             if (r[i] > 0.0) {
-                some = e + i;
-                if (here < 0 && s > goal) here = e + i;
+                some = (int)(e + i);
+                if (here == INT_MAX && s > goal) here = some;
             }
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, here >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
-        if (any) last = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
-        if (hit) found = __shfl_sync(0xffffffffu, here, __ffs(hit) - 1);
-        upto = end;
+        if (some >= 0) atomicMax(&S.last, some);
+        lowest(S, here, 0.0);
+        if (S.first != INT_MAX) break;
+        upto += all;
     }
-    if (lane == 0) *to_ = (int)(found >= 0 ? found : last);   // the stretch's sum was above the goal: its last possible token at the latest
+    // the stretch's sum was above the goal: its last possible token at the latest
+    if (threadIdx.x == 0) *to_ = S.first != INT_MAX ? S.first : S.last;
 }
 
+// grid: (CTAs of a sequence, sequences)
 template <class E, bool GREEDY>
-__global__ void __launch_bounds__(CT) verify_choose_kernel(const VerifyArgs A) {
+__global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A) {
     __shared__ DrawShared shared;
     __shared__ uint8_t pass[MAX_DRAFTS];
     __shared__ float2 s_row[2];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x / (GREEDY ? 1 : CL), rank = blockIdx.x % (GREEDY ? 1 : CL);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
     pdl_wait();
     pdl_release();
     const uint32_t nd = drafts_of(A, b);
     const typename E::T *target = (const typename E::T*)A.target + (size_t)b * (A.n + 1) * A.t_stride, *draft = (const typename E::T*)A.draft + (size_t)b * A.n * A.d_stride;
     const double k = A.inv * 1.4426950408889634;
     // ---- which drafts pass
-    for (uint32_t i = warp; i < nd; i += CT / 32) {
+    for (uint32_t i = warp; i < nd; i += WARPS) {
         const int x = A.tokens[(size_t)b * A.n + i];
+        const bool in = x >= 0 && (uint32_t)x < A.vocab;
+        const double lp = !GREEDY && in ? (double)E::f(target[i * A.t_stride + x]) : 0.0, lq = !GREEDY && in && A.draft ? (double)E::f(draft[i * A.d_stride + x]) : 0.0;
         const float2 p = whole_row<GREEDY>(A, (size_t)b * (A.n + 1) + i);
         bool ok;
         if (GREEDY) {
             ok = isfinite(p.x) && x == __float_as_int(p.y);
         } else {
-            const bool in = x >= 0 && (uint32_t)x < A.vocab;
             double px = 0.0, qx = 1.0;
             ok = sound(p);
-            if (ok && in) px = exp2(((double)E::f(target[i * A.t_stride + x]) - p.x) * k) / p.y;
+            if (ok && in) px = exp2((lp - p.x) * k) / p.y;
             if (A.draft) {
                 const float2 q = whole_row<false>(A, (size_t)A.batch * (A.n + 1) + (size_t)b * A.n + i);
                 ok = ok && sound(q);
-                qx = ok && in ? exp2(((double)E::f(draft[i * A.d_stride + x]) - q.x) * k) / q.y : 0.0;
+                qx = ok && in ? exp2((lq - q.x) * k) / q.y : 0.0;
             }
             ok = ok && (double)A.uniforms[(size_t)b * (A.n + 1) + i] * qx < px;
         }
@@ -428,7 +459,7 @@ __global__ void __launch_bounds__(CT) verify_choose_kernel(const VerifyArgs A) {
     while (a < nd && pass[a]) a++;
     const bool rejected = a < nd;
     int32_t* out = A.out + (size_t)b * (A.n + 1);
-    if (rank == 0) {
+    if (blockIdx.x == 0) {
         if (threadIdx.x == 0) A.accepted[b] = (int)a;
         for (uint32_t i = threadIdx.x; i <= A.n; i += CT)
             if (i != a) out[i] = i < a ? A.tokens[(size_t)b * A.n + i] : -1;
@@ -444,14 +475,13 @@ __global__ void __launch_bounds__(CT) verify_choose_kernel(const VerifyArgs A) {
     if constexpr (GREEDY) {
         if (threadIdx.x == 0) out[a] = isfinite(s_row[0].x) ? __float_as_int(s_row[0].y) : -1;
     } else {
-        if (!sound(s_row[0])) {                                   // a row without a distribution, for the whole cluster
-            if (rank == 0 && threadIdx.x == 0) out[a] = -1;
+        if (!sound(s_row[0])) {                                   // a row without a distribution, for all CTAs of the sequence
+            if (blockIdx.x == 0 && threadIdx.x == 0) out[a] = -1;
             return;
         }
         const int away = rejected && !A.draft ? A.tokens[(size_t)b * A.n + a] : -1;
         const typename E::T *p = target + a * A.t_stride, *q = sound(s_row[1]) ? draft + a * A.d_stride : nullptr;   // a draft row without one takes nothing away
-        draw<E>(p, q, s_row[0], s_row[1], k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], A.vocab, away, shared, out + a);
-        if (rank == 0 && threadIdx.x == 0 && shared.where < 0) out[a] = away;                    // all of p lay on the rejected token
+        draw<E>(A, b, p, q, s_row[0], s_row[1], k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], away, shared, out + a);
     }
 }
 
@@ -471,15 +501,29 @@ void cut_rows(uint32_t batch, uint32_t n, uint32_t vocab, uint32_t* piece, uint3
     *pieces = (uint32_t)(((size_t)vocab + 7 + p - 1) / p);    // up to seven logits in front of the first boundary
 }
 
+// CTAs to a sequence's draw: four an SM over all sequences, while every thread has a vector of logits
+uint32_t cut_draw(uint32_t batch, uint32_t vocab) {
+    return std::max(1u, std::min({MAX_SPLITS, 148 * 4 / batch, vocab / (CT * 8)}));
+}
+
+struct Layout { size_t sums, part, total; };
+Layout lay_out(uint32_t batch, uint32_t n, uint32_t vocab) {
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    uint32_t piece, pieces;
+    cut_rows(batch, n, vocab, &piece, &pieces);
+    Layout l;
+    l.sums = up((size_t)batch * 4);
+    l.part = l.sums + up((size_t)batch * cut_draw(batch, vocab) * WARPS * sizeof(double4));
+    l.total = l.part + up((size_t)batch * (2 * n + 1) * pieces * 8);
+    return l;
+}
+
 template <class E, bool GREEDY>
 bool launch_verify(cudaStream_t st, const VerifyArgs& a) {
     const uint64_t items = ((uint64_t)a.batch * (a.n * (a.draft ? 2 : 1) + 1)) * a.pieces;
     g_launches += 2;
     if (launch_pdl(verify_rows_kernel<E, GREEDY>, dim3((uint32_t)std::min<uint64_t>((items + RT / 32 - 1) / (RT / 32), 148 * 6)), dim3(RT), 0, st, a) != cudaSuccess) return false;
-    cudaLaunchConfig_t cfg = {};
-    const uint32_t cl = GREEDY ? 1 : CL;
-    cfg.gridDim = dim3(a.batch * cl); cfg.blockDim = dim3(CT); cfg.stream = st;
-    return launch_pdl_cluster(verify_choose_kernel<E, GREEDY>, cfg, dim3(cl, 1, 1), a) == cudaSuccess;
+    return launch_pdl(verify_choose_kernel<E, GREEDY>, dim3(GREEDY ? 1 : a.splits, a.batch), dim3(CT), 0, st, a) == cudaSuccess;
 }
 
 }  // namespace
@@ -496,9 +540,7 @@ using namespace gehtp;
 
 extern "C" size_t gehtp_verify_drafts_workspace(uint32_t batch, uint32_t n_drafts, uint32_t vocab) {
     if (const char* why = verify_refuses(batch, n_drafts, vocab)) { g.last_error = why; return 0; }
-    uint32_t piece, pieces;
-    cut_rows(batch, n_drafts, vocab, &piece, &pieces);
-    return ((size_t)batch * (2 * n_drafts + 1) * pieces * 8 + 255) / 256 * 256;
+    return lay_out(batch, n_drafts, vocab).total;
 }
 
 extern "C" int gehtp_verify_drafts(const void* target_dev, const void* draft_dev, const int32_t* tokens_dev, const int32_t* n_drafts_dev,
@@ -519,10 +561,10 @@ extern "C" int gehtp_verify_drafts(const void* target_dev, const void* draft_dev
     if ((((uintptr_t)tokens_dev) | ((uintptr_t)n_drafts_dev) | ((uintptr_t)uniforms_dev) | ((uintptr_t)accepted_dev) | ((uintptr_t)out_dev)) & 3u)
         return fail("verify drafts: tokens, counts, uniforms and outputs lie on 4-byte boundaries");
     if ((uintptr_t)workspace_dev & 255u) return fail("verify drafts: the workspace lies on a 256-byte boundary");
-    const size_t need = gehtp_verify_drafts_workspace(batch, n_drafts, vocab);
-    if (workspace_bytes < need) {
+    const Layout l = lay_out(batch, n_drafts, vocab);
+    if (workspace_bytes < l.total) {
         char m[128];
-        std::snprintf(m, sizeof m, "verify drafts: needs %zu bytes of workspace, got %zu", need, workspace_bytes);
+        std::snprintf(m, sizeof m, "verify drafts: needs %zu bytes of workspace, got %zu", l.total, workspace_bytes);
         return fail(m);
     }
     if (!on_this_device(target_dev, "verify drafts: target") || (draft && !on_this_device(draft, "verify drafts: draft")) ||
@@ -536,7 +578,9 @@ extern "C" int gehtp_verify_drafts(const void* target_dev, const void* draft_dev
     cut_rows(batch, n_drafts, vocab, &a.piece, &a.pieces);
     a.t_stride = target_stride; a.d_stride = draft_stride;
     a.inv = greedy ? 0.0 : 1.0 / temperature;
-    a.part = (float2*)workspace_dev;
+    unsigned char* ws = (unsigned char*)workspace_dev;
+    a.splits = cut_draw(batch, vocab);
+    a.done = (uint32_t*)ws; a.sums = (double4*)(ws + l.sums); a.part = (float2*)(ws + l.part);
     if (!k_verify_drafts((cudaStream_t)stream, a, dtype, greedy)) {
         const cudaError_t e = cudaGetLastError();
         return fail(e == cudaSuccess ? "verify drafts: launch refused" : cudaGetErrorString(e));
