@@ -98,7 +98,7 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
     float* zone = (float*)(smem + ring_bytes<HD>());                // [16 RT][16]
     float2* ml = (float2*)(zone + 16 * RT * 16);                    // [PG][16 RT]
     uint32_t* cum = (uint32_t*)(ml + PG * 16 * RT);
-    __shared__ uint32_t s_k;
+    __shared__ uint32_t s_k, s_next;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
     const uint32_t rt = warp % RT, pg = warp / RT;
     const uint32_t ring = smem_addr(smem);
@@ -117,7 +117,17 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
     }
     const uint32_t items = prefix_items + (with_tails ? cum[A.batch] * A.kv_heads : 0);
     const size_t p_rows = A.p_rows();
-    for (uint32_t w = blockIdx.x; w < items; w += gridDim.x) {
+    // Beside the prefix's kernel most CTAs come up when that one leaves the SMs, and the first take what the others have not begun:
+    // items are handed out by a counter.
+    uint32_t w = blockIdx.x;
+    if (beside) {
+        if (threadIdx.x == 0) s_next = atomicAdd(A.next, 1u);
+        __syncthreads();
+        w = s_next;
+    }
+    while (w < items) {
+        uint32_t ahead = w + gridDim.x;
+        if (beside && threadIdx.x == 0) ahead = atomicAdd(A.next, 1u);
         // ---- the item: rows, keys, place of its partial results
         const bool tail = w >= prefix_items;
         uint32_t h, rows, token0, from, to, c = 0, n = 0, b = 0;
@@ -310,6 +320,7 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             const uint32_t r = rt * 16 + g8 + half * 8;
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+            if (r >= rows) continue;
             if (q4 == 0) ml[pg * 16 * RT + r] = make_float2(m[half], l[half]);
 #pragma unroll
             for (int j = 0; j < HD / 8; j++) *(float2*)&so[(size_t)(pg * 16 * RT + r) * LD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
@@ -360,7 +371,9 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             *(float4*)&A.part_o[(part + r) * HD + c4 * 4] = acc;
             if (c4 == 0) A.part_ml[part + r] = make_float2(M, L);
         }
+        if (threadIdx.x == 0) s_next = ahead;
         __syncthreads();
+        w = s_next;
     }
     if (beside) pdl_wait();
 }
@@ -548,7 +561,7 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     a.t_slices = std::max(1u, 6 * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    l.ml = up((size_t)(a.batch + 1) * 4);
+    l.ml = up((size_t)(a.batch + 2) * 4);
     l.o = l.ml + up(parts * 8);
     l.scores = l.o + up(parts * hd * 4);
     l.total = l.scores + (with_weights ? up((size_t)a.batch * a.kv_heads * a.q_len * a.rep * a.nslots * 4) : 0);
@@ -625,7 +638,7 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
     a.weights_in = weights_in_dev; a.weights = weights_dev; a.out = (uint16_t*)out_dev; a.q_stride = q_stride;
     a.sc = scale * 1.4426950408889634f;
     unsigned char* ws = (unsigned char*)workspace_dev;
-    a.plan = (uint32_t*)ws; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
+    a.next = (uint32_t*)ws; a.plan = a.next + 1; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
     a.scores = weights_dev ? (float*)(ws + l.scores) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = dtype == GEHTP_DT_BF16, umma = n_prefix && l.umma;

@@ -42,9 +42,17 @@ constexpr float kRaise = 8.0f;
 template <int DB, bool PAIR>
 __host__ __device__ constexpr int kv_stages() { return DB == 2 ? (PAIR ? 2 : 3) : 4; }
 
+// whether the phase is complete, without waiting
+__device__ __forceinline__ uint32_t mbar_seen(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok;
+}
+
 template <int ST>
 struct __align__(8) PBars {
-    uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full, merge;
+    uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[2], p_full[2], o_full, merge;
     uint32_t tmem_base, abort_flag;
 };
 
@@ -53,20 +61,21 @@ __device__ __forceinline__ uint64_t desc_v128(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(16384 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// 2^(s sc + off) of 32 scores (EDGE: 0 where the bit is not set), as 16 words of fp16 pairs; adds the values to l
-template <bool EDGE>
-__device__ __forceinline__ void probs32_h(const uint32_t (&v)[32], uint32_t (&w)[32], float sc, float off, uint32_t see, float2 (&l)[2]) {
+// 2^(s sc + off) of 32 scores as 16 words of fp16 pairs; adds the values to l
+__device__ __forceinline__ void probs32_h(const uint32_t (&v)[32], uint32_t (&w)[32], float sc, float off, float2 (&l)[2]) {
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         const float2 x = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), make_float2(sc, sc), make_float2(off, off));
-        float2 e = make_float2(ex2(x.x), ex2(x.y));
-        if (EDGE) {
-            e.x = (see >> (2 * i)) & 1u ? e.x : 0.0f;
-            e.y = (see >> (2 * i + 1)) & 1u ? e.y : 0.0f;
-        }
+        const float2 e = make_float2(ex2(x.x), ex2(x.y));
         l[i & 1] = add2(l[i & 1], e);
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(e.y), "f"(e.x));
     }
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
@@ -97,10 +106,7 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
 
     if (threadIdx.x == 0) {
         mbar_init(&bars->q_full, 1); mbar_init(&bars->o_full, 1); mbar_init(&bars->merge, 8);
-        for (int s = 0; s < ST; s++) {
-            mbar_init(&bars->k_full[s], 1); mbar_init(&bars->k_empty[s], 1);
-            mbar_init(&bars->v_full[s], 1); mbar_init(&bars->v_empty[s], 1);
-        }
+        for (int s = 0; s < ST; s++) { mbar_init(&bars->kv_full[s], 1); mbar_init(&bars->kv_empty[s], 1); }
         for (int s = 0; s < 2; s++) { mbar_init(&bars->s_full[s], 1); mbar_init(&bars->p_full[s], 4); }
         bars->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -114,8 +120,13 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bars->tmem_base;
     pdl_wait();
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
+        if (threadIdx.x == 0) { atomicExch(A.next, 0u); __threadfence(); }
+        __syncthreads();
+    }
     pdl_release();     // behind the wait: the tails' kernel starts beside this one and may read all that was there before the call
 
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
         if (lane == 0) {
@@ -124,102 +135,109 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
 #pragma unroll
                 for (uint32_t d = 0; d < DB; d++)
                     tma_load_3d(sQ + t * TILE + d * BOX, &tmap_q, (int)(d * 64), (int)(h * A.rep), (int)((tile0 + t) * A.p_tokens), &bars->q_full);
-            uint32_t kn = 0, vn = 0;
+            uint32_t n = 0;
             for (uint32_t j = 0; j < n_kt && !*abort_flag; j++) {
                 const uint32_t s = j % ST, ph = (j / ST) & 1;
                 const int y = (int)(from + j * BKV);
-                if (!mbar_wait_or_abort(&bars->k_empty[s], ph ^ 1, abort_flag)) { *abort_flag = 1; break; }
-                mbar_expect_tx(&bars->k_full[s], TILE);
+                if (!mbar_wait_or_abort(&bars->kv_empty[s], ph ^ 1, abort_flag)) { *abort_flag = 1; break; }
+                mbar_expect_tx(&bars->kv_full[s], 2 * TILE);
 #pragma unroll
-                for (uint32_t d = 0; d < DB; d++) tma_load_2d(sK + s * TILE + d * BOX, &tmap_kv, (int)((h * DB + d) * 64), y, &bars->k_full[s]);
-                kn++;
-                if (!mbar_wait_or_abort(&bars->v_empty[s], ph ^ 1, abort_flag)) { *abort_flag = 1; break; }
-                mbar_expect_tx(&bars->v_full[s], TILE);
+                for (uint32_t d = 0; d < DB; d++) tma_load_2d(sK + s * TILE + d * BOX, &tmap_kv, (int)((h * DB + d) * 64), y, &bars->kv_full[s]);
 #pragma unroll
-                for (uint32_t d = 0; d < DB; d++) tma_load_2d(sV + s * TILE + d * BOX, &tmap_kv, (int)(((A.kv_heads + h) * DB + d) * 64), y, &bars->v_full[s]);
-                vn++;
+                for (uint32_t d = 0; d < DB; d++) tma_load_2d(sV + s * TILE + d * BOX, &tmap_kv, (int)(((A.kv_heads + h) * DB + d) * 64), y, &bars->kv_full[s]);
+                n++;
             }
             if (*abort_flag) {   // copies already requested must land before the CTA may go away
                 mbar_wait(&bars->q_full, 0);
-                for (uint32_t j = kn > ST ? kn - ST : 0; j < kn; j++) mbar_wait(&bars->k_full[j % ST], (j / ST) & 1);
-                for (uint32_t j = vn > ST ? vn - ST : 0; j < vn; j++) mbar_wait(&bars->v_full[j % ST], (j / ST) & 1);
+                for (uint32_t j = n > ST ? n - ST : 0; j < n; j++) mbar_wait(&bars->kv_full[j % ST], (j / ST) & 1);
             }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            const uint32_t q_base = smem_u32(sQ), k_base = smem_u32(sK), v_base = smem_u32(sV);
-            bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity) {
-                if (ok) ok = mbar_wait_or_abort(bar, parity, abort_flag);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                return ok;
-            };
-            // S of group t: row tile `q` against K tile j
-            auto issue_s = [&](uint32_t t, uint32_t q, uint32_t j) {
+        // The whole warp walks the tiles, so that counters, descriptors and barrier addresses are warp-uniform values; lane 0 issues. (One
+        // lane on its own took 84 cycles to an instruction that the tensor core runs in 64. A look at a complete barrier takes some
+        // 230: K and V of a tile share one, and the next barrier is looked at while instructions in front of it are issued.)
+        const uint64_t dq = umma_desc(smem_u32(sQ)), dk = umma_desc(smem_u32(sK)), dv = desc_v128(smem_u32(sV));
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t seen = 0) {
+            if (!__all_sync(0xffffffffu, seen)) ok = __all_sync(0xffffffffu, ok && mbar_wait_or_abort(bar, parity, abort_flag));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return ok;
+        };
+        auto commit = [&](uint64_t* bar) { if (lane == 0) umma_commit(bar); };
+        // S of group t: row tile `q` against the K tile of stage s
+        auto issue_s = [&](uint32_t t, uint32_t q, uint32_t s) {
+            if (lane == 0) {
+                const uint64_t a = dq + q * (TILE >> 4), b = dk + s * (TILE >> 4);
 #pragma unroll
-                for (uint32_t d = 0; d < DB; d++)
-#pragma unroll
-                    for (uint32_t k4 = 0; k4 < 4; k4++)
-                        umma_f16(tmem + t * 128, umma_desc(q_base + q * TILE + d * BOX) + (uint64_t)(k4 * 2),
-                                 umma_desc(k_base + (j % ST) * TILE + d * BOX) + (uint64_t)(k4 * 2), idesc_f16(128) | FMT, (d | k4) ? 1u : 0u);
+                for (uint32_t k = 0; k < DB * 4; k++)
+                    umma_f16(tmem + t * 128, a + (k >> 2) * (BOX >> 4) + (k & 3) * 2, b + (k >> 2) * (BOX >> 4) + (k & 3) * 2, idesc_f16(128) | FMT, k ? 1u : 0u);
                 umma_commit(&bars->s_full[t]);
-            };
-            auto issue_o = [&](uint32_t t, uint32_t j, bool first) {
+            }
+        };
+        auto issue_o = [&](uint32_t t, uint32_t s, bool first) {
+            if (lane == 0) {
+                const uint64_t b = dv + s * (TILE >> 4);
 #pragma unroll
-                for (uint32_t part = 0; part < (BF ? 2u : 1u); part++)
+                for (uint32_t k = 0; k < 8; k++)                     // 16 positions = two 8-position groups = 2048 bytes; bit 16: B is MN-major
 #pragma unroll
-                    for (uint32_t k = 0; k < 8; k++)             // 16 positions = two 8-position groups = 2048 bytes; bit 16: B is MN-major
-                        umma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8,
-                                    desc_v128(v_base + (j % ST) * TILE + k * 2048), idesc_f16(DB * 64) | FMT | (1u << 16), (!first || part || k) ? 1u : 0u);
-            };
-            if (PAIR) {
-                if (wait(&bars->q_full, 0) && wait(&bars->k_full[0], 0)) {
-                    issue_s(0, 0, 0);
-                    if (two) issue_s(1, 1, 0);
-                    umma_commit(&bars->k_empty[0]);
+                    for (uint32_t part = 0; part < (BF ? 2u : 1u); part++)
+                        umma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, b + k * (2048 >> 4),
+                                    idesc_f16(DB * 64) | FMT | (1u << 16), (part || k) ? 1u : first ? 0u : 1u);
+            }
+        };
+        uint32_t s = 0, ph = 0, s1 = 0, ph1 = 0;                     // stage and phase of the tile whose P is next, and of the one whose S is
+        auto step = [&](uint32_t& st, uint32_t& p) { if (++st == (uint32_t)ST) { st = 0; p ^= 1; } };
+        wait(&bars->q_full, 0);
+        if (PAIR) {
+            if (wait(&bars->kv_full[0], 0)) {
+                issue_s(0, 0, 0);
+                if (two) issue_s(1, 1, 0);
+            }
+            step(s1, ph1);
+            uint32_t seen0 = 0;
+            for (uint32_t j = 0; ok && j < n_kt; j++) {
+                const bool more = j + 1 < n_kt;
+                if (!wait(&bars->p_full[0], j & 1, seen0)) break;
+                const uint32_t seen_kv = mbar_seen(&bars->kv_full[s1], ph1);
+                issue_o(0, s, j == 0);
+                const uint32_t seen1 = two ? mbar_seen(&bars->p_full[1], j & 1) : 0;
+                if (more) {
+                    if (!wait(&bars->kv_full[s1], ph1, seen_kv)) break;
+                    issue_s(0, 0, s1);
                 }
-                for (uint32_t j = 0; ok && j < n_kt; j++) {
-                    const uint32_t s = j % ST, s1 = (j + 1) % ST, ph1 = ((j + 1) / ST) & 1;
-                    const bool more = j + 1 < n_kt;
-                    if (!wait(&bars->v_full[s], (j / ST) & 1) || !wait(&bars->p_full[0], j & 1)) break;
-                    issue_o(0, j, j == 0);
-                    if (more) {
-                        if (!wait(&bars->k_full[s1], ph1)) break;
-                        issue_s(0, 0, j + 1);
-                    }
-                    if (two) {
-                        if (!wait(&bars->p_full[1], j & 1)) break;
-                        issue_o(1, j, j == 0);
-                    }
-                    umma_commit(&bars->v_empty[s]);
-                    if (more) {
-                        if (two) issue_s(1, 1, j + 1);
-                        umma_commit(&bars->k_empty[s1]);
-                    }
+                if (two) {
+                    if (!wait(&bars->p_full[1], j & 1, seen1)) break;
+                    issue_o(1, s, j == 0);
                 }
-            } else {
-                auto next_s = [&](uint32_t j) {
-                    if (!wait(&bars->k_full[j % ST], (j / ST) & 1)) return;
-                    issue_s(j & 1, 0, j);
-                    umma_commit(&bars->k_empty[j % ST]);
-                };
-                if (wait(&bars->q_full, 0)) {
-                    next_s(0);
-                    if (n_kt > 1) next_s(1);
-                }
-                for (uint32_t j = 0; ok && j < n_kt; j++) {
-                    if (!wait(&bars->v_full[j % ST], (j / ST) & 1) || !wait(&bars->p_full[j & 1], (j >> 1) & 1)) break;
-                    issue_o(j & 1, j, j < 2);
-                    umma_commit(&bars->v_empty[j % ST]);
-                    if (j + 2 < n_kt) next_s(j + 2);             // over the P just read: products run in the order they are issued
+                commit(&bars->kv_empty[s]);
+                seen0 = mbar_seen(&bars->p_full[0], (j + 1) & 1);
+                if (more && two) issue_s(1, 1, s1);
+                step(s, ph);
+                step(s1, ph1);
+            }
+        } else {
+            for (uint32_t j = 0; j < 2 && j < n_kt && wait(&bars->kv_full[s1], ph1); j++) {
+                issue_s(j, 0, s1);
+                step(s1, ph1);
+            }
+            for (uint32_t j = 0; ok && j < n_kt; j++) {
+                if (!wait(&bars->p_full[j & 1], (j >> 1) & 1)) break;
+                issue_o(j & 1, s, j < 2);
+                commit(&bars->kv_empty[s]);
+                step(s, ph);
+                if (j + 2 < n_kt) {                                  // over the P just read: products run in the order they are issued
+                    if (!wait(&bars->kv_full[s1], ph1)) break;
+                    issue_s(j & 1, 0, s1);
+                    step(s1, ph1);
                 }
             }
-            if (ok) umma_commit(&bars->o_full);
-            else *abort_flag = 1;
         }
+        if (ok) commit(&bars->o_full);
+        else if (lane == 0) *abort_flag = 1;
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax and output: one thread per row and group
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");    // 256 x 200 + 128 x 104 = 384 x 168, what the CTA was launched with
         const uint32_t t = (warp - 4) >> 2, quarter = warp & 3;
         const uint32_t ts = tmem + ((quarter * 32) << 16) + t * 128, to_ = ts + 256;
         float m = -INFINITY;
@@ -232,19 +250,24 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
             ok = !__any_sync(0xffffffffu, *abort_flag != 0) && __all_sync(0xffffffffu, mbar_wait_or_abort(&bars->s_full[t], round & 1, abort_flag));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t v[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(ts + c * 32, v[c]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld_wait(v[c]);
             const int hi = (int)(A.n_prefix - 1 - (from + j * BKV));       // last column of the tile that is a position of the prefix
-            const bool edge = hi < (int)BKV - 1;
-            float mt = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < 2; c++) {
-                uint32_t va[32], vb[32];
-                tmem_ld32(ts + c * 64, va);
-                tmem_ld32(ts + c * 64 + 32, vb);
-                tmem_ld_wait(va);
-                tmem_ld_wait(vb);
-                if (edge) mt = fmaxf(mt, fmaxf(max32<true>(va, visible32(c * 64, 0, hi)), max32<true>(vb, visible32(c * 64 + 32, 0, hi))));
-                else mt = fmaxf(mt, fmaxf(max32<false>(va, 0u), max32<false>(vb, 0u)));
+            if (hi < (int)BKV - 1) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[c][i] = c * 32 + i <= hi ? v[c][i] : 0xff800000u;
             }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+            float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
             mt *= A.sc;
             // s_full of this tile came after the group's products of the tile before: its O is at rest
             const bool raise = mt > m + kRaise;
@@ -267,27 +290,16 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
                 }
             }
             const float off = m == -INFINITY ? 0.0f : -m;
-            auto probs = [&](const uint32_t (&v)[32], uint32_t col) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
                 uint32_t w[32];
                 if (BF) {
-                    if (edge) probs32<true>(v, w, A.sc, off, visible32((int)col, 0, hi), l2);
-                    else probs32<false>(v, w, A.sc, off, 0u, l2);
-                    tmem_st32(ts + col, w);
+                    probs32<false>(v[c], w, A.sc, off, 0u, l2);
+                    tmem_st32(ts + c * 32, w);
                 } else {
-                    if (edge) probs32_h<true>(v, w, A.sc, off, visible32((int)col, 0, hi), l2);
-                    else probs32_h<false>(v, w, A.sc, off, 0u, l2);
-                    tmem_st16(ts + col, w);
+                    probs32_h(v[c], w, A.sc, off, l2);
+                    tmem_st16(ts + c * 32, w);
                 }
-            };
-#pragma unroll 1
-            for (int c = 0; c < 2; c++) {
-                uint32_t va[32], vb[32];
-                tmem_ld32(ts + c * 64, va);
-                tmem_ld_wait(va);
-                tmem_ld32(ts + c * 64 + 32, vb);
-                probs(va, c * 64);
-                tmem_ld_wait(vb);
-                probs(vb, c * 64 + 32);
             }
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
