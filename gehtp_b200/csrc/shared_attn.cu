@@ -6,10 +6,11 @@
 // read once for all sequences: its keys meet the rows of all of them, rep query heads to a key head. Rows of one tail are few
 // (q_len * rep). No row's result depends on a position that it does not see, whatever is cached there.
 //
-// shared_parts_kernel: CTAs that stay and walk the items (row tile, key head, slice of the prefix) and (sequence, key head, slice of
-// its tail). K and V tiles of 64 positions by cp.async in three or four stages; a warp has 16 rows and a quarter, a half or all of
-// a tile's positions; S and P stay in registers (mma.sync m16n8k16). How a batch's tails are cut follows from their lengths,
-// which lie on the device: every CTA works that out for itself.
+// Items of work: (row tile, key head, slice of the prefix) and (sequence, key head, slice of its tail). How a batch's tails are cut follows
+// from their lengths, which lie on the device: every CTA works that out for itself. S and P stay in registers (mma.sync m16n8k16).
+// shared_warps_kernel: up to 16 rows to a key head, an item to a warp.
+// shared_parts_kernel: more rows, an item to a CTA; K and V tiles of 64 positions by cp.async in two to four stages, a warp has 16 rows and
+// a half or all of a tile's positions.
 // shared_merge_kernel: partial results of a row together; where asked for, the weights of the tail positions.
 #include <climits>
 #include <cmath>
@@ -80,6 +81,266 @@ __device__ uint32_t cut_tails(const SharedArgs& A, uint32_t* cum) {
     return k;
 }
 
+// What an item has to do: rows against keys, and the place of its partial results.
+struct Item {
+    bool tail, last;                       // last: it holds the end of a tail
+    uint32_t h, rows, token0, from, to;    // key head; rows, their first token; positions
+    uint32_t b, n, c;                      // of a tail: its sequence, its length, positions that all rows see
+    size_t v_off, part;                    // from a key to its value, half of what lies between two keys; first partial row
+    const uint16_t* kbase;
+};
+
+template <int HD>
+__device__ __forceinline__ Item item_of(const SharedArgs& A, const uint32_t* cum, uint32_t k, uint32_t w, uint32_t prefix_items) {
+    Item I;
+    I.tail = w >= prefix_items;
+    I.last = false;
+    I.b = I.n = I.c = 0;
+    if (!I.tail) {
+        const uint32_t tile = w % A.p_tiles, u = w / A.p_tiles, s = u / A.kv_heads;
+        I.h = u % A.kv_heads;
+        I.token0 = tile * A.p_tokens;
+        I.rows = min(A.p_tokens, A.batch * A.q_len - I.token0) * A.rep;
+        I.from = s * A.p_len;
+        I.to = min(A.n_prefix, I.from + A.p_len);
+        I.v_off = (size_t)A.kv_heads * HD;
+        I.kbase = A.prefix + (size_t)I.h * HD;
+        I.part = (((size_t)tile * A.kv_heads + I.h) * A.p_slices + s) * (A.p_tokens * A.rep);
+    } else {
+        const uint32_t u = (w - prefix_items) / A.kv_heads;
+        I.h = (w - prefix_items) % A.kv_heads;
+        uint32_t b = 0, hi = A.batch;                              // cum[b] <= u < cum[b + 1]
+        while (hi - b > 1) {
+            const uint32_t mid = (b + hi) / 2;
+            if (cum[mid] <= u) b = mid; else hi = mid;
+        }
+        I.b = b;
+        I.n = tail_length(A, b);
+        I.c = common_length(A, I.n);
+        I.token0 = b * A.q_len;
+        I.rows = A.q_len * A.rep;
+        I.from = (u - cum[b]) * k * TILE;
+        I.last = u + 1 == cum[b + 1];
+        I.to = I.last ? I.n : I.from + k * TILE;
+        I.v_off = (size_t)A.batch * A.kv_heads * HD;
+        I.kbase = A.tail + ((size_t)b * A.kv_heads + I.h) * HD;
+        I.part = A.p_rows() + ((size_t)u * A.kv_heads + I.h) * I.rows;
+    }
+    return I;
+}
+
+// Up to 16 rows to a key head: a warp to an item, on its own. Tiles of 16 positions by cp.async into the warp's stages; no barrier in the
+// loop, so that what an item costs to begin and to end is other warps' time.
+template <int HD>
+__host__ __device__ constexpr int warp_stages() { return HD == 128 ? 3 : 6; }
+template <int HD>
+__host__ __device__ constexpr size_t warps_smem() { return (size_t)4 * warp_stages<HD>() * 64 * HD + (MAX_BATCH + 4) * 4; }
+
+template <bool BF, int HD>
+__global__ void __launch_bounds__(128, 2) shared_warps_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
+    constexpr uint32_t ST = warp_stages<HD>(), ROW = HD * 2, HALF = 16 * ROW;
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint32_t* cum = (uint32_t*)(smem + 4 * ST * 2 * HALF);
+    __shared__ uint32_t s_k;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
+    const uint32_t ring = smem_addr(smem) + warp * ST * 2 * HALF;
+    // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait: all that was there before the
+    // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
+    if (!beside) pdl_wait();
+    pdl_release();
+    if (with_tails) {
+        if (warp == 0) {
+            const uint32_t k = cut_tails(A, cum);
+            if (lane == 0) s_k = k;
+        }
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (uint32_t b = threadIdx.x; b <= A.batch; b += 128) A.plan[b] = cum[b];
+    }
+    const uint32_t items = prefix_items + (with_tails ? cum[A.batch] * A.kv_heads : 0), k = with_tails ? s_k : 0;
+    // Beside the prefix's kernel most CTAs come up when that one leaves the SMs, and the first take what the others have not begun:
+    // items are handed out by a counter.
+    auto next_item = [&](uint32_t w) {
+        if (!beside) return w + gridDim.x * 4;
+        if (lane == 0) w = atomicAdd(A.next, 1u);
+        return __shfl_sync(0xffffffffu, w, 0);
+    };
+    for (uint32_t w = beside ? next_item(0) : blockIdx.x + gridDim.x * warp, ahead; w < items; w = ahead) {
+        ahead = next_item(w);
+        const Item I = item_of<HD>(A, cum, k, w, prefix_items);
+        const size_t pitch = 2 * I.v_off;
+        const uint32_t tiles = (I.to - I.from + 15) / 16;
+        auto load = [&](uint32_t i) {
+            if (i < tiles) {
+                const uint32_t st = ring + (i % ST) * 2 * HALF;
+#pragma unroll
+                for (uint32_t u = 0; u < HD / 16; u++) {
+                    const uint32_t e = u * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), pos = I.from + i * 16 + r;
+                    const bool in = pos < I.to;                     // rows past the end: zeros, whatever the cache holds there
+                    const uint16_t* src = I.kbase + (in ? (size_t)pos * pitch + ch * 8 : 0);
+                    const uint32_t dst = st + r * ROW + ((ch ^ (r & 7)) * 16);
+                    cp16(dst, src, in ? 16 : 0);
+                    cp16(dst + HALF, src + (in ? I.v_off : 0), in ? 16 : 0);
+                }
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < ST - 1; i++) load(i);
+        uint32_t qf[HD / 16][4];
+        int lim[2];                                                   // the first position that a row does not see
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t r = g8 + half * 8;
+            const bool in = r < I.rows;
+            lim[half] = I.last ? min((int)I.to, (int)(I.n + r / A.rep + 1) - (int)A.q_len) : (int)I.to;
+            const uint16_t* qp = A.q + (in ? (size_t)(I.token0 + r / A.rep) * A.q_stride + (size_t)(I.h * A.rep + r % A.rep) * HD : 0) + q4 * 2;
+#pragma unroll
+            for (int x = 0; x < HD / 16; x++) {
+                qf[x][half] = in ? *(const uint32_t*)(qp + x * 16) : 0u;
+                qf[x][half + 2] = in ? *(const uint32_t*)(qp + x * 16 + 8) : 0u;
+            }
+        }
+        float o[HD / 8][4] = {};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (uint32_t i = 0; i < tiles; i++) {
+            cp_wait<ST - 2>();
+            __syncwarp();
+            load(i + ST - 1);                                         // over the tile before, which the whole warp has read
+            const uint32_t p0 = I.from + i * 16, kt = ring + (i % ST) * 2 * HALF, vt = kt + HALF;
+            float s[2][4] = {};
+            {
+                const uint32_t r = (lane & 7) + ((lane >> 4) & 1) * 8;
+#pragma unroll
+                for (int x = 0; x < HD / 16; x++) {
+                    uint32_t f[4];
+                    ldsm4(f, kt + r * ROW + (((2 * x + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+                    mma16<BF>(s[0], qf[x], f[0], f[1]);
+                    mma16<BF>(s[1], qf[x], f[2], f[3]);
+                }
+            }
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool in = (int)(p0 + t * 8 + q4 * 2 + (e & 1)) < lim[e >> 1];
+                    s[t][e] = in ? s[t][e] * A.sc : -INFINITY;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+                }
+            if (I.tail && A.scores) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const uint32_t r = g8 + half * 8;
+                    float* sp = A.scores + (((size_t)I.b * A.kv_heads + I.h) * I.rows + r) * A.nslots;
+                    if (r < I.rows)
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            const uint32_t p = p0 + t * 8 + q4 * 2;
+                            if (p < I.to) sp[p] = s[t][2 * half];
+                            if (p + 1 < I.to) sp[p + 1] = s[t][2 * half + 1];
+                        }
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
+            }
+            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const float mn = fmaxf(m[half], mx[half]), f = m[half] == -INFINITY ? 0.0f : sm100::ex2(m[half] - mn);
+                    if (mn > m[half]) {
+                        m[half] = mn;
+                        l[half] *= f;
+#pragma unroll
+                        for (int j = 0; j < HD / 8; j++) { o[j][2 * half] *= f; o[j][2 * half + 1] *= f; }
+                    }
+                }
+            }
+            const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[t][e] = sm100::ex2(s[t][e] - off[e >> 1]);
+                    l[e >> 1] += s[t][e];
+                }
+            // Positions that only some rows see have weight 0 for the others, which is 0 times their values: where one of those is no
+            // number, the tile's values are added row by row instead.
+            bool odd = false;
+            if (I.last && p0 + 16 > I.c && I.n > I.c) {
+                constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
+#pragma unroll 1
+                for (uint32_t u = 0; u < HD / 16; u++) {
+                    const uint32_t e = u * 32 + lane, r = e / (HD / 8);
+                    const uint4 v = *(const uint4*)(smem + (vt - smem_addr(smem)) + r * ROW + ((e % (HD / 8)) ^ (r & 7)) * 16);
+                    for (uint32_t x : {v.x, v.y, v.z, v.w}) odd |= (x & EXP & 0xffffu) == (EXP & 0xffffu) || (x & EXP & 0xffff0000u) == (EXP & 0xffff0000u);
+                }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+            if (odd) {
+#pragma unroll 1
+                for (uint32_t col = 0; col < 16; col++) {
+                    const int from = (int)((lane & ~3u) + (col % 8) / 2);
+                    float p[2];
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const float a = col < 8 ? s[0][2 * half] : s[1][2 * half], b = col < 8 ? s[0][2 * half + 1] : s[1][2 * half + 1];
+                        p[half] = __shfl_sync(0xffffffffu, col % 2 ? b : a, from);
+                    }
+#pragma unroll
+                    for (int j = 0; j < HD / 8; j++) {
+                        const float2 v = unpack2<BF>(*(const uint32_t*)(smem + (vt - smem_addr(smem)) + col * ROW + ((j ^ (col & 7)) * 16) + q4 * 4));
+#pragma unroll
+                        for (int half = 0; half < 2; half++)
+                            if ((int)(p0 + col) < lim[half]) { o[j][2 * half] = fmaf(p[half], v.x, o[j][2 * half]); o[j][2 * half + 1] = fmaf(p[half], v.y, o[j][2 * half + 1]); }
+                    }
+                }
+                continue;
+            }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {                          // fragment register e: tile e / 2, rows of half e % 2
+                const float a = s[e >> 1][2 * (e & 1)], c2 = s[e >> 1][2 * (e & 1) + 1];
+                hi[e] = pack2<BF>(a, c2);
+                // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
+                if (BF) {
+                    const float2 u = unpack2<BF>(hi[e]);
+                    lo[e] = pack2<BF>(a - u.x, c2 - u.y);
+                }
+            }
+            const uint32_t r = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) {
+                uint32_t f[4];
+                ldsm4_t(f, vt + r * ROW + (((2 * j + ((lane >> 4) & 1)) ^ (r & 7)) * 16));
+                mma16<BF>(o[2 * j], hi, f[0], f[1]);
+                mma16<BF>(o[2 * j + 1], hi, f[2], f[3]);
+                if (BF) {
+                    mma16<BF>(o[2 * j], lo, f[0], f[1]);
+                    mma16<BF>(o[2 * j + 1], lo, f[2], f[3]);
+                }
+            }
+        }
+        cp_wait<0>();
+        __syncwarp();                                              // the next item's tiles go over the ones just read
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t r = g8 + half * 8;
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+            if (r < I.rows) {
+                if (q4 == 0) A.part_ml[I.part + r] = make_float2(m[half], l[half]);
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) *(float2*)&A.part_o[(I.part + r) * HD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+            }
+        }
+    }
+    if (beside) pdl_wait();
+}
+
 template <int HD>
 __host__ __device__ constexpr int stages() { return HD == 128 ? 3 : 4; }
 template <int HD>
@@ -116,7 +377,6 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             for (uint32_t b = threadIdx.x; b <= A.batch; b += NT) A.plan[b] = cum[b];
     }
     const uint32_t items = prefix_items + (with_tails ? cum[A.batch] * A.kv_heads : 0);
-    const size_t p_rows = A.p_rows();
     // Beside the prefix's kernel most CTAs come up when that one leaves the SMs, and the first take what the others have not begun:
     // items are handed out by a counter.
     uint32_t w = blockIdx.x;
@@ -128,42 +388,12 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
     while (w < items) {
         uint32_t ahead = w + gridDim.x;
         if (beside && threadIdx.x == 0) ahead = atomicAdd(A.next, 1u);
-        // ---- the item: rows, keys, place of its partial results
-        const bool tail = w >= prefix_items;
-        uint32_t h, rows, token0, from, to, c = 0, n = 0, b = 0;
-        size_t pitch, v_off, part;
-        const uint16_t* kbase;
-        bool last = false;
-        if (!tail) {
-            const uint32_t tile = w % A.p_tiles, u = w / A.p_tiles, s = u / A.kv_heads;
-            h = u % A.kv_heads;
-            token0 = tile * A.p_tokens;
-            rows = min(A.p_tokens, A.batch * A.q_len - token0) * A.rep;
-            from = s * A.p_len;
-            to = min(A.n_prefix, from + A.p_len);
-            v_off = (size_t)A.kv_heads * HD;
-            kbase = A.prefix + (size_t)h * HD;
-            part = (((size_t)tile * A.kv_heads + h) * A.p_slices + s) * (A.p_tokens * A.rep);
-        } else {
-            const uint32_t u = (w - prefix_items) / A.kv_heads;
-            h = (w - prefix_items) % A.kv_heads;
-            uint32_t hi = A.batch;                                  // cum[b] <= u < cum[b + 1]
-            while (hi - b > 1) {
-                const uint32_t mid = (b + hi) / 2;
-                if (cum[mid] <= u) b = mid; else hi = mid;
-            }
-            n = tail_length(A, b);
-            c = common_length(A, n);
-            token0 = b * A.q_len;
-            rows = A.q_len * A.rep;
-            from = (u - cum[b]) * s_k * TILE;
-            last = u + 1 == cum[b + 1];
-            to = last ? n : from + s_k * TILE;
-            v_off = (size_t)A.batch * A.kv_heads * HD;
-            kbase = A.tail + ((size_t)b * A.kv_heads + h) * HD;
-            part = p_rows + ((size_t)u * A.kv_heads + h) * rows;
-        }
-        pitch = 2 * v_off;
+        const Item I = item_of<HD>(A, cum, s_k, w, prefix_items);
+        const bool tail = I.tail, last = I.last;
+        const uint32_t h = I.h, rows = I.rows, token0 = I.token0, from = I.from, c = I.c, n = I.n, b = I.b;
+        const size_t v_off = I.v_off, pitch = 2 * v_off, part = I.part;
+        const uint16_t* kbase = I.kbase;
+        uint32_t to = I.to;
         uint32_t tiles = (to - from + TILE - 1) / TILE;
 
         auto load = [&](uint32_t i) {
@@ -501,9 +731,19 @@ bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, b
                       prefix_items, tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
 }
 template <bool BF, int HD>
+bool launch_warps(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, bool tails, bool beside) {
+    static int have[64] = {};
+    if (!ensure_dyn_smem(shared_warps_kernel<BF, HD>, warps_smem<HD>(), have)) return false;
+    const size_t items = prefix_items + (tails ? ((size_t)a.t_slices + a.batch) * a.kv_heads : 0);
+    if (!items) return true;
+    g_launches++;
+    return launch_pdl(shared_warps_kernel<BF, HD>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * 2)), dim3(128), warps_smem<HD>(), st, a, prefix_items,
+                      tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
+}
+template <bool BF, int HD>
 bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t prefix_items, bool tails, bool beside) {
     switch (rt) {
-        case 1: return launch_parts<BF, HD, 1>(st, a, prefix_items, tails, beside);
+        case 1: return launch_warps<BF, HD>(st, a, prefix_items, tails, beside);
         case 2: return launch_parts<BF, HD, 2>(st, a, prefix_items, tails, beside);
         case 4: return launch_parts<BF, HD, 4>(st, a, prefix_items, tails, beside);
         default: return launch_parts<BF, HD, 8>(st, a, prefix_items, tails, beside);
@@ -547,18 +787,18 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     const uint32_t unit = l.umma ? 128 : TILE, tiles = (a.n_prefix + unit - 1) / unit;
     a.p_slices = a.p_len = 0;
     if (tiles) {
-        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * (l.t_rt == 8 ? 1 : 2);
-        uint32_t best = 1;
+        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * (l.t_rt == 8 ? 1 : l.t_rt == 1 ? 8 : 2);
+        uint32_t best = l.umma ? 1 : std::min(tiles, std::max(1u, fit / groups));
         size_t least = SIZE_MAX;
         // rounds over the SMs of slices and about three tiles' time to begin and end one
-        for (uint32_t s = 1; s <= std::min(tiles, fit); s++) {
+        for (uint32_t s = 1; l.umma && s <= std::min(tiles, fit); s++) {
             const size_t cost = ((size_t)groups * s + fit - 1) / fit * ((tiles + s - 1) / s + 3);
             if (cost < least) { least = cost; best = s; }
         }
         a.p_len = (tiles + best - 1) / best * unit;
         a.p_slices = (a.n_prefix + a.p_len - 1) / a.p_len;
     }
-    a.t_slices = std::max(1u, 6 * SMS / a.kv_heads);
+    a.t_slices = std::max(1u, (l.t_rt == 1 ? 24 : 6) * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     l.ml = up((size_t)(a.batch + 2) * 4);
