@@ -16,6 +16,7 @@
 // true c, one pass gives sum(e_p - c0 e_q) and sum(e_q) over the tokens where e_p > c0 e_q, and so sum(e_p - c e_q) = the first -
 // (c - c0) times the second; tokens whose e_p / e_q lies between c0 and c (some 2^-22 wide) are off by no more than that width
 // squared. Where p and q are so alike that this could show (a sum below 2^-10) the row is read once more with the true c.
+#include <cooperative_groups.h>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -29,8 +30,12 @@ namespace gehtp {
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr uint32_t MAX_DRAFTS = 64, MAX_SPLITS = 64;
 constexpr int RT = 256, CT = 256, WARPS = CT / 32;
+constexpr int CL = 8, GT = 512;             // T = 0 in one launch: CTAs of a cluster, their threads
+constexpr uint32_t MAX_ROWS = 16;           // and the rows that it takes
 
 struct VerifyArgs {
     const void *target, *draft;             // draft NULL: drafts without probabilities (and always with T = 0)
@@ -116,12 +121,92 @@ __device__ __forceinline__ bool ahead(float a, int pa, float b, int pb) {
     return a > b || ((a == b || na) && pa < pb);
 }
 
+template <bool GREEDY>
+__device__ __forceinline__ float2 together(float2 a, float2 b, float k) {
+    if (GREEDY) return ahead(b.x, __float_as_int(b.y), a.x, __float_as_int(a.y)) ? b : a;
+    return join(a, b, k);
+}
+// Parts of a row in N neighbouring lanes together (N a power of two); every one of them has the result.
+template <bool GREEDY, int N>
+__device__ __forceinline__ float2 join_lanes(float2 x, float k) {
+#pragma unroll
+    for (int o = N / 2; o; o >>= 1) x = together<GREEDY>(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)), k);
+    return x;
+}
+
 constexpr int AHEAD = 4;                    // loads of a thread in flight
+
+// {maximum, sum of 2^((x - maximum) k)} - GREEDY: {maximum, its place} - of the logits first .. end, by one warp; every lane has it.
+// first is on a 16-byte boundary, or in front of the row by less than a vector.
+template <class E, bool GREEDY>
+__device__ __forceinline__ float2 part_of_row(const typename E::T* p, int64_t first, int64_t end, float k) {
+    const uint32_t lane = threadIdx.x & 31;
+    float2 best = make_float2(-INFINITY, 0.0f);
+    int place = INT_MAX;
+    bool odd = false;                                                // GREEDY: some logit is no number
+    constexpr int64_t STEP = 32 * E::V;
+    // N vectors of places e, e + STEP, ... together: one look at the maximum
+    auto take = [&](const auto& x, int64_t e) {
+        constexpr int N = sizeof(x) / sizeof(float);
+        if (GREEDY) {
+#pragma unroll
+            for (int j = 0; j < N; j++) {                            // a lane's places ascend: the first of equal ones stays
+                odd |= x[j] != x[j];
+                if (x[j] > best.x) { best.x = x[j]; place = (int)(e + (j / E::V) * STEP + j % E::V); }
+            }
+        } else {
+            float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int j = 4; j < N; j++) m[j & 3] = fmaxf(m[j & 3], x[j]);
+            m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            if (m[0] > best.x) {
+                best.y = best.x == -INFINITY ? best.y : best.y * sm100::ex2((best.x - m[0]) * k);
+                best.x = m[0];
+            }
+            const float off = best.x == -INFINITY ? 0.0f : best.x;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < N; j++) sum[j & 3] += sm100::ex2((x[j] - off) * k);
+            best.y += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+    };
+    int64_t e = first + lane * E::V;
+    if (e < 0 && end > 0) {                                          // in front of the row's first boundary
+        float x[E::V];
+        load_logits<E>(p, e, end, x);
+        take(x, e);
+        e += STEP;
+    }
+    for (; e + (AHEAD - 1) * STEP + E::V <= end; e += AHEAD * STEP) {
+        uint4 w[AHEAD];
+        float x[AHEAD * E::V];
+#pragma unroll
+        for (int u2 = 0; u2 < AHEAD; u2++) w[u2] = __ldg((const uint4*)(p + e + u2 * STEP));
+#pragma unroll
+        for (int u2 = 0; u2 < AHEAD; u2++) {
+            float y[E::V];
+            unpack_logits<E>(w[u2], y);
+#pragma unroll
+            for (int j = 0; j < E::V; j++) x[u2 * E::V + j] = y[j];
+        }
+        take(x, e);
+    }
+    for (; e < end; e += STEP) {
+        float x[E::V];
+        load_logits<E>(p, e, end, x);
+        take(x, e);
+    }
+    __syncwarp();
+    if (GREEDY) {
+        if (odd) { best.x = NAN; place = 0; }
+        best.y = __int_as_float(place);
+    }
+    return join_lanes<GREEDY, 32>(best, k);
+}
 
 // A warp to a piece of a row, CTAs that stay. Rows in the order of their drafts, so that all CTAs have like shares of the ones that are there.
 template <class E, bool GREEDY>
 __global__ void __launch_bounds__(RT) verify_rows_kernel(const VerifyArgs A) {
-    const uint32_t lane = threadIdx.x & 31;
     pdl_wait();
     pdl_release();
     const uint32_t kinds = A.draft ? 2 : 1, rows = A.batch * (A.n * kinds + 1);
@@ -135,97 +220,18 @@ __global__ void __launch_bounds__(RT) verify_rows_kernel(const VerifyArgs A) {
         if (i >= drafts_of(A, b) + (target ? 1 : 0)) continue;
         const size_t row = target ? (size_t)b * (A.n + 1) + i : (size_t)b * A.n + i;
         const typename E::T* p = target ? (const typename E::T*)A.target + row * A.t_stride : (const typename E::T*)A.draft + row * A.d_stride;
-        const int64_t first = (int64_t)piece * A.piece - lead<E>(p), end = piece + 1 == A.pieces ? (int64_t)A.vocab : min((int64_t)A.vocab, first + A.piece);
-        float2 best = make_float2(-INFINITY, 0.0f);
-        int place = 0x7fffffff;
-        bool odd = false;                                            // T = 0: some logit is no number
-        // N vectors of places e, e + STEP, ... together: one look at the maximum
-        constexpr int64_t STEP = 32 * E::V;
-        auto take = [&](const auto& x, int64_t e) {
-            constexpr int N = sizeof(x) / sizeof(float);
-            if (GREEDY) {
-#pragma unroll
-                for (int j = 0; j < N; j++) {                        // a lane's places ascend: the first of equal ones stays
-                    odd |= x[j] != x[j];
-                    if (x[j] > best.x) { best.x = x[j]; place = (int)(e + (j / E::V) * STEP + j % E::V); }
-                }
-            } else {
-                float m[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int j = 4; j < N; j++) m[j & 3] = fmaxf(m[j & 3], x[j]);
-                m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                if (m[0] > best.x) {
-                    best.y = best.x == -INFINITY ? best.y : best.y * sm100::ex2((best.x - m[0]) * k);
-                    best.x = m[0];
-                }
-                const float off = best.x == -INFINITY ? 0.0f : best.x;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < N; j++) sum[j & 3] += sm100::ex2((x[j] - off) * k);
-                best.y += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            }
-        };
-        int64_t e = first + lane * E::V;
-        if (e < 0) {                                                 // in front of the row's first boundary
-            float x[E::V];
-            load_logits<E>(p, e, end, x);
-            take(x, e);
-            e += STEP;
-        }
-        for (; e + (AHEAD - 1) * STEP + E::V <= end; e += AHEAD * STEP) {
-            uint4 w[AHEAD];
-            float x[AHEAD * E::V];
-#pragma unroll
-            for (int u2 = 0; u2 < AHEAD; u2++) w[u2] = __ldg((const uint4*)(p + e + u2 * STEP));
-#pragma unroll
-            for (int u2 = 0; u2 < AHEAD; u2++) {
-                float y[E::V];
-                unpack_logits<E>(w[u2], y);
-#pragma unroll
-                for (int j = 0; j < E::V; j++) x[u2 * E::V + j] = y[j];
-            }
-            take(x, e);
-        }
-        for (; e < end; e += STEP) {
-            float x[E::V];
-            load_logits<E>(p, e, end, x);
-            take(x, e);
-        }
-        __syncwarp();
-        if (GREEDY) {
-            if (odd) { best.x = NAN; place = 0; }
-            for (int o = 16; o; o >>= 1) {
-                const float y = __shfl_xor_sync(0xffffffffu, best.x, o);
-                const int q = __shfl_xor_sync(0xffffffffu, place, o);
-                if (ahead(y, q, best.x, place)) { best.x = y; place = q; }
-            }
-            best.y = __int_as_float(place);
-        } else {
-            for (int o = 16; o; o >>= 1) {
-                const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.y, o));
-                best = join(best, y, k);
-            }
-        }
-        if (lane == 0) A.part[(row + (target ? 0 : (size_t)A.batch * (A.n + 1))) * A.pieces + piece] = best;
+        const int64_t first = (int64_t)piece * A.piece - lead<E>(p);
+        const float2 best = part_of_row<E, GREEDY>(p, first, piece + 1 == A.pieces ? (int64_t)A.vocab : min((int64_t)A.vocab, first + A.piece), k);
+        if ((threadIdx.x & 31) == 0) A.part[(row + (target ? 0 : (size_t)A.batch * (A.n + 1))) * A.pieces + piece] = best;
     }
 }
 
 // A row's parts together, by one warp.
 template <bool GREEDY>
-__device__ __forceinline__ float2 whole_row(const VerifyArgs& A, size_t row) {
-    const float k = (float)(A.inv * 1.4426950408889634);
-    float2 x = make_float2(-INFINITY, GREEDY ? __int_as_float(0x7fffffff) : 0.0f);
-    for (uint32_t i = threadIdx.x & 31; i < A.pieces; i += 32) {
-        const float2 y = __ldcg(&A.part[row * A.pieces + i]);
-        if (GREEDY) { if (ahead(y.x, __float_as_int(y.y), x.x, __float_as_int(x.y))) x = y; }
-        else x = join(x, y, k);
-    }
-    for (int o = 16; o; o >>= 1) {
-        const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o));
-        if (GREEDY) { if (ahead(y.x, __float_as_int(y.y), x.x, __float_as_int(x.y))) x = y; }
-        else x = join(x, y, k);
-    }
-    return x;
+__device__ __forceinline__ float2 whole_row(const float2* part, uint32_t pieces, float k) {
+    float2 x = make_float2(-INFINITY, GREEDY ? __int_as_float(INT_MAX) : 0.0f);
+    for (uint32_t i = threadIdx.x & 31; i < pieces; i += 32) x = together<GREEDY>(x, part[i], k);
+    return join_lanes<GREEDY, 32>(x, k);
 }
 __device__ __forceinline__ bool sound(float2 x) { return x.y > 0.0f && isfinite(x.y) && isfinite(x.x); }
 
@@ -420,6 +426,14 @@ __device__ __forceinline__ void draw(const VerifyArgs& A, uint32_t b, const type
     if (threadIdx.x == 0) *to_ = S.first != INT_MAX ? S.first : S.last;
 }
 
+// What a sequence gets: `a` accepted drafts, -1 behind the token that follows them.
+__device__ __forceinline__ void write_accepted(const VerifyArgs& A, uint32_t b, uint32_t a) {
+    int32_t* out = A.out + (size_t)b * (A.n + 1);
+    if (threadIdx.x == 0) A.accepted[b] = (int)a;
+    for (uint32_t i = threadIdx.x; i <= A.n; i += blockDim.x)
+        if (i != a) out[i] = i < a ? A.tokens[(size_t)b * A.n + i] : -1;
+}
+
 // grid: (CTAs of a sequence, sequences)
 template <class E, bool GREEDY>
 __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A) {
@@ -432,12 +446,13 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
     const uint32_t nd = drafts_of(A, b);
     const typename E::T *target = (const typename E::T*)A.target + (size_t)b * (A.n + 1) * A.t_stride, *draft = (const typename E::T*)A.draft + (size_t)b * A.n * A.d_stride;
     const double k = A.inv * 1.4426950408889634;
+    const float2 *t_part = A.part + (size_t)b * (A.n + 1) * A.pieces, *d_part = A.part + ((size_t)A.batch * (A.n + 1) + (size_t)b * A.n) * A.pieces;
     // ---- which drafts pass
     for (uint32_t i = warp; i < nd; i += WARPS) {
         const int x = A.tokens[(size_t)b * A.n + i];
         const bool in = x >= 0 && (uint32_t)x < A.vocab;
         const double lp = !GREEDY && in ? (double)E::f(target[i * A.t_stride + x]) : 0.0, lq = !GREEDY && in && A.draft ? (double)E::f(draft[i * A.d_stride + x]) : 0.0;
-        const float2 p = whole_row<GREEDY>(A, (size_t)b * (A.n + 1) + i);
+        const float2 p = whole_row<GREEDY>(t_part + (size_t)i * A.pieces, A.pieces, (float)k);
         bool ok;
         if (GREEDY) {
             ok = isfinite(p.x) && x == __float_as_int(p.y);
@@ -446,7 +461,7 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
             ok = sound(p);
             if (ok && in) px = exp2((lp - p.x) * k) / p.y;
             if (A.draft) {
-                const float2 q = whole_row<false>(A, (size_t)A.batch * (A.n + 1) + (size_t)b * A.n + i);
+                const float2 q = whole_row<false>(d_part + (size_t)i * A.pieces, A.pieces, (float)k);
                 ok = ok && sound(q);
                 qx = ok && in ? exp2((lq - q.x) * k) / q.y : 0.0;
             }
@@ -458,31 +473,61 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
     uint32_t a = 0;
     while (a < nd && pass[a]) a++;
     const bool rejected = a < nd;
-    int32_t* out = A.out + (size_t)b * (A.n + 1);
-    if (blockIdx.x == 0) {
-        if (threadIdx.x == 0) A.accepted[b] = (int)a;
-        for (uint32_t i = threadIdx.x; i <= A.n; i += CT)
-            if (i != a) out[i] = i < a ? A.tokens[(size_t)b * A.n + i] : -1;
-    }
+    int32_t* token = A.out + (size_t)b * (A.n + 1) + a;
+    if (blockIdx.x == 0) write_accepted(A, b, a);
     // ---- the row behind the accepted ones
     if (warp < 2) {
         float2 x = make_float2(NAN, NAN);
-        if (warp == 0) x = whole_row<GREEDY>(A, (size_t)b * (A.n + 1) + a);
-        else if (!GREEDY && rejected && A.draft) x = whole_row<false>(A, (size_t)A.batch * (A.n + 1) + (size_t)b * A.n + a);
+        if (warp == 0) x = whole_row<GREEDY>(t_part + (size_t)a * A.pieces, A.pieces, (float)k);
+        else if (!GREEDY && rejected && A.draft) x = whole_row<false>(d_part + (size_t)a * A.pieces, A.pieces, (float)k);
         if (lane == 0) s_row[warp] = x;
     }
     __syncthreads();
     if constexpr (GREEDY) {
-        if (threadIdx.x == 0) out[a] = isfinite(s_row[0].x) ? __float_as_int(s_row[0].y) : -1;
+        if (threadIdx.x == 0) *token = isfinite(s_row[0].x) ? __float_as_int(s_row[0].y) : -1;
     } else {
         if (!sound(s_row[0])) {                                   // a row without a distribution, for all CTAs of the sequence
-            if (blockIdx.x == 0 && threadIdx.x == 0) out[a] = -1;
+            if (blockIdx.x == 0 && threadIdx.x == 0) *token = -1;
             return;
         }
         const int away = rejected && !A.draft ? A.tokens[(size_t)b * A.n + a] : -1;
         const typename E::T *p = target + a * A.t_stride, *q = sound(s_row[1]) ? draft + a * A.d_stride : nullptr;   // a draft row without one takes nothing away
-        draw<E>(A, b, p, q, s_row[0], s_row[1], k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], away, shared, out + a);
+        draw<E>(A, b, p, q, s_row[0], s_row[1], k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], away, shared, token);
     }
+}
+
+// T = 0 and few logits, in one launch: a cluster of eight CTAs to a sequence, a warp to a piece of a row. The CTAs' warps tell one another what
+// they found, and the first CTA decides. A launch less is some 2 us of the host's time, which is what a small call costs: one
+// sequence, four drafts, 32768 tokens 10.8 us against 13.5 call by call.
+template <class E>
+__global__ void __launch_bounds__(GT) verify_greedy_kernel(const VerifyArgs A) {
+    constexpr uint32_t GW = GT / 32, ALL = CL * GW;
+    __shared__ float2 parts[ALL], whole[MAX_ROWS];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x / CL, mine = cluster.block_rank() * GW + warp;
+    cluster_arrive();                                             // with the wait below: nothing is written to a CTA before it runs
+    pdl_wait();
+    pdl_release();
+    const uint32_t nd = drafts_of(A, b), per = ALL / (nd + 1), r = mine / per;
+    float2 v = make_float2(-INFINITY, __int_as_float(INT_MAX));
+    if (r <= nd) {
+        const typename E::T* p = (const typename E::T*)A.target + ((size_t)b * (A.n + 1) + r) * A.t_stride;
+        const int64_t p_lead = lead<E>(p), vecs = ((int64_t)A.vocab + p_lead + E::V - 1) / E::V, at = mine % per;
+        v = part_of_row<E, true>(p, vecs * at / per * E::V - p_lead, min((int64_t)A.vocab, vecs * (at + 1) / per * E::V - p_lead), 0.0f);
+    }
+    cluster_wait();
+    if (lane == 0) *cluster.map_shared_rank(&parts[mine], 0) = v;
+    cluster.sync();
+    if (cluster.block_rank() != 0) return;
+    if (warp <= nd) {
+        const float2 x = whole_row<true>(parts + warp * per, per, 0.0f);
+        if (lane == 0) whole[warp] = x;
+    }
+    __syncthreads();
+    uint32_t a = 0;
+    while (a < nd && isfinite(whole[a].x) && A.tokens[(size_t)b * A.n + a] == __float_as_int(whole[a].y)) a++;
+    write_accepted(A, b, a);
+    if (threadIdx.x == 0) A.out[(size_t)b * (A.n + 1) + a] = isfinite(whole[a].x) ? __float_as_int(whole[a].y) : -1;
 }
 
 const char* verify_refuses(uint32_t batch, uint32_t n, uint32_t vocab) {
@@ -520,6 +565,13 @@ Layout lay_out(uint32_t batch, uint32_t n, uint32_t vocab) {
 
 template <class E, bool GREEDY>
 bool launch_verify(cudaStream_t st, const VerifyArgs& a) {
+    // one launch while a cluster's share is a megabyte at most and the clusters find room at once
+    if (GREEDY && a.n < MAX_ROWS && (size_t)(a.n + 1) * a.vocab * sizeof(typename E::T) <= (1u << 20) && a.batch <= 148 / CL) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(a.batch * CL); cfg.blockDim = dim3(GT); cfg.stream = st;
+        g_launches++;
+        return launch_pdl_cluster(verify_greedy_kernel<E>, cfg, dim3(CL, 1, 1), a) == cudaSuccess;
+    }
     const uint64_t items = ((uint64_t)a.batch * (a.n * (a.draft ? 2 : 1) + 1)) * a.pieces;
     g_launches += 2;
     if (launch_pdl(verify_rows_kernel<E, GREEDY>, dim3((uint32_t)std::min<uint64_t>((items + RT / 32 - 1) / (RT / 32), 148 * 6)), dim3(RT), 0, st, a) != cudaSuccess) return false;
