@@ -2,11 +2,17 @@
 // its first `sinks`, its last `recent` and those of greatest weight between them (equal weights: the lower position); they move
 // up in their order.
 //
-// evict_select_kernel: a CTA per (sequence, key head). The weights become whole numbers of the same order, four passes over eight bits
-// each find the smallest that stays, one pass in order writes the list of the positions that stay and moves the weights.
-// evict_move_kernel: rows by the list. Every destination lies at or in front of its source, so a walk in ascending order moves a cache in
-// place: a step's loads are complete before its stores, and later steps read behind all that earlier ones wrote. Columns of a row
-// have nothing to do with one another; CTAs that share a cache in place share its columns, not its rows.
+// select_head: the weights become whole numbers of the same order; passes over eight bits each find the smallest that stays (two or three
+// of four, mostly: a pass whose digit stays as a whole is the last), then every thread lists those of its share of the positions.
+// Rows move by the list. Every destination lies at or in front of its source, so a walk in ascending order moves a cache in place: a
+// step's loads are complete before its stores, and later steps read behind all that earlier ones wrote. Columns of a row have nothing to
+// do with one another; CTAs that share a cache in place share its columns, not its rows.
+//
+// evict_kernel: one launch. The CTAs of a cluster share a (sequence, key head); each makes the list for itself. Other CTAs' moves hide
+// that where there are many: 64 sequences of 512 to 2048 positions cut to 1024 100 us in two launches, 90 in one; and a launch is some 2 us of the
+// host's time: two sequences 13.5 -> 11.8 us call by call.
+// evict_select_kernel, evict_move_kernel: lists that shared memory does not hold, and lengths replaced in place, which no CTA may write
+// before all have read them.
 #include <cstdio>
 #include <algorithm>
 #include "engine.h"
@@ -35,101 +41,153 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 }
 
 constexpr int ST = 512;
+constexpr uint32_t LIST = 8192;            // positions of a list in shared memory
 
-__global__ void __launch_bounds__(ST) evict_select_kernel(const EvictArgs A) {
-    __shared__ uint32_t hist[256], warps[ST / 32], s_digit, s_need;
+struct SelectShared {
+    uint32_t hist[256], warps[ST / 32], digit, need, count;
+};
+
+__device__ __forceinline__ uint32_t length_of(const EvictArgs& A, uint32_t b) { return (uint32_t)min(max(A.n_in[b], 0), (int)A.nslots); }
+
+// Exclusive sum over the CTA's threads; *total: of all
+__device__ __forceinline__ uint32_t before_me(SelectShared& S, uint32_t v, uint32_t* total) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t x = v;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= (uint32_t)o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) S.warps[warp] = x;
+    __syncthreads();
+    uint32_t front = 0, all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < ST / 32; i++) { if (i == warp) front = all; all += S.warps[i]; }
+    *total = all;
+    return front + x - v;
+}
+
+// list: the positions of a key head that stay, in order (min(n, keep) of them). Ends with the list visible to the CTA.
+__device__ void select_head(const EvictArgs& A, SelectShared& S, const float* w, uint32_t n, int32_t* list) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_wait();
-    pdl_release();
-    const uint32_t b = blockIdx.x / A.kv_heads;
-    const size_t head = blockIdx.x;
-    const uint32_t n = (uint32_t)min(max(A.n_in[b], 0), (int)A.nslots), count = min(n, A.keep);
-    const float* w = A.w_in + head * A.nslots;
-    float* wo = A.w_out + head * A.nslots;
-    int32_t *list = A.list + head * A.keep, *kept = A.kept ? A.kept + head * A.keep : nullptr;
-    if (kept)
-        for (uint32_t i = count + tid; i < A.keep; i += ST) kept[i] = -1;
     if (n <= A.keep) {
-        for (uint32_t i = tid; i < n; i += ST) {
-            list[i] = (int)i;
-            if (kept) kept[i] = (int)i;
-            if (w != wo) wo[i] = w[i];
-        }
+        for (uint32_t i = tid; i < n; i += ST) list[i] = (int)i;
+        __syncthreads();
         return;
     }
-    // ---- the smallest number that stays, digit by digit, and how many that are equal to it stay
+    // ---- the smallest number that stays, digit by digit, and how many that share its digits so far stay
     const uint32_t first = A.sinks, end = n - A.recent;
     uint32_t need = A.keep - A.sinks - A.recent, prefix = 0;
-    if (need) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (uint32_t i = tid; i < 256; i += ST) hist[i] = 0;
-            __syncthreads();
-            for (uint32_t p = first + tid; p < end; p += ST) {
-                const uint32_t k = order_of(w[p]);
-                if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (warp == 0) {                               // lane l: digits 255 - 8 l and the seven below
-                uint32_t c[8], sum = 0;
-#pragma unroll
-                for (int i = 0; i < 8; i++) { c[i] = hist[255 - 8 * lane - i]; sum += c[i]; }
-                uint32_t upto = sum;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= (uint32_t)o) upto += y;
-                }
-                uint32_t above = upto - sum;
-                if (above < need && need <= upto) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        if (above < need && need <= above + c[i]) { s_digit = 255 - 8 * lane - i; s_need = need - above; }
-                        above += c[i];
-                    }
-                }
-            }
-            __syncthreads();
-            prefix = (prefix << 8) | s_digit;
-            need = s_need;
+    int shift = 32;
+    while (need && shift > 0) {
+        shift -= 8;
+        if (tid < 256) S.hist[tid] = 0;
+        __syncthreads();
+        for (uint32_t p = first + tid; p < end; p += ST) {
+            const uint32_t k = order_of(w[p]);
+            if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&S.hist[(k >> shift) & 255u], 1u);
         }
-    } else {
-        prefix = 0xFFFFFFFFu;                              // no weight's number: none of the middle stays
+        __syncthreads();
+        if (warp == 0) {                                   // lane l: digits 255 - 8 l and the seven below
+            uint32_t c[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) { c[i] = S.hist[255 - 8 * lane - i]; sum += c[i]; }
+            uint32_t upto = sum;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += y;
+            }
+            uint32_t above = upto - sum;
+            if (above < need && need <= upto) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (above < need && need <= above + c[i]) { S.digit = 255 - 8 * lane - i; S.need = need - above; S.count = c[i]; }
+                    above += c[i];
+                }
+            }
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | S.digit;
+        need = S.need;
+        if (S.count == need) break;                        // all that share these digits stay
     }
-    // ---- in order: who stays, and where it goes. equal: how many equal to `prefix` lie in front
-    uint32_t placed = 0, equal = 0;
-    for (uint32_t p0 = 0; p0 < n; p0 += ST) {
-        const uint32_t p = p0 + tid;
-        float x = 0.0f;
-        bool stay = false, same = false;
-        if (p < n) {
-            x = w[p];
-            if (p < first || p >= end) stay = true;
-            else { const uint32_t k = order_of(x); stay = k > prefix; same = k == prefix && need; }
+    // ---- who stays, in order: a run of positions to a thread
+    const uint32_t per = (n + ST - 1) / ST, p0 = min(n, tid * per), p1 = min(n, p0 + per);
+    const bool some = A.keep > A.sinks + A.recent;         // any of the middle stays
+    uint32_t more = 0, same = 0, total;                    // that stay for certain, that share all digits looked at
+    for (uint32_t p = p0; p < p1; p++) {
+        if (p < first || p >= end) more++;
+        else if (some) { const uint32_t k = order_of(w[p]) >> shift; more += k > prefix; same += k == prefix; }
+    }
+    const uint32_t equal = before_me(S, same, &total), left = equal < need ? min(same, need - equal) : 0;
+    uint32_t at = before_me(S, more + left, &total), taken = 0;
+    for (uint32_t p = p0; p < p1; p++) {
+        bool stays = p < first || p >= end;
+        if (!stays && some) {
+            const uint32_t k = order_of(w[p]) >> shift;
+            stays = k > prefix || (k == prefix && taken < left);
+            taken += k == prefix;
         }
-        const uint32_t below = (1u << lane) - 1u, sb = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) warps[warp] = __popc(sb);
-        __syncthreads();
-        uint32_t e = equal, all = 0;
-        for (uint32_t i = 0; i < ST / 32; i++) { if (i < warp) e += warps[i]; all += warps[i]; }
-        equal += all;
-        if (same && e + __popc(sb & below) < need) stay = true;
-        const uint32_t tb = __ballot_sync(0xffffffffu, stay);
-        __syncthreads();
-        if (lane == 0) warps[warp] = __popc(tb);
-        __syncthreads();
-        uint32_t at = placed;
-        all = 0;
-        for (uint32_t i = 0; i < ST / 32; i++) { if (i < warp) at += warps[i]; all += warps[i]; }
-        placed += all;
-        at += __popc(tb & below);
-        if (stay) {                                        // in place: `at` <= p, and all weights up to p0 + ST - 1 have been read
-            list[at] = (int)p;
-            if (kept) kept[at] = (int)p;
-            wo[at] = x;
-        }
-        __syncthreads();
+        if (stays) list[at++] = (int)p;
+    }
+    __syncthreads();
+}
+
+// Weights and old positions by the list; in place, zeros where positions left.
+__device__ __forceinline__ void move_weights(const EvictArgs& A, size_t head, uint32_t n, const int32_t* list) {
+    const float* w = A.w_in + head * A.nslots;
+    float* wo = A.w_out + head * A.nslots;
+    int32_t* kept = A.kept ? A.kept + head * A.keep : nullptr;
+    const uint32_t count = min(n, A.keep);
+    for (uint32_t i0 = 0; i0 < A.keep; i0 += ST) {
+        const uint32_t i = i0 + threadIdx.x;
+        const bool in = i < count;
+        const int p = in ? list[i] : -1;
+        const float x = in ? w[p] : 0.0f;
+        __syncthreads();                                   // in place: all of a step has been read, and later steps read behind it
+        if (in) wo[i] = x;
+        if (kept && i < A.keep) kept[i] = p;
     }
     if (w == wo)
-        for (uint32_t p = A.keep + tid; p < n; p += ST) wo[p] = 0.0f;
+        for (uint32_t i = count + threadIdx.x; i < n; i += ST) wo[i] = 0.0f;
+}
+
+// Rows r0 .. end of the list, pieces c0 .. c0 + cols (16 bytes each) of the K or V half v; T threads, U pieces of each in flight.
+template <int T, int U>
+__device__ __forceinline__ void move_rows(const EvictArgs& A, uint32_t head, uint32_t v, uint32_t c0, uint32_t cols, uint32_t r0, uint32_t end, const int32_t* list) {
+    const size_t width = (size_t)A.batch * A.kv_heads * A.hd, pitch = 2 * width / 8;     // a slot in 16-byte pieces
+    const size_t base = (v * width + (size_t)head * A.hd) / 8 + c0;
+    const uint4* in = (const uint4*)A.in + base;
+    uint4* out = (uint4*)A.out + base;
+    const bool in_place = A.in == A.out;
+    const uint32_t step = T / cols, c = threadIdx.x % cols, r = threadIdx.x / cols;
+    for (uint32_t i0 = r0; i0 < end; i0 += step * U) {
+        uint4 x[U];
+        uint32_t src[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * step + r;
+            src[u] = i < end && r < step ? (uint32_t)list[i] : 0xFFFFFFFFu;
+            if (in_place && src[u] == i) src[u] = 0xFFFFFFFFu;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (src[u] != 0xFFFFFFFFu) x[u] = in[src[u] * pitch + c];
+        if (in_place) __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (src[u] != 0xFFFFFFFFu) out[(size_t)(i0 + u * step + r) * pitch + c] = x[u];
+    }
+}
+
+__global__ void __launch_bounds__(ST) evict_select_kernel(const EvictArgs A) {
+    __shared__ SelectShared S;
+    pdl_wait();
+    pdl_release();
+    const uint32_t n = length_of(A, blockIdx.x / A.kv_heads);
+    int32_t* list = A.list + (size_t)blockIdx.x * A.keep;
+    select_head(A, S, A.w_in + (size_t)blockIdx.x * A.nslots, n, list);
+    move_weights(A, blockIdx.x, n, list);
 }
 
 constexpr int MT = 256, MU = 8;
@@ -138,35 +196,34 @@ constexpr int MT = 256, MU = 8;
 __global__ void __launch_bounds__(MT) evict_move_kernel(const EvictArgs A, uint32_t cols, uint32_t rows_each) {
     pdl_wait();
     pdl_release();
-    const uint32_t b = blockIdx.y / A.kv_heads, per = A.hd / 8 / cols;
-    const uint32_t n = (uint32_t)min(max(A.n_in[b], 0), (int)A.nslots), count = min(n, A.keep);
+    const uint32_t b = blockIdx.y / A.kv_heads, per = A.hd / 8 / cols, count = min(length_of(A, b), A.keep);
     // n_out may be n_in: what other CTAs then read gives the same count
     if (blockIdx.x == 0 && blockIdx.z == 0 && blockIdx.y % A.kv_heads == 0 && threadIdx.x == 0) A.n_out[b] = (int)count;
-    const uint32_t v = blockIdx.x / per, c0 = (blockIdx.x % per) * cols;
-    const size_t width = (size_t)A.batch * A.kv_heads * A.hd, pitch = 2 * width / 8;     // a slot in 16-byte pieces
-    const size_t base = (v * width + (size_t)blockIdx.y * A.hd) / 8 + c0;
-    const uint4* in = (const uint4*)A.in + base;
-    uint4* out = (uint4*)A.out + base;
-    const int32_t* list = A.list + (size_t)blockIdx.y * A.keep;
-    const bool in_place = A.in == A.out;
-    const uint32_t r0 = blockIdx.z * rows_each, end = min(count, r0 + rows_each), step = MT / cols;
-    const uint32_t c = threadIdx.x % cols, r = threadIdx.x / cols;
-    for (uint32_t i0 = r0; i0 < end; i0 += step * MU) {
-        uint4 x[MU];
-        uint32_t src[MU];
-#pragma unroll
-        for (int u = 0; u < MU; u++) {
-            const uint32_t i = i0 + u * step + r;
-            src[u] = i < end && r < step ? (uint32_t)list[i] : 0xFFFFFFFFu;
-            if (in_place && src[u] == i) src[u] = 0xFFFFFFFFu;
-        }
-#pragma unroll
-        for (int u = 0; u < MU; u++)
-            if (src[u] != 0xFFFFFFFFu) x[u] = in[src[u] * pitch + c];
-        if (in_place) __syncthreads();
-#pragma unroll
-        for (int u = 0; u < MU; u++)
-            if (src[u] != 0xFFFFFFFFu) out[(size_t)(i0 + u * step + r) * pitch + c] = x[u];
+    const uint32_t r0 = blockIdx.z * rows_each;
+    move_rows<MT, MU>(A, blockIdx.y, blockIdx.x / per, blockIdx.x % per * cols, cols, r0, min(count, r0 + rows_each), A.list + (size_t)blockIdx.y * A.keep);
+}
+
+// grid: (CTAs of a cluster, (sequence, key head)). In place a CTA has `cols` pieces of all rows, else all pieces of a part of the rows.
+__global__ void __launch_bounds__(ST) evict_kernel(const EvictArgs A, uint32_t cols) {
+    __shared__ SelectShared S;
+    __shared__ int32_t list[LIST];
+    pdl_wait();
+    pdl_release();
+    const uint32_t b = blockIdx.y / A.kv_heads, n = length_of(A, b), count = min(n, A.keep), pieces = A.hd / 8, per = pieces / cols;
+    select_head(A, S, A.w_in + (size_t)blockIdx.y * A.nslots, n, list);
+    if (A.w_in == A.w_out && gridDim.x > 1) {                 // all have read the weights before the first writes them
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (blockIdx.x == 0) {
+        if (blockIdx.y % A.kv_heads == 0 && threadIdx.x == 0) A.n_out[b] = (int)count;
+        move_weights(A, blockIdx.y, n, list);
+    }
+    if (A.in == A.out) {
+        for (uint32_t part = blockIdx.x; part < 2 * per; part += gridDim.x) move_rows<ST, 4>(A, blockIdx.y, part / per, part % per * cols, cols, 0, count, list);
+    } else {
+        const uint32_t r0 = (uint32_t)((uint64_t)count * blockIdx.x / gridDim.x), r1 = (uint32_t)((uint64_t)count * (blockIdx.x + 1) / gridDim.x);
+        for (uint32_t v = 0; v < 2; v++) move_rows<ST, 4>(A, blockIdx.y, v, 0, pieces, r0, r1, list);
     }
 }
 
@@ -187,6 +244,18 @@ bool apart(const void* a, const void* b, size_t bytes) {
 }  // namespace
 
 bool k_kv_evict(cudaStream_t st, const EvictArgs& a) {
+    if (a.n_in != a.n_out && a.keep <= LIST) {
+        // CTAs to a cluster: up to eight, while they do not fill the SMs twice
+        const uint32_t heads = a.batch * a.kv_heads, pieces = a.hd / 8;
+        uint32_t parts = 1, cols = pieces;
+        while (parts < 8 && heads * parts * 2 <= 2 * 148) parts *= 2;
+        if (a.in == a.out)
+            while (cols % 2 == 0 && cols > 2 && 2 * (pieces / cols) < parts) cols /= 2;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(parts, heads); cfg.blockDim = dim3(ST); cfg.stream = st;
+        g_launches++;
+        return launch_pdl_cluster(evict_kernel, cfg, dim3(parts, 1, 1), a, cols) == cudaSuccess;
+    }
     g_launches += 2;
     if (launch_pdl(evict_select_kernel, dim3(a.batch * a.kv_heads), dim3(ST), 0, st, a) != cudaSuccess) return false;
     // 16-byte pieces of a row half to a CTA: all of them, fewer where a cache that is moved in place would leave SMs idle

@@ -25,9 +25,10 @@ class Call:
         self.kept = torch.full((batch, kv_heads, keep), -7, dtype=torch.int32, device="cuda")
 
     def run(self, lib, in_place, kept=True):
+        """in_place: caches, weights and lengths ("all"), or the lengths written elsewhere ("rows")."""
         import torch
         if in_place:
-            self.o_ring, self.o_w, self.o_n = self.d_ring, self.d_w, self.d_n
+            self.o_ring, self.o_w, self.o_n = self.d_ring, self.d_w, self.d_n if in_place == "all" else torch.full_like(self.d_n, -1)
         else:
             self.o_ring, self.o_w, self.o_n = torch.full_like(self.d_ring, 77), torch.full_like(self.d_w, 9.0), torch.full_like(self.d_n, -1)
         ws = torch.full((lib.gehtp_kv_evict_workspace(*self.shape),), 255, dtype=torch.uint8, device="cuda")
@@ -68,7 +69,7 @@ CASES = [
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c[:4] + c[5:8])))
-@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("in_place", [False, "rows", "all"])
 def test_against_the_rule(cuda, case, in_place):
     call = Call(*case[:8], weights=case[8], seed=case[3])
     kept = case[0] != 3
@@ -82,10 +83,10 @@ def test_again_and_again(cuda):
     import torch
     call = Call(3, 2, 64, 96, [96, 80, 40], 48, 2, 16, seed=3)
     for turn in range(4):
-        call.run(cuda, True)
-        call.check(True)
+        call.run(cuda, "all")
+        call.check("all")
         before = call.d_ring.clone(), call.d_w.clone(), call.d_n.clone()
-        call.run(cuda, True)
+        call.run(cuda, "all")
         assert torch.equal(before[0], call.d_ring) and torch.equal(before[1], call.d_w) and torch.equal(before[2], call.d_n)
         call.d_n += 30 - turn
         call.d_w += torch.rand_like(call.d_w)
