@@ -780,8 +780,10 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     if (with_weights && !a.nslots) return false;
     const size_t tokens = (size_t)a.batch * a.q_len, rows = tokens * a.rep;
     l.t_rt = row_tiles((size_t)a.q_len * a.rep);
-    // the prefix goes with the tails while its rows fit into their row tiles, else on tcgen05
-    l.umma = rows > l.t_rt * 16;
+    // The prefix goes with the tails, in their launch, while its rows fit into their row tile, or are in few tiles of 16 and meet few
+    // positions; else on tcgen05. 8 heads of 128, 32 rows: 512 positions 11.2 us with the tails, 13.3 on tcgen05; 2048 15.0 and
+    // 14.9; 8192 24.9 and 20.1. 64 rows: 512 12.2 and 13.8; 2048 20.6 and 19.9. 128 rows: 512 13.4 and 14.4.
+    l.umma = rows > l.t_rt * 16 && !(l.t_rt == 1 && rows * a.n_prefix <= 65536);
     a.p_tokens = (uint32_t)std::min<size_t>(tokens, (l.umma ? 128 : l.t_rt * 16) / a.rep);
     a.p_tiles = (uint32_t)((tokens + a.p_tokens - 1) / a.p_tokens);
     const uint32_t unit = l.umma ? 128 : TILE, tiles = (a.n_prefix + unit - 1) / unit;

@@ -10,7 +10,8 @@
 //   P               one thread per row: maximum, 2^(s - m) written over S as matrix operand: fp16, or bf16 as hi + lo pairs (bf16's 8 bits
 //                   are fewer than a result of that type has)
 //   O += P V        tcgen05.mma with P as the A operand from TMEM, V as it lies in memory (MN-major B operand)
-// The maximum a row is referred to is raised - and its O rescaled - only when a tile exceeds it by more than 2^8.
+// The maximum that a row's weights are referred to is one of an earlier tile: the exponentials need not wait for the tile's own. It is
+// raised - and O rescaled - when a tile has exceeded it by more than 2^8.
 //
 // Rows of a tile: p_tokens tokens of rep heads, heads fastest (a three-dimensional TMA box over [head_dim][heads][tokens]). Where rep does
 // not divide 128 the last rows of a tile are left over: what lies in their shared memory never reaches another row.
@@ -36,7 +37,9 @@ namespace {
 
 constexpr uint32_t BKV = 128;
 constexpr int NTHREADS = 384;
-constexpr float kRaise = 8.0f;
+// A reference is raised behind a tile that exceeds it by more than 2^8, and before a tile's weights are used where they would exceed 2^14
+// (fp16 ends at 2^16)
+constexpr float kRaise = 8.0f, kMost = 14.0f;
 
 // stages of K and of V tiles: as many as 227 KB hold behind the rows' tiles
 template <int DB, bool PAIR>
@@ -78,6 +81,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// largest of a row's 128 scores
+__device__ __forceinline__ float max128(const uint32_t (&v)[4][32]) {
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+    return max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
         ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
@@ -104,6 +117,8 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
     const bool two = PAIR && tile0 + 1 < A.p_tiles;               // an odd number of row tiles leaves the last CTA one
     const uint32_t box_rows = A.p_tokens * A.rep;
 
+    if (threadIdx.x == 32)
+        for (const CUtensorMap* map : {&tmap_q, &tmap_kv}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     if (threadIdx.x == 0) {
         mbar_init(&bars->q_full, 1); mbar_init(&bars->o_full, 1); mbar_init(&bars->merge, 8);
         for (int s = 0; s < ST; s++) { mbar_init(&bars->kv_full[s], 1); mbar_init(&bars->kv_empty[s], 1); }
@@ -240,7 +255,7 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");    // 256 x 200 + 128 x 104 = 384 x 168, what the CTA was launched with
         const uint32_t t = (warp - 4) >> 2, quarter = warp & 3;
         const uint32_t ts = tmem + ((quarter * 32) << 16) + t * 128, to_ = ts + 256;
-        float m = -INFINITY;
+        float m = -INFINITY, top = -INFINITY;                    // reference of the weights; maximum of the last tile
         float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         bool ok = true;
         const bool works = t == 0 || (PAIR ? two : n_kt > 1);
@@ -262,36 +277,28 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[c][i] = c * 32 + i <= hi ? v[c][i] : 0xff800000u;
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
-            float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-            mt *= A.sc;
-            // s_full of this tile came after the group's products of the tile before: its O is at rest
-            const bool raise = mt > m + kRaise;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float f = raise ? (m == -INFINITY ? 0.0f : ex2(m - mt)) : 1.0f;
-                if (raise) m = mt;
+            // O is at rest: s_full of this tile came after the group's products of the tile before
+            auto rescale = [&](bool raise, float to_m) {
+                const float f = raise ? (m == -INFINITY ? 0.0f : ex2(m - to_m)) : 1.0f;
+                if (raise) m = to_m;
 #pragma unroll
                 for (int i = 0; i < 2; i++) { l2[i].x *= f; l2[i].y *= f; }
                 if (round) {
 #pragma unroll 1
-                    for (int c = 0; c < DB * 2; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(to_ + c * 32, v);
-                        tmem_ld_wait(v);
+                    for (int c = 0; c < DB * 4; c++) {
+                        uint32_t x[16];
+                        tmem_ld16(to_ + c * 16, x);
+                        tmem_ld_wait(x);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tmem_st32(to_ + c * 32, v);
+                        for (int i = 0; i < 16; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                        tmem_st16(to_ + c * 16, x);
                     }
                     tmem_st_wait();
                 }
-            }
-            const float off = m == -INFINITY ? 0.0f : -m;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
+            };
+            if (round == 0) m = max128(v) * A.sc;
+            else if (__any_sync(0xffffffffu, top > m + kRaise)) rescale(top > m + kRaise, top);
+            auto probs = [&](int c, float off) {
                 uint32_t w[32];
                 if (BF) {
                     probs32<false>(v[c], w, A.sc, off, 0u, l2);
@@ -300,7 +307,23 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
                     probs32_h(v[c], w, A.sc, off, l2);
                     tmem_st16(ts + c * 32, w);
                 }
+            };
+            // The first half's weights by the reference known from earlier tiles, while the tile's maximum is found: only where that is more
+            // than 2^14 above the reference they are made again.
+            const float2 l0 = l2[0], l1 = l2[1];
+            float off;
+#pragma unroll 1
+            for (int again = 0; ; again = 1) {
+                off = m == -INFINITY ? 0.0f : -m;
+                probs(0, off);
+                probs(1, off);
+                top = max128(v) * A.sc;
+                if (again || !__any_sync(0xffffffffu, top > m + kMost)) break;
+                l2[0] = l0; l2[1] = l1;
+                rescale(top > m + kMost, top);
             }
+            probs(2, off);
+            probs(3, off);
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
