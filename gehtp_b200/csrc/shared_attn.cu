@@ -8,9 +8,7 @@
 //
 // Items of work: (row tile, key head, slice of the prefix) and (sequence, key head, slice of its tail). How a batch's tails are cut follows
 // from their lengths, which lie on the device: every CTA works that out for itself. S and P stay in registers (mma.sync m16n8k16).
-// shared_warps_kernel: up to 16 rows to a key head, an item to a warp.
-// shared_parts_kernel: more rows, an item to a CTA; K and V tiles of 64 positions by cp.async in two to four stages, a warp has 16 rows and
-// a half or all of a tile's positions.
+// shared_parts_kernel: an item to as many warps as it has 16 rows.
 // shared_merge_kernel: partial results of a row together; where asked for, the weights of the tail positions.
 #include <climits>
 #include <cmath>
@@ -86,7 +84,7 @@ struct Item {
     bool tail, last;                       // last: it holds the end of a tail
     uint32_t h, rows, token0, from, to;    // key head; rows, their first token; positions
     uint32_t b, n, c;                      // of a tail: its sequence, its length, positions that all rows see
-    size_t v_off, part;                    // from a key to its value, half of what lies between two keys; first partial row
+    size_t v_off, out;                     // from a key to its value, half of what lies between two keys; first partial row
     const uint16_t* kbase;
 };
 
@@ -105,7 +103,7 @@ __device__ __forceinline__ Item item_of(const SharedArgs& A, const uint32_t* cum
         I.to = min(A.n_prefix, I.from + A.p_len);
         I.v_off = (size_t)A.kv_heads * HD;
         I.kbase = A.prefix + (size_t)I.h * HD;
-        I.part = (((size_t)tile * A.kv_heads + I.h) * A.p_slices + s) * (A.p_tokens * A.rep);
+        I.out = (((size_t)tile * A.kv_heads + I.h) * A.p_slices + s) * (A.p_tokens * A.rep);
     } else {
         const uint32_t u = (w - prefix_items) / A.kv_heads;
         I.h = (w - prefix_items) % A.kv_heads;
@@ -124,26 +122,34 @@ __device__ __forceinline__ Item item_of(const SharedArgs& A, const uint32_t* cum
         I.to = I.last ? I.n : I.from + k * TILE;
         I.v_off = (size_t)A.batch * A.kv_heads * HD;
         I.kbase = A.tail + ((size_t)b * A.kv_heads + I.h) * HD;
-        I.part = A.p_rows() + ((size_t)u * A.kv_heads + I.h) * I.rows;
+        I.out = A.p_rows() + ((size_t)u * A.kv_heads + I.h) * I.rows;
     }
     return I;
 }
 
-// Up to 16 rows to a key head: a warp to an item, on its own. Tiles of 16 positions by cp.async into the warp's stages; no barrier in the
-// loop, so that what an item costs to begin and to end is other warps' time.
+// RT warps share an item, 16 rows each (RT: 1, 2, 4 or 8), and the tiles of 16 RT positions that they bring in by cp.async. They meet once a
+// tile among themselves and with nobody else, so that what an item costs to begin and to end is other groups' time: eight warps an
+// SM, 24 KB of tiles each. A CTA to an item, with 64 positions split over its warps, took 93 us where this takes 89 (32 sequences,
+// tails of 1024 to 4096).
 template <int HD>
 __host__ __device__ constexpr int warp_stages() { return HD == 128 ? 3 : 6; }
-template <int HD>
-__host__ __device__ constexpr size_t warps_smem() { return (size_t)4 * warp_stages<HD>() * 64 * HD + (MAX_BATCH + 4) * 4; }
+template <int RT>
+__host__ __device__ constexpr int warps_of() { return RT == 8 ? 8 : 4; }
+template <int HD, int RT>
+__host__ __device__ constexpr size_t parts_smem() { return (size_t)warps_of<RT>() * warp_stages<HD>() * 64 * HD + (MAX_BATCH + 4) * 4; }
 
-template <bool BF, int HD>
-__global__ void __launch_bounds__(128, 2) shared_warps_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
-    constexpr uint32_t ST = warp_stages<HD>(), ROW = HD * 2, HALF = 16 * ROW;
+template <bool BF, int HD, int RT>
+__global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
+    constexpr uint32_t ST = warp_stages<HD>(), ROW = HD * 2, TP = 16 * RT, HALF = TP * ROW, NT = warps_of<RT>() * 32, GROUPS = warps_of<RT>() / RT;
     extern __shared__ __align__(128) unsigned char smem[];
-    uint32_t* cum = (uint32_t*)(smem + 4 * ST * 2 * HALF);
-    __shared__ uint32_t s_k;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
-    const uint32_t ring = smem_addr(smem) + warp * ST * 2 * HALF;
+    uint32_t* cum = (uint32_t*)(smem + GROUPS * ST * 2 * HALF);
+    __shared__ uint32_t s_k, s_next[GROUPS][2];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3, group = warp / RT, part = warp % RT;
+    const uint32_t base = smem_addr(smem), ring = base + group * ST * 2 * HALF;
+    auto meet = [&] {
+        if (RT == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(RT * 32) : "memory");
+    };
     // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait: all that was there before the
     // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
     if (!beside) pdl_wait();
@@ -155,27 +161,29 @@ __global__ void __launch_bounds__(128, 2) shared_warps_kernel(const SharedArgs A
         }
         __syncthreads();
         if (blockIdx.x == 0)
-            for (uint32_t b = threadIdx.x; b <= A.batch; b += 128) A.plan[b] = cum[b];
+            for (uint32_t b = threadIdx.x; b <= A.batch; b += NT) A.plan[b] = cum[b];
     }
     const uint32_t items = prefix_items + (with_tails ? cum[A.batch] * A.kv_heads : 0), k = with_tails ? s_k : 0;
     // Beside the prefix's kernel most CTAs come up when that one leaves the SMs, and the first take what the others have not begun:
     // items are handed out by a counter.
-    auto next_item = [&](uint32_t w) {
-        if (!beside) return w + gridDim.x * 4;
-        if (lane == 0) w = atomicAdd(A.next, 1u);
-        return __shfl_sync(0xffffffffu, w, 0);
-    };
-    for (uint32_t w = beside ? next_item(0) : blockIdx.x + gridDim.x * warp, ahead; w < items; w = ahead) {
-        ahead = next_item(w);
+    uint32_t w = blockIdx.x + gridDim.x * group, turn = 0;
+    if (beside) {
+        if (part == 0 && lane == 0) s_next[group][1] = atomicAdd(A.next, 1u);
+        meet();
+        w = s_next[group][1];
+    }
+    for (; w < items; turn ^= 1) {
+        uint32_t ahead = w + gridDim.x * GROUPS;
+        if (beside && part == 0 && lane == 0) ahead = atomicAdd(A.next, 1u);
         const Item I = item_of<HD>(A, cum, k, w, prefix_items);
         const size_t pitch = 2 * I.v_off;
-        const uint32_t tiles = (I.to - I.from + 15) / 16;
+        const uint32_t tiles = (I.to - I.from + TP - 1) / TP, row0 = part * 16;
         auto load = [&](uint32_t i) {
             if (i < tiles) {
                 const uint32_t st = ring + (i % ST) * 2 * HALF;
 #pragma unroll
                 for (uint32_t u = 0; u < HD / 16; u++) {
-                    const uint32_t e = u * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), pos = I.from + i * 16 + r;
+                    const uint32_t e = u * (RT * 32) + part * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), pos = I.from + i * TP + r;
                     const bool in = pos < I.to;                     // rows past the end: zeros, whatever the cache holds there
                     const uint16_t* src = I.kbase + (in ? (size_t)pos * pitch + ch * 8 : 0);
                     const uint32_t dst = st + r * ROW + ((ch ^ (r & 7)) * 16);
@@ -191,7 +199,7 @@ __global__ void __launch_bounds__(128, 2) shared_warps_kernel(const SharedArgs A
         int lim[2];                                                   // the first position that a row does not see
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-            const uint32_t r = g8 + half * 8;
+            const uint32_t r = row0 + g8 + half * 8;
             const bool in = r < I.rows;
             lim[half] = I.last ? min((int)I.to, (int)(I.n + r / A.rep + 1) - (int)A.q_len) : (int)I.to;
             const uint16_t* qp = A.q + (in ? (size_t)(I.token0 + r / A.rep) * A.q_stride + (size_t)(I.h * A.rep + r % A.rep) * HD : 0) + q4 * 2;
@@ -205,322 +213,108 @@ __global__ void __launch_bounds__(128, 2) shared_warps_kernel(const SharedArgs A
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         for (uint32_t i = 0; i < tiles; i++) {
             cp_wait<ST - 2>();
-            __syncwarp();
-            load(i + ST - 1);                                         // over the tile before, which the whole warp has read
-            const uint32_t p0 = I.from + i * 16, kt = ring + (i % ST) * 2 * HALF, vt = kt + HALF;
-            float s[2][4] = {};
-            {
-                const uint32_t r = (lane & 7) + ((lane >> 4) & 1) * 8;
+            meet();
+            load(i + ST - 1);                                         // over the tile before, which all have read
+#pragma unroll 1
+            for (uint32_t sub = 0; sub < RT && row0 < I.rows; sub++) {
+                const uint32_t p0 = I.from + i * TP + sub * 16, kt = ring + (i % ST) * 2 * HALF + sub * 16 * ROW, vt = kt + HALF;
+                if (p0 >= I.to) break;
+                float s[2][4] = {};
+                {
+                    const uint32_t r = (lane & 7) + ((lane >> 4) & 1) * 8;
 #pragma unroll
-                for (int x = 0; x < HD / 16; x++) {
-                    uint32_t f[4];
-                    ldsm4(f, kt + r * ROW + (((2 * x + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
-                    mma16<BF>(s[0], qf[x], f[0], f[1]);
-                    mma16<BF>(s[1], qf[x], f[2], f[3]);
-                }
-            }
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool in = (int)(p0 + t * 8 + q4 * 2 + (e & 1)) < lim[e >> 1];
-                    s[t][e] = in ? s[t][e] * A.sc : -INFINITY;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
-                }
-            if (I.tail && A.scores) {
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const uint32_t r = g8 + half * 8;
-                    float* sp = A.scores + (((size_t)I.b * A.kv_heads + I.h) * I.rows + r) * A.nslots;
-                    if (r < I.rows)
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            const uint32_t p = p0 + t * 8 + q4 * 2;
-                            if (p < I.to) sp[p] = s[t][2 * half];
-                            if (p + 1 < I.to) sp[p + 1] = s[t][2 * half + 1];
-                        }
-                }
-            }
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-            }
-            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const float mn = fmaxf(m[half], mx[half]), f = m[half] == -INFINITY ? 0.0f : sm100::ex2(m[half] - mn);
-                    if (mn > m[half]) {
-                        m[half] = mn;
-                        l[half] *= f;
-#pragma unroll
-                        for (int j = 0; j < HD / 8; j++) { o[j][2 * half] *= f; o[j][2 * half + 1] *= f; }
+                    for (int x = 0; x < HD / 16; x++) {
+                        uint32_t f[4];
+                        ldsm4(f, kt + r * ROW + (((2 * x + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+                        mma16<BF>(s[0], qf[x], f[0], f[1]);
+                        mma16<BF>(s[1], qf[x], f[2], f[3]);
                     }
                 }
-            }
-            const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s[t][e] = sm100::ex2(s[t][e] - off[e >> 1]);
-                    l[e >> 1] += s[t][e];
-                }
-            // Positions that only some rows see have weight 0 for the others, which is 0 times their values: where one of those is no
-            // number, the tile's values are added row by row instead.
-            bool odd = false;
-            if (I.last && p0 + 16 > I.c && I.n > I.c) {
-                constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
-#pragma unroll 1
-                for (uint32_t u = 0; u < HD / 16; u++) {
-                    const uint32_t e = u * 32 + lane, r = e / (HD / 8);
-                    const uint4 v = *(const uint4*)(smem + (vt - smem_addr(smem)) + r * ROW + ((e % (HD / 8)) ^ (r & 7)) * 16);
-                    for (uint32_t x : {v.x, v.y, v.z, v.w}) odd |= (x & EXP & 0xffffu) == (EXP & 0xffffu) || (x & EXP & 0xffff0000u) == (EXP & 0xffff0000u);
-                }
-                odd = __any_sync(0xffffffffu, odd);
-            }
-            if (odd) {
-#pragma unroll 1
-                for (uint32_t col = 0; col < 16; col++) {
-                    const int from = (int)((lane & ~3u) + (col % 8) / 2);
-                    float p[2];
+                    for (int e = 0; e < 4; e++) {
+                        const bool in = (int)(p0 + t * 8 + q4 * 2 + (e & 1)) < lim[e >> 1];
+                        s[t][e] = in ? s[t][e] * A.sc : -INFINITY;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+                    }
+                if (I.tail && A.scores) {
 #pragma unroll
                     for (int half = 0; half < 2; half++) {
-                        const float a = col < 8 ? s[0][2 * half] : s[1][2 * half], b = col < 8 ? s[0][2 * half + 1] : s[1][2 * half + 1];
-                        p[half] = __shfl_sync(0xffffffffu, col % 2 ? b : a, from);
+                        const uint32_t r = row0 + g8 + half * 8;
+                        float* sp = A.scores + (((size_t)I.b * A.kv_heads + I.h) * I.rows + r) * A.nslots;
+                        if (r < I.rows)
+#pragma unroll
+                            for (int t = 0; t < 2; t++) {
+                                const uint32_t p = p0 + t * 8 + q4 * 2;
+                                if (p < I.to) sp[p] = s[t][2 * half];
+                                if (p + 1 < I.to) sp[p + 1] = s[t][2 * half + 1];
+                            }
                     }
-#pragma unroll
-                    for (int j = 0; j < HD / 8; j++) {
-                        const float2 v = unpack2<BF>(*(const uint32_t*)(smem + (vt - smem_addr(smem)) + col * ROW + ((j ^ (col & 7)) * 16) + q4 * 4));
-#pragma unroll
-                        for (int half = 0; half < 2; half++)
-                            if ((int)(p0 + col) < lim[half]) { o[j][2 * half] = fmaf(p[half], v.x, o[j][2 * half]); o[j][2 * half + 1] = fmaf(p[half], v.y, o[j][2 * half + 1]); }
-                    }
                 }
-                continue;
-            }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {                          // fragment register e: tile e / 2, rows of half e % 2
-                const float a = s[e >> 1][2 * (e & 1)], c2 = s[e >> 1][2 * (e & 1) + 1];
-                hi[e] = pack2<BF>(a, c2);
-                // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
-                if (BF) {
-                    const float2 u = unpack2<BF>(hi[e]);
-                    lo[e] = pack2<BF>(a - u.x, c2 - u.y);
-                }
-            }
-            const uint32_t r = (lane & 7) + ((lane >> 3) & 1) * 8;
-#pragma unroll
-            for (int j = 0; j < HD / 16; j++) {
-                uint32_t f[4];
-                ldsm4_t(f, vt + r * ROW + (((2 * j + ((lane >> 4) & 1)) ^ (r & 7)) * 16));
-                mma16<BF>(o[2 * j], hi, f[0], f[1]);
-                mma16<BF>(o[2 * j + 1], hi, f[2], f[3]);
-                if (BF) {
-                    mma16<BF>(o[2 * j], lo, f[0], f[1]);
-                    mma16<BF>(o[2 * j + 1], lo, f[2], f[3]);
-                }
-            }
-        }
-        cp_wait<0>();
-        __syncwarp();                                              // the next item's tiles go over the ones just read
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const uint32_t r = g8 + half * 8;
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-            if (r < I.rows) {
-                if (q4 == 0) A.part_ml[I.part + r] = make_float2(m[half], l[half]);
-#pragma unroll
-                for (int j = 0; j < HD / 8; j++) *(float2*)&A.part_o[(I.part + r) * HD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-            }
-        }
-    }
-    if (beside) pdl_wait();
-}
-
-template <int HD>
-__host__ __device__ constexpr int stages() { return HD == 128 ? 3 : 4; }
-template <int HD>
-__host__ __device__ constexpr size_t ring_bytes() { return (size_t)stages<HD>() * 2 * TILE * HD * 2; }
-template <int HD, int RT>
-__host__ __device__ constexpr size_t parts_smem() { return ring_bytes<HD>() + (size_t)16 * RT * 16 * 4 + (size_t)64 * (RT == 8 ? 2 : 1) * 8 + (MAX_BATCH + 4) * 4; }
-
-// RT row tiles of 16; the warps that RT leaves share a tile's positions
-template <bool BF, int HD, int RT>
-__global__ void __launch_bounds__(RT == 8 ? 256 : 128, RT == 8 ? 1 : 2)
-shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
-    constexpr int NW = RT == 8 ? 8 : 4, NT = NW * 32, PG = NW / RT, NP = TILE / PG / 16, STG = stages<HD>(), LD = HD + 8;
-    constexpr uint32_t ROW = HD * 2, HALF = TILE * ROW;
-    extern __shared__ __align__(128) unsigned char smem[];
-    float* so = (float*)smem;                                       // [PG][16 RT][LD] once the tiles are done with
-    float* zone = (float*)(smem + ring_bytes<HD>());                // [16 RT][16]
-    float2* ml = (float2*)(zone + 16 * RT * 16);                    // [PG][16 RT]
-    uint32_t* cum = (uint32_t*)(ml + PG * 16 * RT);
-    __shared__ uint32_t s_k, s_next;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
-    const uint32_t rt = warp % RT, pg = warp / RT;
-    const uint32_t ring = smem_addr(smem);
-    // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait: all that was there before the
-    // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
-    if (!beside) pdl_wait();
-    pdl_release();
-    if (with_tails) {
-        if (warp == 0) {
-            const uint32_t k = cut_tails(A, cum);
-            if (lane == 0) s_k = k;
-        }
-        __syncthreads();
-        if (blockIdx.x == 0)
-            for (uint32_t b = threadIdx.x; b <= A.batch; b += NT) A.plan[b] = cum[b];
-    }
-    const uint32_t items = prefix_items + (with_tails ? cum[A.batch] * A.kv_heads : 0);
-    // Beside the prefix's kernel most CTAs come up when that one leaves the SMs, and the first take what the others have not begun:
-    // items are handed out by a counter.
-    uint32_t w = blockIdx.x;
-    if (beside) {
-        if (threadIdx.x == 0) s_next = atomicAdd(A.next, 1u);
-        __syncthreads();
-        w = s_next;
-    }
-    while (w < items) {
-        uint32_t ahead = w + gridDim.x;
-        if (beside && threadIdx.x == 0) ahead = atomicAdd(A.next, 1u);
-        const Item I = item_of<HD>(A, cum, s_k, w, prefix_items);
-        const bool tail = I.tail, last = I.last;
-        const uint32_t h = I.h, rows = I.rows, token0 = I.token0, from = I.from, c = I.c, n = I.n, b = I.b;
-        const size_t v_off = I.v_off, pitch = 2 * v_off, part = I.part;
-        const uint16_t* kbase = I.kbase;
-        uint32_t to = I.to;
-        uint32_t tiles = (to - from + TILE - 1) / TILE;
-
-        auto load = [&](uint32_t i) {
-            if (i < tiles) {
-                const uint32_t st = ring + (i % STG) * 2 * HALF;
-#pragma unroll 4
-                for (uint32_t e = threadIdx.x; e < TILE * HD / 8; e += NT) {
-                    const uint32_t r = e / (HD / 8), ch = e % (HD / 8), pos = from + i * TILE + r;
-                    const bool in = pos < to;                       // rows past the end: zeros, whatever the cache holds there
-                    const uint16_t* src = kbase + (in ? (size_t)pos * pitch + ch * 8 : 0);
-                    const uint32_t dst = st + r * ROW + ((ch ^ (r & 7)) * 16);
-                    cp16(dst, src, in ? 16 : 0);
-                    cp16(dst + HALF, src + (in ? v_off : 0), in ? 16 : 0);
-                }
-            }
-            cp_commit();
-        };
-        for (int i = 0; i < STG - 1; i++) load(i);
-        // Positions that only some rows see carry weight 0 for the others, which is 0 times their values: where one of those is no number,
-        // the positions are left to the code behind the tiles, which adds them row by row.
-        uint32_t nz = last ? n - c : 0;
-        if (nz) {
-            bool odd = false;
-            for (uint32_t e = threadIdx.x; e < nz * (HD / 8); e += NT) {
-                const uint4 v = *(const uint4*)(kbase + (size_t)(c + e / (HD / 8)) * pitch + v_off + e % (HD / 8) * 8);
-                constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
-                for (uint32_t x : {v.x, v.y, v.z, v.w}) odd |= (x & EXP & 0xffffu) == (EXP & 0xffffu) || (x & EXP & 0xffff0000u) == (EXP & 0xffff0000u);
-            }
-            if (__syncthreads_or(odd)) {
-                cp_wait<0>();
-                __syncthreads();
-                to = max(c, from);
-                tiles = (to - from + TILE - 1) / TILE;
-                for (int i = 0; i < STG - 1; i++) load(i);
-            } else {
-                nz = 0;
-            }
-        }
-
-        // ---- queries of this warp's rows as A fragments
-        uint32_t qf[HD / 16][4];
-        int lim[2];                                                   // the first position that a row does not see
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const uint32_t r = rt * 16 + g8 + half * 8;
-            const bool in = r < rows;
-            lim[half] = last ? min((int)to, (int)(n + r / A.rep + 1) - (int)A.q_len) : (int)to;
-            const uint16_t* qp = A.q + (in ? (size_t)(token0 + r / A.rep) * A.q_stride + (size_t)(h * A.rep + r % A.rep) * HD : 0) + q4 * 2;
-#pragma unroll
-            for (int k = 0; k < HD / 16; k++) {
-                qf[k][half] = in ? *(const uint32_t*)(qp + k * 16) : 0u;
-                qf[k][half + 2] = in ? *(const uint32_t*)(qp + k * 16 + 8) : 0u;
-            }
-        }
-        float o[HD / 8][4] = {};
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
-        for (uint32_t i = 0; i < tiles; i++) {
-            cp_wait<STG - 2>();
-            __syncthreads();
-            load(i + STG - 1);
-            const uint32_t p0 = from + i * TILE + pg * (TILE / PG);   // this warp's first position
-            if (p0 >= to || rt * 16 >= rows) continue;                 // the same for the whole warp
-            const uint32_t kt = ring + (i % STG) * 2 * HALF, vt = kt + HALF;
-            float s[2 * NP][4];
-#pragma unroll
-            for (int t = 0; t < NP; t++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[2 * t][e] = s[2 * t + 1][e] = 0.0f;
-                const uint32_t r = pg * (TILE / PG) + t * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
-#pragma unroll
-                for (int k = 0; k < HD / 16; k++) {
-                    uint32_t f[4];
-                    ldsm4(f, kt + r * ROW + (((2 * k + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
-                    mma16<BF>(s[2 * t], qf[k], f[0], f[1]);
-                    mma16<BF>(s[2 * t + 1], qf[k], f[2], f[3]);
-                }
-            }
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int t = 0; t < 2 * NP; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool in = (int)(p0 + t * 8 + q4 * 2 + (e & 1)) < lim[e >> 1];
-                    s[t][e] = in ? s[t][e] * A.sc : -INFINITY;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
-                }
-            if (tail && A.scores) {
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    const uint32_t r = rt * 16 + g8 + half * 8;
-                    float* sp = A.scores + (((size_t)b * A.kv_heads + h) * rows + r) * A.nslots;
-                    if (r < rows)
+                    mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+                    mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
+                }
+                if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
 #pragma unroll
-                        for (int t = 0; t < 2 * NP; t++) {
-                            const uint32_t p = p0 + t * 8 + q4 * 2;
-                            if (p < to) sp[p] = s[t][2 * half];
-                            if (p + 1 < to) sp[p + 1] = s[t][2 * half + 1];
+                    for (int half = 0; half < 2; half++) {
+                        const float mn = fmaxf(m[half], mx[half]), f = m[half] == -INFINITY ? 0.0f : sm100::ex2(m[half] - mn);
+                        if (mn > m[half]) {
+                            m[half] = mn;
+                            l[half] *= f;
+#pragma unroll
+                            for (int j = 0; j < HD / 8; j++) { o[j][2 * half] *= f; o[j][2 * half + 1] *= f; }
                         }
-                }
-            }
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-                mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-            }
-            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const float mn = fmaxf(m[half], mx[half]), f = m[half] == -INFINITY ? 0.0f : sm100::ex2(m[half] - mn);
-                    if (mn > m[half]) {
-                        m[half] = mn;
-                        l[half] *= f;
-#pragma unroll
-                        for (int j = 0; j < HD / 8; j++) { o[j][2 * half] *= f; o[j][2 * half + 1] *= f; }
                     }
                 }
-            }
-            const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+                const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
 #pragma unroll
-            for (int t = 0; t < NP; t++) {
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        s[t][e] = sm100::ex2(s[t][e] - off[e >> 1]);
+                        l[e >> 1] += s[t][e];
+                    }
+                // Positions that only some rows see have weight 0 for the others, which is 0 times their values: where one of those is no
+                // number, the tile's values are added row by row instead.
+                bool odd = false;
+                if (I.last && p0 + 16 > I.c && I.n > I.c) {
+                    constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
+#pragma unroll 1
+                    for (uint32_t u = 0; u < HD / 16; u++) {
+                        const uint32_t e = u * 32 + lane, r = e / (HD / 8);
+                        const uint4 v = *(const uint4*)(smem + (vt - base) + r * ROW + ((e % (HD / 8)) ^ (r & 7)) * 16);
+                        for (uint32_t x : {v.x, v.y, v.z, v.w}) odd |= (x & EXP & 0xffffu) == (EXP & 0xffffu) || (x & EXP & 0xffff0000u) == (EXP & 0xffff0000u);
+                    }
+                    odd = __any_sync(0xffffffffu, odd);
+                }
+                if (odd) {
+#pragma unroll 1
+                    for (uint32_t col = 0; col < 16; col++) {
+                        const int from = (int)((lane & ~3u) + (col % 8) / 2);
+                        float p[2];
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const float a = col < 8 ? s[0][2 * half] : s[1][2 * half], b = col < 8 ? s[0][2 * half + 1] : s[1][2 * half + 1];
+                            p[half] = __shfl_sync(0xffffffffu, col % 2 ? b : a, from);
+                        }
+#pragma unroll
+                        for (int j = 0; j < HD / 8; j++) {
+                            const float2 v = unpack2<BF>(*(const uint32_t*)(smem + (vt - base) + col * ROW + ((j ^ (col & 7)) * 16) + q4 * 4));
+#pragma unroll
+                            for (int half = 0; half < 2; half++)
+                                if ((int)(p0 + col) < lim[half]) { o[j][2 * half] = fmaf(p[half], v.x, o[j][2 * half]); o[j][2 * half + 1] = fmaf(p[half], v.y, o[j][2 * half + 1]); }
+                        }
+                    }
+                    continue;
+                }
                 uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {                          // fragment register e: tile 2 t + e / 2, rows of half e % 2
-                    float* x = &s[2 * t + (e >> 1)][2 * (e & 1)];
-                    const float a = sm100::ex2(x[0] - off[e & 1]), c2 = sm100::ex2(x[1] - off[e & 1]);
-                    l[e & 1] += a + c2;
+                for (int e = 0; e < 4; e++) {                          // fragment register e: tile e / 2, rows of half e % 2
+                    const float a = s[e >> 1][2 * (e & 1)], c2 = s[e >> 1][2 * (e & 1) + 1];
                     hi[e] = pack2<BF>(a, c2);
                     // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
                     if (BF) {
@@ -528,7 +322,7 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
                         lo[e] = pack2<BF>(a - u.x, c2 - u.y);
                     }
                 }
-                const uint32_t r = pg * (TILE / PG) + t * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+                const uint32_t r = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
                 for (int j = 0; j < HD / 16; j++) {
                     uint32_t f[4];
@@ -543,67 +337,20 @@ shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tai
             }
         }
         cp_wait<0>();
-        __syncthreads();
-        // ---- the warps' results of a row together
+        if (part == 0 && lane == 0) s_next[group][turn] = ahead;
+        meet();                                                    // the next item's tiles go over the ones just read
+        w = s_next[group][turn];
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-            const uint32_t r = rt * 16 + g8 + half * 8;
+            const uint32_t r = row0 + g8 + half * 8;
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-            if (r >= rows) continue;
-            if (q4 == 0) ml[pg * 16 * RT + r] = make_float2(m[half], l[half]);
+            if (r < I.rows) {
+                if (q4 == 0) A.part_ml[I.out + r] = make_float2(m[half], l[half]);
 #pragma unroll
-            for (int j = 0; j < HD / 8; j++) *(float2*)&so[(size_t)(pg * 16 * RT + r) * LD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-        }
-        for (uint32_t e = warp; e < rows * nz; e += NW) {
-            const uint32_t r = e / nz, i = e % nz, t = r / A.rep;
-            float s = -INFINITY;
-            if (c + i + A.q_len < n + t + 1) {                         // position c + i < n - q_len + t + 1
-                const uint16_t* qp = A.q + (size_t)(token0 + t) * A.q_stride + (size_t)(h * A.rep + r % A.rep) * HD + lane * (HD / 32);
-                const uint16_t* kp = kbase + (size_t)(c + i) * pitch + lane * (HD / 32);
-                float d = 0.0f;
-#pragma unroll
-                for (int x = 0; x < HD / 32; x += 2) {
-                    const float2 a = unpack2<BF>(*(const uint32_t*)(qp + x)), k2 = unpack2<BF>(*(const uint32_t*)(kp + x));
-                    d = fmaf(a.x, k2.x, fmaf(a.y, k2.y, d));
-                }
-                s = warp_sum(d) * A.sc;
-            }
-            if (lane == 0) {
-                zone[r * 16 + i] = s;
-                if (A.scores) A.scores[(((size_t)b * A.kv_heads + h) * rows + r) * A.nslots + c + i] = s;
+                for (int j = 0; j < HD / 8; j++) *(float2*)&A.part_o[(I.out + r) * HD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
             }
         }
-        __syncthreads();
-        for (uint32_t e = threadIdx.x; e < rows * (HD / 4); e += NT) {
-            const uint32_t r = e / (HD / 4), c4 = e % (HD / 4);
-            float M = -INFINITY, L = 0.0f;
-#pragma unroll
-            for (int p = 0; p < PG; p++) M = fmaxf(M, ml[p * 16 * RT + r].x);
-            for (uint32_t i = 0; i < nz; i++) M = fmaxf(M, zone[r * 16 + i]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int p = 0; p < PG; p++) {
-                const float2 x = ml[p * 16 * RT + r];
-                const float f = x.x == -INFINITY ? (x.y == 0.0f ? 0.0f : 1.0f) : sm100::ex2(x.x - M);   // a sum without a maximum is no number and stays one
-                const float4 v = *(const float4*)&so[(size_t)(p * 16 * RT + r) * LD + c4 * 4];
-                acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-                L = fmaf(x.y, f, L);
-            }
-            const uint32_t t = r / A.rep;
-            for (uint32_t i = 0; i < nz && c + i + A.q_len < n + t + 1; i++) {
-                const float p = sm100::ex2(zone[r * 16 + i] - (M == -INFINITY ? 0.0f : M));
-                const uint2 vw = *(const uint2*)(kbase + (size_t)(c + i) * pitch + v_off + c4 * 4);
-                const float2 va = unpack2<BF>(vw.x), vb = unpack2<BF>(vw.y);
-                acc.x = fmaf(p, va.x, acc.x); acc.y = fmaf(p, va.y, acc.y); acc.z = fmaf(p, vb.x, acc.z); acc.w = fmaf(p, vb.y, acc.w);
-                L += p;
-            }
-            *(float4*)&A.part_o[(part + r) * HD + c4 * 4] = acc;
-            if (c4 == 0) A.part_ml[part + r] = make_float2(M, L);
-        }
-        if (threadIdx.x == 0) s_next = ahead;
-        __syncthreads();
-        w = s_next;
     }
     if (beside) pdl_wait();
 }
@@ -721,29 +468,17 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, u
 template <bool BF, int HD, int RT>
 bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, bool tails, bool beside) {
     static int have[64] = {};
-    const size_t smem = parts_smem<HD, RT>();
-    if (!ensure_dyn_smem(shared_parts_kernel<BF, HD, RT>, smem, have)) return false;
-    const uint32_t fit = RT == 8 ? 1 : HD == 128 ? 2 : 3;
+    if (!ensure_dyn_smem(shared_parts_kernel<BF, HD, RT>, parts_smem<HD, RT>(), have)) return false;
     const size_t items = prefix_items + (tails ? ((size_t)a.t_slices + a.batch) * a.kv_heads : 0);
     if (!items) return true;
     g_launches++;
-    return launch_pdl(shared_parts_kernel<BF, HD, RT>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * fit)), dim3(RT == 8 ? 256 : 128), smem, st, a,
-                      prefix_items, tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
-}
-template <bool BF, int HD>
-bool launch_warps(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, bool tails, bool beside) {
-    static int have[64] = {};
-    if (!ensure_dyn_smem(shared_warps_kernel<BF, HD>, warps_smem<HD>(), have)) return false;
-    const size_t items = prefix_items + (tails ? ((size_t)a.t_slices + a.batch) * a.kv_heads : 0);
-    if (!items) return true;
-    g_launches++;
-    return launch_pdl(shared_warps_kernel<BF, HD>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * 2)), dim3(128), warps_smem<HD>(), st, a, prefix_items,
-                      tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
+    return launch_pdl(shared_parts_kernel<BF, HD, RT>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * (RT == 8 ? 1 : 2))), dim3(warps_of<RT>() * 32),
+                      parts_smem<HD, RT>(), st, a, prefix_items, tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
 }
 template <bool BF, int HD>
 bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t prefix_items, bool tails, bool beside) {
     switch (rt) {
-        case 1: return launch_warps<BF, HD>(st, a, prefix_items, tails, beside);
+        case 1: return launch_parts<BF, HD, 1>(st, a, prefix_items, tails, beside);
         case 2: return launch_parts<BF, HD, 2>(st, a, prefix_items, tails, beside);
         case 4: return launch_parts<BF, HD, 4>(st, a, prefix_items, tails, beside);
         default: return launch_parts<BF, HD, 8>(st, a, prefix_items, tails, beside);
@@ -789,7 +524,7 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     const uint32_t unit = l.umma ? 128 : TILE, tiles = (a.n_prefix + unit - 1) / unit;
     a.p_slices = a.p_len = 0;
     if (tiles) {
-        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * (l.t_rt == 8 ? 1 : l.t_rt == 1 ? 8 : 2);
+        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * 8 / l.t_rt;
         uint32_t best = l.umma ? 1 : std::min(tiles, std::max(1u, fit / groups));
         size_t least = SIZE_MAX;
         // rounds over the SMs of slices and about three tiles' time to begin and end one
@@ -800,7 +535,7 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
         a.p_len = (tiles + best - 1) / best * unit;
         a.p_slices = (a.n_prefix + a.p_len - 1) / a.p_len;
     }
-    a.t_slices = std::max(1u, (l.t_rt == 1 ? 24 : 6) * SMS / a.kv_heads);
+    a.t_slices = std::max(1u, std::max(6u, 24 / l.t_rt) * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     l.ml = up((size_t)(a.batch + 2) * 4);
