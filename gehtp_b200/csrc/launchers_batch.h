@@ -25,7 +25,7 @@ struct SharedArgs {
     float* part_o;                                 // [partial row][head_dim], the prefix's first
     float2* part_ml;                               // [partial row] {m, sum}
     float* scores;                                 // s of every tail position: [sequence][key head][row][nslots], or NULL
-    uint32_t* next;                                // next item of the tails' kernel where it runs beside the prefix's, which sets it to 0
+    uint32_t* next;                                // where the tails' kernel runs beside the prefix's, which sets both to 0: items handed out; items + 1
     uint32_t* plan;                                // written by the first kernel: slices in front of each sequence's, batch + 1 of them
     __host__ __device__ size_t p_rows() const { return (size_t)p_tiles * kv_heads * p_slices * p_tokens * rep; }
 };

@@ -154,6 +154,16 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
     // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
     if (!beside) pdl_wait();
     pdl_release();
+    // A CTA that comes up when all items have been handed out has nothing left to work out: the first one left their number.
+    if (beside) {
+        if (threadIdx.x == 0) {
+            const uint32_t all = *(volatile uint32_t*)(A.next + 1), out = *(volatile uint32_t*)A.next;
+            s_k = all && out >= all - 1;
+        }
+        __syncthreads();
+        if (s_k) { pdl_wait(); return; }
+        __syncthreads();
+    }
     if (with_tails) {
         if (warp == 0) {
             const uint32_t k = cut_tails(A, cum);
@@ -168,6 +178,7 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
     // items are handed out by a counter.
     uint32_t w = blockIdx.x + gridDim.x * group, turn = 0;
     if (beside) {
+        if (threadIdx.x == 0) *(volatile uint32_t*)(A.next + 1) = items + 1;
         if (part == 0 && lane == 0) s_next[group][1] = atomicAdd(A.next, 1u);
         meet();
         w = s_next[group][1];
@@ -358,7 +369,7 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
 // Places of a row's partial results: `first` + i * step for i < count, of the prefix and of the tail.
 struct RowParts { size_t p_first, p_step, t_first, t_step; uint32_t p_count, t_count; };
 
-__device__ __forceinline__ RowParts row_parts(const SharedArgs& A, uint32_t token, uint32_t head) {
+__device__ __forceinline__ RowParts row_parts(const SharedArgs& A, const uint32_t* plan, uint32_t token, uint32_t head) {
     RowParts x;
     const uint32_t h = head / A.rep, g = head % A.rep;
     x.p_step = (size_t)A.p_tokens * A.rep;
@@ -368,8 +379,8 @@ __device__ __forceinline__ RowParts row_parts(const SharedArgs& A, uint32_t toke
     x.t_step = (size_t)A.kv_heads * rows;
     x.t_count = 0; x.t_first = 0;
     if (A.nslots) {
-        const uint32_t c0 = A.plan[b];
-        x.t_count = A.plan[b + 1] - c0;
+        const uint32_t c0 = plan[b];
+        x.t_count = plan[b + 1] - c0;
         x.t_first = A.p_rows() + ((size_t)c0 * A.kv_heads + h) * rows + (token % A.q_len) * A.rep + g;
     }
     return x;
@@ -379,76 +390,118 @@ __device__ __forceinline__ size_t part_at(const RowParts& x, uint32_t i) {
 }
 __device__ __forceinline__ float part_factor(float2 ml, float M) { return ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : sm100::ex2(ml.x - M); }
 
-constexpr uint32_t W_CHUNK = 512;
+constexpr uint32_t W_CHUNK = 1024;
 
-// The first `row_blocks` CTAs: WR warps to a row of the result. The others: 512 tail positions of a (sequence, key head) each.
+// The first `weight_blocks` CTAs: 1024 tail positions of a (sequence, key head) each. The others stay and walk the rows of the result, WR warps
+// to one, with eight partial results on their way at a time and maxima and sums beside them. What a call's end takes is
+// latencies one behind the other: 2048 rows of 18 slices and their tails took 20 us by a warp each that read the maxima first, @@
+// this way.
 template <bool BF, int HD, int WR>
-__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, uint32_t row_blocks, uint32_t chunks) {
+__global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A, uint32_t weight_blocks, uint32_t chunks) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_release();
-    if (blockIdx.x < row_blocks) {
-        const uint32_t heads = A.kv_heads * A.rep, row = blockIdx.x * (8 / WR) + warp / WR, wr = warp % WR;
-        const bool there = row < A.batch * A.q_len * heads;
-        if (WR == 1 && !there) return;
-        constexpr int V = HD / 32;
-        float acc[V] = {};
-        float inv = 0.0f;
-        if (there) {
-        const RowParts x = row_parts(A, row / heads, row % heads);
-        const uint32_t count = x.p_count + x.t_count;
-        float M = -INFINITY, L = 0.0f;
-        for (uint32_t i = lane; i < count; i += 32) M = fmaxf(M, __ldcg(&A.part_ml[part_at(x, i)]).x);
-        M = warp_max(M);
-        for (uint32_t i0 = 0; i0 < count; i0 += 32) {
-            const uint32_t mine = i0 + lane;
-            const float2 ml = mine < count ? __ldcg(&A.part_ml[part_at(x, mine)]) : make_float2(-INFINITY, 0.0f);
-            const float f = part_factor(ml, M);
-            L = fmaf(ml.y, f, L);
-            const uint32_t here = min(32u, count - i0);
-#pragma unroll 4
-            for (uint32_t i = wr; i < here; i += WR) {
-                const float fi = __shfl_sync(0xffffffffu, f, i);
-                const float* p = A.part_o + part_at(x, i0 + i) * HD + lane * V;
-                if (V == 4) {
-                    const float4 v = __ldcg((const float4*)p);
-                    acc[0] = fmaf(v.x, fi, acc[0]); acc[1] = fmaf(v.y, fi, acc[1]); acc[V - 2] = fmaf(v.z, fi, acc[V - 2]); acc[V - 1] = fmaf(v.w, fi, acc[V - 1]);
-                } else {
-                    const float2 v = __ldcg((const float2*)p);
-                    acc[0] = fmaf(v.x, fi, acc[0]); acc[1] = fmaf(v.y, fi, acc[1]);
+    if (blockIdx.x >= weight_blocks) {
+        __shared__ uint32_t plan[MAX_BATCH + 1];
+        if (A.nslots)
+            for (uint32_t b = threadIdx.x; b <= A.batch; b += 256) plan[b] = A.plan[b];
+        __syncthreads();
+        const uint32_t heads = A.kv_heads * A.rep, rows = A.batch * A.q_len * heads, wr = warp % WR, step = (gridDim.x - weight_blocks) * (8 / WR);
+        for (uint32_t row = (blockIdx.x - weight_blocks) * (8 / WR) + warp / WR; ; row += step) {
+            const bool there = row < rows;
+            if (WR == 1 ? !there : !__syncthreads_or(there)) return;
+            constexpr int V = HD / 32, U = 8;
+            float acc[V] = {};
+            float M = -INFINITY, L = 0.0f;
+            if (there) {
+                const RowParts x = row_parts(A, plan, row / heads, row % heads);
+                const uint32_t count = x.p_count + x.t_count;
+                for (uint32_t i0 = wr * U; i0 < count; i0 += WR * U) {
+                    float2 ml[U];
+                    float v[U][V];
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        ml[u] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                        for (int e = 0; e < V; e++) v[u][e] = 0.0f;
+                        if (i0 + u < count) {
+                            const size_t at = part_at(x, i0 + u);
+                            ml[u] = __ldcg(&A.part_ml[at]);
+                            const float* p = A.part_o + at * HD + lane * V;
+                            if constexpr (V == 4) { const float4 w = __ldcg((const float4*)p); v[u][0] = w.x; v[u][1] = w.y; v[u][2] = w.z; v[u][3] = w.w; }
+                            else { const float2 w = __ldcg((const float2*)p); v[u][0] = w.x; v[u][1] = w.y; }
+                        }
+                    }
+                    float top = M;
+#pragma unroll
+                    for (int u = 0; u < U; u++) top = fmaxf(top, ml[u].x);
+                    const float back = part_factor(make_float2(M, L), top);
+                    L *= back;
+#pragma unroll
+                    for (int e = 0; e < V; e++) acc[e] *= back;
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const float f = part_factor(ml[u], top);
+                        L = fmaf(ml[u].y, f, L);
+#pragma unroll
+                        for (int e = 0; e < V; e++) acc[e] = fmaf(v[u][e], f, acc[e]);
+                    }
+                    M = top;
                 }
             }
-        }
-        L = warp_sum(L);
-        inv = L == 0.0f ? 0.0f : 1.0f / L;                  // a row that sees nothing: zeros
-        }
-        if (WR > 1) {
-            __shared__ float sums[8][HD];
+            if (WR > 1) {
+                __shared__ float sums[8][HD];
+                __shared__ float2 sums_ml[8];
 #pragma unroll
-            for (int v = 0; v < V; v++) sums[warp][v * 32 + lane] = acc[v];
-            __syncthreads();
-            if (wr || !there) return;
+                for (int e = 0; e < V; e++) sums[warp][e * 32 + lane] = acc[e];
+                if (lane == 0) sums_ml[warp] = make_float2(M, L);
+                __syncthreads();
+                if (wr || !there) continue;
+                float top = M;
 #pragma unroll
-            for (int w = 1; w < WR; w++)
+                for (int w = 1; w < WR; w++) top = fmaxf(top, sums_ml[warp + w].x);
+                const float back = part_factor(make_float2(M, L), top);
+                L *= back;
 #pragma unroll
-                for (int v = 0; v < V; v++) acc[v] += sums[warp + w][v * 32 + lane];
+                for (int e = 0; e < V; e++) acc[e] *= back;
+#pragma unroll
+                for (int w = 1; w < WR; w++) {
+                    const float f = part_factor(sums_ml[warp + w], top);
+                    L = fmaf(sums_ml[warp + w].y, f, L);
+#pragma unroll
+                    for (int e = 0; e < V; e++) acc[e] = fmaf(sums[warp + w][e * 32 + lane], f, acc[e]);
+                }
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;      // a row that sees nothing: zeros
+            uint32_t* out = (uint32_t*)(A.out + (size_t)row * HD + lane * V);
+            if (V == 4) *(uint2*)out = make_uint2(pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[V - 2] * inv, acc[V - 1] * inv));
+            else *out = pack2<BF>(acc[0] * inv, acc[1] * inv);
         }
-        uint32_t* out = (uint32_t*)(A.out + (size_t)row * HD + lane * V);
-        if (V == 4) *(uint2*)out = make_uint2(pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[V - 2] * inv, acc[V - 1] * inv));
-        else *out = pack2<BF>(acc[0] * inv, acc[1] * inv);
-        return;
     }
     __shared__ float2 norm[MAX_ROWS];       // {maximum, 1 / sum} of the rows of the key head
-    const uint32_t u = blockIdx.x - row_blocks, p0 = (u % chunks) * W_CHUNK, h = (u / chunks) % A.kv_heads, b = u / chunks / A.kv_heads;
+    const uint32_t u = blockIdx.x, p0 = (u % chunks) * W_CHUNK, h = (u / chunks) % A.kv_heads, b = u / chunks / A.kv_heads;
     const uint32_t n = tail_length(A, b), rows = A.q_len * A.rep;
     if (p0 >= n) return;
+    const size_t head = (size_t)b * A.kv_heads + h;
+    // what does not need the rows' sums is on its way before them: the scores of four rows
+    float sum[4], s0[4][4];
+    const float* scores = A.scores + head * rows * A.nslots + p0 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool in = p0 + i * 256 + threadIdx.x < n;
+        sum[i] = in && A.weights_in ? A.weights_in[head * A.nslots + p0 + i * 256 + threadIdx.x] : 0.0f;
+#pragma unroll
+        for (uint32_t r = 0; r < 4; r++) s0[r][i] = in && r < rows ? __ldcg(scores + (size_t)r * A.nslots + i * 256) : -INFINITY;
+    }
     for (uint32_t r = warp; r < rows; r += 8) {
-        const RowParts x = row_parts(A, b * A.q_len + r / A.rep, h * A.rep + r % A.rep);
+        const RowParts x = row_parts(A, A.plan, b * A.q_len + r / A.rep, h * A.rep + r % A.rep);
         const uint32_t count = x.p_count + x.t_count;
-        float M = -INFINITY, L = 0.0f;
-        for (uint32_t i = lane; i < count; i += 32) M = fmaxf(M, __ldcg(&A.part_ml[part_at(x, i)]).x);
+        const float2 none = make_float2(-INFINITY, 0.0f), first = lane < count ? __ldcg(&A.part_ml[part_at(x, lane)]) : none;
+        float M = first.x;
+        for (uint32_t i = lane + 32; i < count; i += 32) M = fmaxf(M, __ldcg(&A.part_ml[part_at(x, i)]).x);
         M = warp_max(M);
-        for (uint32_t i = lane; i < count; i += 32) {
+        float L = first.y * part_factor(first, M);
+        for (uint32_t i = lane + 32; i < count; i += 32) {
             const float2 ml = __ldcg(&A.part_ml[part_at(x, i)]);
             L = fmaf(ml.y, part_factor(ml, M), L);
         }
@@ -456,13 +509,24 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedArgs A, u
         if (lane == 0) norm[r] = make_float2(M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L);
     }
     __syncthreads();
-    const size_t head = (size_t)b * A.kv_heads + h;
-    for (uint32_t p = p0 + threadIdx.x; p < min(n, p0 + W_CHUNK); p += 256) {
-        float sum = A.weights_in ? A.weights_in[head * A.nslots + p] : 0.0f;
-        float add = 0.0f;
-        for (uint32_t r = 0; r < rows; r++) add = fmaf(sm100::ex2(__ldcg(&A.scores[(head * rows + r) * A.nslots + p]) - norm[r].x), norm[r].y, add);
-        A.weights[head * A.nslots + p] = sum + add;
+    float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t r = 0; r < 4; r++)
+        if (r < rows) {
+            const float2 x = norm[r];
+#pragma unroll
+            for (int i = 0; i < 4; i++) add[i] = fmaf(sm100::ex2(s0[r][i] - x.x), x.y, add[i]);
+        }
+#pragma unroll 2
+    for (uint32_t r = 4; r < rows; r++) {
+        const float2 x = norm[r];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (p0 + i * 256 + threadIdx.x < n) add[i] = fmaf(sm100::ex2(__ldcg(scores + (size_t)r * A.nslots + i * 256) - x.x), x.y, add[i]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (p0 + i * 256 + threadIdx.x < n) A.weights[head * A.nslots + p0 + i * 256 + threadIdx.x] = sum[i] + add[i];
 }
 
 template <bool BF, int HD, int RT>
@@ -488,11 +552,11 @@ template <bool BF, int HD>
 bool launch_merge(cudaStream_t st, const SharedArgs& a) {
     const size_t rows = (size_t)a.batch * a.q_len * a.kv_heads * a.rep;
     const uint32_t chunks = (a.nslots + W_CHUNK - 1) / W_CHUNK;
-    // four warps to a row while a warp each would leave the SMs room
-    const bool wide = rows <= 8 * SMS;
-    const size_t blocks = wide ? (rows + 1) / 2 : (rows + 7) / 8, more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
+    // four warps to a row while they all find room on the SMs
+    const bool wide = rows <= 16 * SMS;
+    const size_t blocks = std::min<size_t>(wide ? (rows + 1) / 2 : (rows + 7) / 8, SMS * 3), more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
     g_launches++;
-    return launch_pdl(wide ? shared_merge_kernel<BF, HD, 4> : shared_merge_kernel<BF, HD, 1>, dim3((uint32_t)(blocks + more)), dim3(256), 0, st, a, (uint32_t)blocks,
+    return launch_pdl(wide ? shared_merge_kernel<BF, HD, 4> : shared_merge_kernel<BF, HD, 1>, dim3((uint32_t)(blocks + more)), dim3(256), 0, st, a, (uint32_t)more,
                       std::max(1u, chunks)) == cudaSuccess;
 }
 
@@ -538,7 +602,7 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     a.t_slices = std::max(1u, std::max(6u, 24 / l.t_rt) * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    l.ml = up((size_t)(a.batch + 2) * 4);
+    l.ml = up((size_t)(a.batch + 3) * 4);
     l.o = l.ml + up(parts * 8);
     l.scores = l.o + up(parts * hd * 4);
     l.total = l.scores + (with_weights ? up((size_t)a.batch * a.kv_heads * a.q_len * a.rep * a.nslots * 4) : 0);
@@ -615,7 +679,7 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
     a.weights_in = weights_in_dev; a.weights = weights_dev; a.out = (uint16_t*)out_dev; a.q_stride = q_stride;
     a.sc = scale * 1.4426950408889634f;
     unsigned char* ws = (unsigned char*)workspace_dev;
-    a.next = (uint32_t*)ws; a.plan = a.next + 1; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
+    a.next = (uint32_t*)ws; a.plan = a.next + 2; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
     a.scores = weights_dev ? (float*)(ws + l.scores) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = dtype == GEHTP_DT_BF16, umma = n_prefix && l.umma;

@@ -136,7 +136,7 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
     const uint32_t tmem = bars->tmem_base;
     pdl_wait();
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
-        if (threadIdx.x == 0) { atomicExch(A.next, 0u); __threadfence(); }
+        if (threadIdx.x == 0) { atomicExch(A.next, 0u); atomicExch(A.next + 1, 0u); __threadfence(); }
         __syncthreads();
     }
     pdl_release();     // behind the wait: the tails' kernel starts beside this one and may read all that was there before the call
