@@ -11,6 +11,14 @@ namespace gehtp {
 // prefix together are those of p_tokens tokens (a row tile), those that meet a tail are the q_len * rep of its sequence.
 // Every (row tile, key head, slice of the prefix) and every (sequence, key head, slice of its tail) leaves a partial result per
 // row: the sum of 2^(s - m) v, the sum of 2^(s - m) and the maximum m, with s = log2(e) * scale * q.k.
+// n / d by a product, for n * d < 2^32
+struct Div {
+    uint64_t m;
+    Div() = default;
+    explicit Div(uint32_t d) : m(((1ull << 32) + d - 1) / d) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((n * m) >> 32); }
+};
+
 struct SharedArgs {
     const uint16_t *q, *prefix, *tail;
     const int32_t* n_tail;
@@ -21,6 +29,7 @@ struct SharedArgs {
     size_t q_stride;
     uint32_t p_tokens, p_tiles, p_slices, p_len;   // prefix: slices of p_len positions
     uint32_t t_slices;                             // the tails of all sequences are cut into about so many slices
+    Div by_rep, by_q_len, by_p_tokens;             // of heads below 65536 by up to 128, of tokens below 16384 by up to 16 and 128
     float sc;                                      // log2(e) * scale
     float* part_o;                                 // [partial row][head_dim], the prefix's first
     float2* part_ml;                               // [partial row] {m, sum}

@@ -367,21 +367,20 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
 }
 
 // Places of a row's partial results: `first` + i * step for i < count, of the prefix and of the tail.
-struct RowParts { size_t p_first, p_step, t_first, t_step; uint32_t p_count, t_count; };
+struct RowParts { uint32_t p_first, p_step, p_count, t_first, t_step, t_count; };
 
 __device__ __forceinline__ RowParts row_parts(const SharedArgs& A, const uint32_t* plan, uint32_t token, uint32_t head) {
     RowParts x;
-    const uint32_t h = head / A.rep, g = head % A.rep;
-    x.p_step = (size_t)A.p_tokens * A.rep;
-    x.p_count = A.n_prefix ? A.p_slices : 0;
-    x.p_first = x.p_count ? ((size_t)(token / A.p_tokens) * A.kv_heads + h) * A.p_slices * x.p_step + (token % A.p_tokens) * A.rep + g : 0;
-    const uint32_t b = token / A.q_len, rows = A.q_len * A.rep;
-    x.t_step = (size_t)A.kv_heads * rows;
-    x.t_count = 0; x.t_first = 0;
+    const uint32_t h = A.by_rep(head), g = head - h * A.rep, tile = A.by_p_tokens(token), b = A.by_q_len(token), rows = A.q_len * A.rep;
+    x.p_step = A.p_tokens * A.rep;
+    x.p_count = A.p_slices;
+    x.p_first = (tile * A.kv_heads + h) * A.p_slices * x.p_step + (token - tile * A.p_tokens) * A.rep + g;
+    x.t_step = A.kv_heads * rows;
+    x.t_count = x.t_first = 0;
     if (A.nslots) {
         const uint32_t c0 = plan[b];
         x.t_count = plan[b + 1] - c0;
-        x.t_first = A.p_rows() + ((size_t)c0 * A.kv_heads + h) * rows + (token % A.q_len) * A.rep + g;
+        x.t_first = (uint32_t)A.p_rows() + (c0 * A.kv_heads + h) * rows + (token - b * A.q_len) * A.rep + g;
     }
     return x;
 }
@@ -406,15 +405,16 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
         if (A.nslots)
             for (uint32_t b = threadIdx.x; b <= A.batch; b += 256) plan[b] = A.plan[b];
         __syncthreads();
-        const uint32_t heads = A.kv_heads * A.rep, rows = A.batch * A.q_len * heads, wr = warp % WR, step = (gridDim.x - weight_blocks) * (8 / WR);
-        for (uint32_t row = (blockIdx.x - weight_blocks) * (8 / WR) + warp / WR; ; row += step) {
-            const bool there = row < rows;
-            if (WR == 1 ? !there : !__syncthreads_or(there)) return;
+        // a CTA's turn: 8 / WR neighbouring heads of a token
+        const uint32_t heads = A.kv_heads * A.rep, wr = warp % WR, each = (heads + 8 / WR - 1) / (8 / WR), turns = A.batch * A.q_len * each;
+        for (uint32_t turn = blockIdx.x - weight_blocks; turn < turns; turn += gridDim.x - weight_blocks) {
+            const uint32_t token = turn / each, head = (turn - token * each) * (8 / WR) + warp / WR;
+            const bool there = head < heads;
             constexpr int V = HD / 32, U = 8;
             float acc[V] = {};
             float M = -INFINITY, L = 0.0f;
             if (there) {
-                const RowParts x = row_parts(A, plan, row / heads, row % heads);
+                const RowParts x = row_parts(A, plan, token, head);
                 const uint32_t count = x.p_count + x.t_count;
                 for (uint32_t i0 = wr * U; i0 < count; i0 += WR * U) {
                     float2 ml[U];
@@ -452,9 +452,10 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
             if (WR > 1) {
                 __shared__ float sums[8][HD];
                 __shared__ float2 sums_ml[8];
+                __syncthreads();                            // the turn before has been read
+                if (lane == 0) sums_ml[warp] = make_float2(M, L);
 #pragma unroll
                 for (int e = 0; e < V; e++) sums[warp][e * 32 + lane] = acc[e];
-                if (lane == 0) sums_ml[warp] = make_float2(M, L);
                 __syncthreads();
                 if (wr || !there) continue;
                 float top = M;
@@ -472,11 +473,13 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
                     for (int e = 0; e < V; e++) acc[e] = fmaf(sums[warp + w][e * 32 + lane], f, acc[e]);
                 }
             }
+            if (!there) continue;
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;      // a row that sees nothing: zeros
-            uint32_t* out = (uint32_t*)(A.out + (size_t)row * HD + lane * V);
+            uint32_t* out = (uint32_t*)(A.out + ((size_t)token * heads + head) * HD + lane * V);
             if (V == 4) *(uint2*)out = make_uint2(pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[V - 2] * inv, acc[V - 1] * inv));
             else *out = pack2<BF>(acc[0] * inv, acc[1] * inv);
         }
+        return;
     }
     __shared__ float2 norm[MAX_ROWS];       // {maximum, 1 / sum} of the rows of the key head
     const uint32_t u = blockIdx.x, p0 = (u % chunks) * W_CHUNK, h = (u / chunks) % A.kv_heads, b = u / chunks / A.kv_heads;
@@ -494,7 +497,7 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
         for (uint32_t r = 0; r < 4; r++) s0[r][i] = in && r < rows ? __ldcg(scores + (size_t)r * A.nslots + i * 256) : -INFINITY;
     }
     for (uint32_t r = warp; r < rows; r += 8) {
-        const RowParts x = row_parts(A, A.plan, b * A.q_len + r / A.rep, h * A.rep + r % A.rep);
+        const RowParts x = row_parts(A, A.plan, b * A.q_len + A.by_rep(r), h * A.rep + r - A.by_rep(r) * A.rep);
         const uint32_t count = x.p_count + x.t_count;
         const float2 none = make_float2(-INFINITY, 0.0f), first = lane < count ? __ldcg(&A.part_ml[part_at(x, lane)]) : none;
         float M = first.x;
@@ -550,11 +553,11 @@ bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t
 }
 template <bool BF, int HD>
 bool launch_merge(cudaStream_t st, const SharedArgs& a) {
-    const size_t rows = (size_t)a.batch * a.q_len * a.kv_heads * a.rep;
+    const size_t tokens = (size_t)a.batch * a.q_len, heads = (size_t)a.kv_heads * a.rep;
     const uint32_t chunks = (a.nslots + W_CHUNK - 1) / W_CHUNK;
     // four warps to a row while they all find room on the SMs
-    const bool wide = rows <= 16 * SMS;
-    const size_t blocks = std::min<size_t>(wide ? (rows + 1) / 2 : (rows + 7) / 8, SMS * 3), more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
+    const bool wide = tokens * heads <= 16 * SMS;
+    const size_t blocks = std::min<size_t>(tokens * (wide ? (heads + 1) / 2 : (heads + 7) / 8), SMS * 3), more = a.weights ? (size_t)chunks * a.batch * a.kv_heads : 0;
     g_launches++;
     return launch_pdl(wide ? shared_merge_kernel<BF, HD, 4> : shared_merge_kernel<BF, HD, 1>, dim3((uint32_t)(blocks + more)), dim3(256), 0, st, a, (uint32_t)more,
                       std::max(1u, chunks)) == cudaSuccess;
@@ -601,6 +604,9 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     }
     a.t_slices = std::max(1u, std::max(6u, 24 / l.t_rt) * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
+    *why = "attn shared: 2^31 partial results at most";
+    if (parts >= (1ull << 31)) return false;
+    a.by_rep = Div(a.rep); a.by_q_len = Div(a.q_len); a.by_p_tokens = Div(a.p_tokens);
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     l.ml = up((size_t)(a.batch + 3) * 4);
     l.o = l.ml + up(parts * 8);
