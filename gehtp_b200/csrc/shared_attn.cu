@@ -602,7 +602,9 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
         a.p_len = (tiles + best - 1) / best * unit;
         a.p_slices = (a.n_prefix + a.p_len - 1) / a.p_len;
     }
-    a.t_slices = std::max(1u, std::max(6u, 24 / l.t_rt) * SMS / a.kv_heads);
+    // slices: three to a group of warps that one row tile makes, one or two where more do (32 sequences with weights: 24 an SM 85 us, 12 90;
+    // 64 sequences x 8 tokens: 6 an SM 165 us, 12 170)
+    a.t_slices = std::max(1u, (l.t_rt == 1 ? 24 : std::max(3u, 12 / l.t_rt)) * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
     *why = "attn shared: 2^31 partial results at most";
     if (parts >= (1ull << 31)) return false;
