@@ -236,11 +236,6 @@ const char* evict_refuses(uint32_t batch, uint32_t kv_heads, uint32_t hd, uint32
     return nullptr;
 }
 
-bool apart(const void* a, const void* b, size_t bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x + bytes <= y || y + bytes <= x;
-}
-
 }  // namespace
 
 bool k_kv_evict(cudaStream_t st, const EvictArgs& a) {
@@ -294,9 +289,9 @@ extern "C" int gehtp_kv_evict(const void* ring_dev, void* ring_out_dev, const fl
         return fail("kv evict: weights, counts and kept lie on 4-byte boundaries");
     if ((uintptr_t)workspace_dev & 255u) return fail("kv evict: the workspace lies on a 256-byte boundary");
     const size_t heads = (size_t)batch * kv_heads, need = gehtp_kv_evict_workspace(batch, kv_heads, head_dim, nslots, keep, sinks, recent);
-    if (ring_dev != ring_out_dev && !apart(ring_dev, ring_out_dev, heads * nslots * head_dim * 4)) return fail("kv evict: ring and ring_out overlap");
-    if (weights_dev != weights_out_dev && !apart(weights_dev, weights_out_dev, heads * nslots * 4)) return fail("kv evict: weights and weights_out overlap");
-    if (n_dev != n_out_dev && !apart(n_dev, n_out_dev, (size_t)batch * 4)) return fail("kv evict: n and n_out overlap");
+    if (ring_dev != ring_out_dev && !apart(ring_dev, heads * nslots * head_dim * 4, ring_out_dev, heads * nslots * head_dim * 4)) return fail("kv evict: ring and ring_out overlap");
+    if (weights_dev != weights_out_dev && !apart(weights_dev, heads * nslots * 4, weights_out_dev, heads * nslots * 4)) return fail("kv evict: weights and weights_out overlap");
+    if (n_dev != n_out_dev && !apart(n_dev, (size_t)batch * 4, n_out_dev, (size_t)batch * 4)) return fail("kv evict: n and n_out overlap");
     if (workspace_bytes < need) {
         char m[128];
         std::snprintf(m, sizeof m, "kv evict: needs %zu bytes of workspace, got %zu", need, workspace_bytes);

@@ -45,6 +45,10 @@ bool k_shared_prefix_sm100(cudaStream_t st, const SharedArgs& a, uint32_t hd, bo
 bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16, uint32_t row_tiles, bool prefix, bool tails, bool beside);
 bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16);
 
+inline bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return !a || !b || x + a_bytes <= y || y + b_bytes <= x;
+}
 // true: `p` is memory of the current device (or managed); else g.last_error says which argument is not
 bool on_this_device(const void* p, const char* what);
 

@@ -673,6 +673,8 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
         return fail("attn shared: q, prefix, tail and out lie on 16-byte boundaries");
     if ((uintptr_t)workspace_dev & 255u) return fail("attn shared: the workspace lies on a 256-byte boundary");
     if ((((uintptr_t)n_tail_dev) | ((uintptr_t)weights_in_dev) | ((uintptr_t)weights_dev)) & 3u) return fail("attn shared: n_tail and weights lie on 4-byte boundaries");
+    const size_t w_bytes = (size_t)batch * kv_heads * nslots * 4;
+    if (weights_in_dev && weights_in_dev != weights_dev && !apart(weights_in_dev, w_bytes, weights_dev, w_bytes)) return fail("attn shared: weights_in and weights overlap");
     if (workspace_bytes < l.total) {
         char m[128];
         std::snprintf(m, sizeof m, "attn shared: needs %zu bytes of workspace, got %zu", l.total, workspace_bytes);

@@ -612,6 +612,12 @@ extern "C" int gehtp_verify_drafts(const void* target_dev, const void* draft_dev
     if ((((uintptr_t)target_dev) | ((uintptr_t)draft)) & el) return fail("verify drafts: logits lie on boundaries of their type");
     if ((((uintptr_t)tokens_dev) | ((uintptr_t)n_drafts_dev) | ((uintptr_t)uniforms_dev) | ((uintptr_t)accepted_dev) | ((uintptr_t)out_dev)) & 3u)
         return fail("verify drafts: tokens, counts, uniforms and outputs lie on 4-byte boundaries");
+    // a sequence's outputs are written while other CTAs read its inputs
+    const size_t each = (size_t)batch * 4, all = each * n_drafts;
+    for (const void* in : {(const void*)tokens_dev, (const void*)n_drafts_dev, (const void*)uniforms_dev}) {
+        const size_t bytes = in == n_drafts_dev ? each : in == tokens_dev ? all : all + each;
+        if (!apart(in, bytes, accepted_dev, each) || !apart(in, bytes, out_dev, all + each)) return fail("verify drafts: an output overlaps an input");
+    }
     if ((uintptr_t)workspace_dev & 255u) return fail("verify drafts: the workspace lies on a 256-byte boundary");
     const Layout l = lay_out(batch, n_drafts, vocab);
     if (workspace_bytes < l.total) {

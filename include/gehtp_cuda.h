@@ -408,7 +408,7 @@ int gehtp_kv_evict(const void* ring_dev, void* ring_out_dev, const float* weight
  *   uniforms fp32 [batch][n_drafts + 1] in [0, 1): one for each draft, the last for the draw, whatever the number of drafts
  *   accepted int32 [batch]; out int32 [batch][n_drafts + 1]: the accepted drafts, the token behind them, -1 in the rest
  * A target row without a distribution (a logit that is no number or +inf, -inf throughout) accepts nothing and yields the token -1; a
- * draft row without one is not accepted and takes nothing away from p. Logits of type `dtype`; -inf stands for a token that is ruled out.
+ * draft row without one is not accepted and takes nothing away from p. Outputs overlap no input. Logits of type `dtype`; -inf stands for a token that is ruled out.
  * n_drafts 0 (no tokens, no draft) draws a token per sequence. Up to 64 drafts and 4096 sequences; temperature 0 or 1e-4 to 1e4. */
 size_t gehtp_verify_drafts_workspace(uint32_t batch, uint32_t n_drafts, uint32_t vocab);
 int gehtp_verify_drafts(const void* target_dev, const void* draft_dev, const int32_t* tokens_dev, const int32_t* n_drafts_dev,

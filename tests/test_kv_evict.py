@@ -93,6 +93,59 @@ def test_again_and_again(cuda):
         call.ring, call.w, call.n = (x.cpu().numpy() for x in (call.d_ring, call.d_w, call.d_n))
 
 
+@pytest.mark.gpu
+def test_captured_replayed_and_on_two_streams(cuda):
+    import torch
+    calls = [Call(5, 4, 128, 700, [700, 300, 650, 0, 699], 512, 4, 100, seed=1), Call(3, 2, 64, 90, [90, 89, 20], 40, 0, 8, weights=few, seed=2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graph = torch.cuda.CUDAGraph()
+
+    def queue(call, stream):
+        assert cuda.gehtp_kv_evict(call.d_ring.data_ptr(), call.o_ring.data_ptr(), call.d_w.data_ptr(), call.o_w.data_ptr(), call.d_n.data_ptr(), call.o_n.data_ptr(),
+                                   call.kept.data_ptr(), *call.shape, call.ws.data_ptr(), call.ws.numel(), stream.cuda_stream) == 0
+    for call in calls:
+        call.ws = torch.empty(cuda.gehtp_kv_evict_workspace(*call.shape), dtype=torch.uint8, device="cuda")
+        call.o_ring, call.o_w, call.o_n = torch.full_like(call.d_ring, 77), torch.full_like(call.d_w, 9.0), torch.full_like(call.d_n, -1)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for call, stream in zip(calls, streams):
+            queue(call, stream)
+    torch.cuda.synchronize()
+    for call in calls:
+        call.check(False)
+    a, b = calls[0], Call(5, 4, 128, 700, [1, 700, 513, 512, 600], 512, 4, 100, seed=9)
+    with torch.cuda.graph(graph, stream=streams[0]):
+        queue(a, streams[0])
+    for x, y in ((a.d_ring, b.d_ring), (a.d_w, b.d_w), (a.d_n, b.d_n)):
+        x.copy_(y)
+    a.o_ring.fill_(77), a.o_w.fill_(9.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    a.ring, a.w, a.n = b.ring, b.w, b.n
+    a.check(False)
+
+
+@pytest.mark.gpu
+def test_caches_past_four_gigabytes(cuda):
+    """The last rows of a cache that is 4.3 GB long, in place and to another."""
+    import torch
+    batch, kvh, d, slots, keep = 64, 8, 128, 16500, 3
+    ring = torch.zeros(slots, 2, batch * kvh, d, dtype=torch.int16, device="cuda")
+    assert ring.numel() * 2 > 1 << 32
+    ring[-2:] = torch.randint(-30000, 30000, ring[-2:].shape, dtype=torch.int16, device="cuda")
+    want = ring[-2:].clone()
+    w = torch.zeros(batch, kvh, slots, device="cuda")
+    n = torch.full((batch,), slots, dtype=torch.int32, device="cuda")
+    ws = torch.empty(cuda.gehtp_kv_evict_workspace(batch, kvh, d, slots, keep, 0, 2), dtype=torch.uint8, device="cuda")
+    for out_n in (torch.zeros_like(n), n):
+        out_ring = torch.zeros(slots, 2, batch * kvh, d, dtype=torch.int16, device="cuda") if out_n is not n else ring
+        assert cuda.gehtp_kv_evict(ring.data_ptr(), out_ring.data_ptr(), w.data_ptr(), w.data_ptr(), n.data_ptr(), out_n.data_ptr(), None, batch, kvh, d, slots, keep, 0, 2,
+                                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert (out_n == keep).all() and torch.equal(out_ring[1:3], want) and (out_ring[0] == 0).all()
+        del out_ring
+
+
 def test_workspace_refuses_what_the_call_refuses(cuda):
     ws = cuda.gehtp_kv_evict_workspace
     assert ws(2, 8, 128, 640, 512, 4, 64) >= 2 * 8 * 512 * 4

@@ -136,6 +136,12 @@ CASES = [
     (70, 5, 6, 2, 64, 127, 9, [i % 10 for i in range(70)]),
     (4, 1, 32, 8, 128, 2049, 3000, [3000, 1, 64, 1777]),
     (9, 8, 12, 4, 128, 513, 100, [-3, 1000, 8, 7, 9, 100, 64, 72, 71]),      # lengths outside the cache count as its ends
+    (3, 2, 8, 2, 128, 0, 0, [0, 0, 0]),                     # nothing to see at all
+    (20, 1, 16, 4, 128, 700, 0, [0] * 20),                  # no tails
+    (33, 1, 16, 2, 128, 5000, 70, [i % 71 for i in range(33)]),              # two row tiles and a part of a third
+    (12, 3, 28, 4, 64, 3000, 40, [(7 * i) % 41 for i in range(12)]),         # 18 tokens of seven heads to a row tile
+    (4, 12, 10, 1, 128, 257, 150, [150, 13, 12, 11]),       # 120 rows to a tail
+    (16, 1, 8, 1, 128, 513, 33, [33 - i for i in range(16)]),                # 128 rows that meet few positions: with the tails
     (130, 1, 2, 2, 64, 40, 300, [300 if i == 77 else 2 for i in range(130)]),
 ]
 
@@ -228,7 +234,7 @@ def test_workspace_refuses_what_the_call_refuses(cuda):
 
 @pytest.mark.parametrize("change,message", [
     (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(ws=None), b"null"), (dict(prefix=None), b"null"), (dict(tail=None), b"null"),
-    (dict(n_tail=None), b"null"), (dict(w=None), b"weights_in"), (dict(q=8), b"16-byte"), (dict(tail=8), b"16-byte"), (dict(ws=64), b"256-byte"),
+    (dict(n_tail=None), b"null"), (dict(w=None), b"weights_in"), (dict(w=64), b"overlap"), (dict(q=8), b"16-byte"), (dict(tail=8), b"16-byte"), (dict(ws=64), b"256-byte"),
     (dict(n_tail=2), b"4-byte"), (dict(stride=1024), b"q_stride"), (dict(stride=2052), b"q_stride"), (dict(dt=DT_F32), b"element type"),
     (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"),
     (dict(size=1000), b"workspace"), (dict(heads=24, kv=16), b"shape"), (dict(), b"no memory of the current device"),
@@ -242,3 +248,65 @@ def test_refusals(cuda, change, message):
     rc = cuda.gehtp_attn_shared(at("q"), at("prefix"), at("tail"), at("n_tail"), base, at("w"), at("out"), 2, 1, heads, kv, 128, change.get("stride", 2048), 512, 64,
                                 change.get("dt", DT_F16), change.get("scale", 0.1), at("ws"), change.get("size", 1 << 40), None)
     assert rc == -1 and message in cuda.gehtp_cuda_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("batch,prefix", [(2, 700), (40, 3000), (140, 2000)])
+@pytest.mark.parametrize("order", [1, -1])
+def test_scores_that_outgrow_earlier_tiles(cuda, dtype, batch, prefix, order):
+    """Keys that grow along the cache, or shrink: references raised behind a tile, within one, and never."""
+    import torch
+    call = Call(batch, 1, 8, 2, 128, prefix, 150, [(11 * i) % 151 for i in range(batch)], getattr(torch, dtype), weights=True, seed=batch)
+    grow = torch.exp(order * torch.linspace(-2.25, 2.25, prefix + 150) + 0.25)
+    call.prefix[:, 0] *= grow[:prefix, None, None].to(call.prefix)
+    call.tail[:, 0] *= grow[prefix:, None, None].to(call.tail)
+    call.run(cuda)
+    call.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 30, 60])
+def test_prefix_position_that_is_no_number(cuda, batch):
+    """All rows see the prefix: a key that is no number makes none of the rows of its head, an infinite value none of its component."""
+    import torch
+    call = Call(batch, 1, 8, 2, 128, 4000, 20, [i % 21 for i in range(batch)], torch.float16, seed=batch)
+    want, _, _, tol = call.expected()
+    call.prefix[1234, 0, 0] = float("nan")
+    call.prefix[3999, 1, 1, 7] = float("inf")
+    call.run(cuda)
+    torch.cuda.synchronize()
+    out = call.out.cpu().double()
+    assert not torch.isfinite(out[:, :, :4]).any() and not torch.isfinite(out[:, :, 4:, 7]).any()
+    rest = [i for i in range(128) if i != 7]
+    assert ((out - want).abs() <= tol)[:, :, 4:, rest].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [2, 24])
+def test_caches_past_four_gigabytes(cuda, batch):
+    """One key far behind the 2^32nd byte of the prefix, one of the tails, against zeros everywhere else."""
+    import torch
+    heads, kvh, d, prefix, slots = 16, 8, 128, (1 << 20) + 4097, (1 << 32) // (batch * 8 * 128 * 4) + 300
+    q = torch.randn(batch, 1, heads, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    pre, tail = torch.zeros(prefix, 2, kvh, d, dtype=torch.bfloat16, device="cuda"), torch.zeros(slots, 2, batch * kvh, d, dtype=torch.bfloat16, device="cuda")
+    n = torch.full((batch,), slots - 3, dtype=torch.int32, device="cuda")
+    assert pre.numel() * 2 > 1 << 32 and tail.numel() * 2 > 1 << 32
+    pre[prefix - 5, 0], pre[prefix - 5, 1] = 6.0, 3.0             # a key that queries meet by the sum of their components
+    tail[slots - 4, 0], tail[slots - 4, 1] = -6.0, -5.0
+    tail[slots - 3:] = float("nan")
+    dots = q.cpu().double().sum(-1)[:, 0] * 6.0 * 0.125
+    top = dots.abs()
+    a, b, rest = torch.exp(dots - top), torch.exp(-dots - top), torch.exp(-top) * (prefix + slots - 3 - 2)
+    want = (3.0 * a - 5.0 * b) / (a + b + rest)
+    out = torch.zeros(batch, 1, heads, d, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(cuda.gehtp_attn_shared_workspace(batch, 1, heads, kvh, d, prefix, slots, 0), dtype=torch.uint8, device="cuda")
+    rc = cuda.gehtp_attn_shared(q.data_ptr(), pre.data_ptr(), tail.data_ptr(), n.data_ptr(), None, None, out.data_ptr(), batch, 1, heads, kvh, d, heads * d, prefix, slots,
+                                DT_BF16, 0.125, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, cuda.gehtp_cuda_last_error()
+    torch.cuda.synchronize()
+    got = out.cpu().double()[:, 0]
+    # the scores as in `tolerance`, of one dot product; weights of the others are sums of a million equal terms, each sum 2^-24 a term off
+    err = 2.0 ** -8 * want.abs() + (3 * a + 5 * b) / (a + b + rest) * (2.0 ** -16 + 2 * top * 130 * 2.0 ** -23 + 2.0 ** -19 + 2.0 ** -8)
+    assert ((got - want[..., None]).abs() <= err[..., None] + 1e-30).all()
+    assert cuda.gehtp_attn_shared_status() == 0

@@ -109,6 +109,8 @@ CASES = [
     (9, 4, 1000, "float32", 0.8, True, (0, 0), 0), (9, 4, 1001, "float32", 0.8, True, (0, 3), 1), (9, 3, 1003, "bfloat16", 1.0, True, (2, 0), 5),
     (20, 5, 4099, "float16", 1.3, True, (0, 0), 1), (33, 0, 777, "float32", 1.0, False, (0, 0), 0), (12, 6, 5000, "float32", 0.6, False, (0, 0), 2),
     (2, 8, 70001, "bfloat16", 1.0, True, (0, 0), 0), (2, 2, 151936, "float16", 0.8, True, (64, 0), 0), (5, 64, 300, "float32", 1.0, True, (0, 0), 0),
+    (33, 5, 3001, "float32", 0.0, False, (0, 0), 3), (2, 20, 30000, "bfloat16", 0.0, False, (0, 0), 1), (700, 2, 90, "float16", 0.0, False, (0, 0), 1),
+    (700, 2, 90, "float32", 0.9, True, (0, 0), 1),
     (9, 4, 1001, "float32", 0.0, False, (0, 0), 1), (3, 8, 40000, "bfloat16", 0.0, False, (0, 0), 0), (4, 3, 20011, "float16", 0.0, True, (5, 0), 0),
 ]
 
@@ -192,13 +194,58 @@ def test_workspace_refuses_what_the_call_refuses(cuda):
     (dict(target=None), b"null"), (dict(tokens=None), b"null"), (dict(uniforms=None), b"null"), (dict(accepted=None), b"null"), (dict(out=None), b"null"),
     (dict(ws=None), b"null"), (dict(target=2), b"boundaries of their type"), (dict(draft=2), b"boundaries of their type"), (dict(out=2), b"4-byte"),
     (dict(ws=64), b"256-byte"), (dict(ts=999), b"rows"), (dict(ds=999), b"rows"), (dict(dt=3), b"element type"), (dict(heat=-1.0), b"temperature"),
-    (dict(heat=1e-9), b"temperature"), (dict(heat=float("nan")), b"temperature"), (dict(heat=float("inf")), b"temperature"), (dict(size=8), b"workspace"),
+    (dict(heat=1e-9), b"temperature"), (dict(heat=float("nan")), b"temperature"), (dict(heat=float("inf")), b"temperature"), (dict(size=8), b"workspace"), (dict(accepted=-192), b"overlaps"), (dict(out=-516), b"overlaps"), (dict(out=-340), b"overlaps"),
     (dict(), b"no memory of the current device"),
 ])
 def test_refusals(cuda, change, message):
     buf = np.zeros(1 << 16, np.uint8)
     base = (buf.ctypes.data + 255) // 256 * 256
-    at = lambda k: None if k in change and change[k] is None else base + change.get(k, 0)
+    place = dict(target=0, draft=0, tokens=0, n=64, uniforms=128, accepted=256, out=512, ws=1024)
+    at = lambda k: None if k in change and change[k] is None else base + change.get(k, 0) + place[k]
     rc = cuda.gehtp_verify_drafts(at("target"), at("draft"), at("tokens"), at("n"), at("uniforms"), at("accepted"), at("out"), 4, 3, 1000, change.get("ts", 1000),
                                   change.get("ds", 1000), change.get("dt", DT_F32), change.get("heat", 1.0), at("ws"), change.get("size", 1 << 30), None)
     assert rc == -1 and message in cuda.gehtp_cuda_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,noise", [("float32", 3e-5), ("float32", 1e-3), ("float16", 0.0), ("float32", 0.0)])
+def test_rows_that_are_nearly_alike(cuda, dtype, noise):
+    """A token outside the vocabulary is refused, and the draw is from the little that p is above q: where that is a hundredth of a percent, its
+    sum's 2^-45 of p are 2^-31 of it. Equal rows: from p."""
+    import torch
+    for seed in range(20):
+        target, draft, tokens, uniforms = make(12, 2, 3001, dtype, 0.9, True, 7 + seed, noise=noise)
+        tokens[:, 0] = -1
+        accepted, out, near, border = by_rule(target, draft, tokens, None, uniforms, 3001, 0.9)
+        if border > 2.0 ** -26:
+            break
+    got = verify(cuda, target, draft, tokens, None, uniforms, 3001, 0.9)
+    assert border > 2.0 ** -26 and np.array_equal(got[0], accepted) and np.array_equal(got[1], out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heat", [0.0, 0.8])
+def test_captured_and_replayed(cuda, heat):
+    """Logits, tokens, counts and random numbers are those of the replay."""
+    import torch
+    batch, n, vocab = 6, 4, 5003
+    t, d, tok, u = (x.cuda() for x in make(batch, n, vocab, "bfloat16", heat, True, 1))
+    cnt = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    accepted, out = torch.zeros(batch, dtype=torch.int32, device="cuda"), torch.zeros(batch, n + 1, dtype=torch.int32, device="cuda")
+    ws = torch.full((cuda.gehtp_verify_drafts_workspace(batch, n, vocab),), 255, dtype=torch.uint8, device="cuda")
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        assert cuda.gehtp_verify_drafts(t.data_ptr(), d.data_ptr(), tok.data_ptr(), cnt.data_ptr(), u.data_ptr(), accepted.data_ptr(), out.data_ptr(), batch, n, vocab, vocab,
+                                        vocab, DT_BF16, heat, ws.data_ptr(), ws.numel(), stream.cuda_stream) == 0
+    for seed in range(2, 40):
+        t2, d2, tok2, u2 = make(batch, n, vocab, "bfloat16", heat, True, seed, noise=0.4)
+        cnt2 = torch.tensor([(seed + b) % (n + 1) for b in range(batch)], dtype=torch.int32)
+        want, rows, near, border = by_rule(t2, d2, tok2, cnt2, u2, vocab, heat)
+        if near <= 2.0 ** -18 or border <= 1e-11:
+            continue
+        for x, y in ((t, t2), (d, d2), (tok, tok2), (cnt, cnt2), (u, u2)):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(accepted.cpu().numpy(), want) and np.array_equal(out.cpu().numpy(), rows)
