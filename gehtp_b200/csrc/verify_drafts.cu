@@ -82,25 +82,23 @@ __device__ __forceinline__ void load_logits(const typename E::T* row, int64_t e,
 template <class E>
 __device__ __forceinline__ int lead(const typename E::T* row) { return (int)(((uintptr_t)row & 15u) / sizeof(typename E::T)); }
 
-// 2^((x - m) k) in 64 bits: x k - m k split into a whole number and at most a half, 2^that by the interpolation of degree 9 at the Chebyshev
-// points of [-1/2, 1/2] (within 2^-45). 0 below 2^-1000 and for -inf.
+// 2^((x - m) k) in 64 bits: x k - m k split into 32nds and at most half a 32nd; 2^that by a table of the 32 and the interpolation of degree 4 at
+// the Chebyshev points of [-1/64, 1/64] (within 2^-43): nine 64-bit operations, of which 64 a cycle and SM run, where degree 9 over
+// [-1/2, 1/2] takes thirteen. 0 below 2^-1000 and for -inf.
 struct Power64 {
+    const double* table;                                      // 2^(j / 32)
     double k, mk;
     float floor;
-    __device__ __forceinline__ Power64(double k_, float m) : k(k_), mk(-(double)m * k_), floor((float)((double)m - 1000.0 / k_)) {}
+    __device__ __forceinline__ Power64(const double* table_, double k_, float m) : table(table_), k(k_), mk(-(double)m * k_), floor((float)((double)m - 1000.0 / k_)) {}
     __device__ __forceinline__ double operator()(float x) const {
-        const double t = fma((double)fmaxf(x, floor), k, mk), magic = 6755399441055744.0, n = t + magic, f = t - (n - magic);
-        double v = 1.0205905413765595e-07;
-        v = fma(v, f, 1.325964524488711e-06);
-        v = fma(v, f, 1.5252672924850737e-05);
-        v = fma(v, f, 0.0001540343375125101);
-        v = fma(v, f, 0.0013333558200794592);
-        v = fma(v, f, 0.009618129193934313);
-        v = fma(v, f, 0.05550410866465167);
-        v = fma(v, f, 0.2402265069564034);
-        v = fma(v, f, 0.6931471805599462);
-        v = fma(v, f, 1.0000000000000135);
-        const double e = __hiloint2double(__double2hiint(v) + (__double2loint(n) << 20), __double2loint(v));
+        const double t = fma((double)fmaxf(x, floor), k, mk), magic = 211106232532992.0 /* 1.5 * 2^47 */, n = t + magic, f = t - (n - magic);
+        const int i = __double2loint(n);                      // t in 32nds
+        double v = 0.009618176115571158;
+        v = fma(v, f, 0.055504515573860415);
+        v = fma(v, f, 0.24022650695623157);
+        v = fma(v, f, 0.6931471805351095);
+        v = fma(v, f, 1.0) * table[i & 31];
+        const double e = __hiloint2double(__double2hiint(v) + ((i >> 5) << 20), __double2loint(v));
         return x >= floor ? e : 0.0;
     }
 };
@@ -269,6 +267,7 @@ struct DrawShared {
     BlockScan scan;
     int first, last, is_last;
     double front;
+    double table[32];                                         // of Power64
 };
 
 // The lowest place of `hit` (a place or INT_MAX) over the CTA, and the sum in front of it.
@@ -288,7 +287,7 @@ __device__ __forceinline__ void draw(const VerifyArgs& A, uint32_t b, const type
                                      DrawShared& S, int32_t* to_) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stretches = A.splits * WARPS;
     const int64_t vocab = A.vocab, p_lead = lead<E>(p), vecs = (vocab + p_lead + E::V - 1) / E::V;
-    const Power64 ep(k, rp.x), eq(k, rq.x);
+    const Power64 ep(S.table, k, rp.x), eq(S.table, k, rq.x);
     const double c0 = q ? (double)(rp.y / rq.y) : 0.0;
     {
         const int64_t mine = blockIdx.x * WARPS + warp, from = vecs * mine / stretches, to = vecs * (mine + 1) / stretches;
@@ -444,6 +443,7 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
     pdl_wait();
     pdl_release();
     const uint32_t nd = drafts_of(A, b);
+    if (!GREEDY && threadIdx.x < 32) shared.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
     const typename E::T *target = (const typename E::T*)A.target + (size_t)b * (A.n + 1) * A.t_stride, *draft = (const typename E::T*)A.draft + (size_t)b * A.n * A.d_stride;
     const double k = A.inv * 1.4426950408889634;
     const float2 *t_part = A.part + (size_t)b * (A.n + 1) * A.pieces, *d_part = A.part + ((size_t)A.batch * (A.n + 1) + (size_t)b * A.n) * A.pieces;

@@ -211,7 +211,7 @@ def test_refusals(cuda, change, message):
 @pytest.mark.parametrize("dtype,noise", [("float32", 3e-5), ("float32", 1e-3), ("float16", 0.0), ("float32", 0.0)])
 def test_rows_that_are_nearly_alike(cuda, dtype, noise):
     """A token outside the vocabulary is refused, and the draw is from the little that p is above q: where that is a hundredth of a percent, its
-    sum's 2^-45 of p are 2^-31 of it. Equal rows: from p."""
+    sum's 2^-43 of p are 2^-29 of it. Equal rows: from p."""
     import torch
     for seed in range(20):
         target, draft, tokens, uniforms = make(12, 2, 3001, dtype, 0.9, True, 7 + seed, noise=noise)
