@@ -393,7 +393,7 @@ constexpr uint32_t W_CHUNK = 1024;
 
 // The first `weight_blocks` CTAs: 1024 tail positions of a (sequence, key head) each. The others stay and walk the rows of the result, WR warps
 // to one, with eight partial results on their way at a time and maxima and sums beside them. What a call's end takes is
-// latencies one behind the other: 2048 rows of 18 slices and their tails took 20 us by a warp each that read the maxima first, @@
+// latencies one behind the other: 2048 rows of 18 slices and their tails took 20 us by a warp each that read the maxima first, 10
 // this way.
 template <bool BF, int HD, int WR>
 __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A, uint32_t weight_blocks, uint32_t chunks) {
