@@ -29,7 +29,7 @@ struct SharedArgs {
     size_t q_stride;
     uint32_t p_tokens, p_tiles, p_slices, p_len;   // prefix: slices of p_len positions
     uint32_t t_slices;                             // the tails of all sequences are cut into about so many slices
-    Div by_rep, by_q_len, by_p_tokens;             // of heads below 65536 by up to 128, of tokens below 16384 by up to 16 and 128
+    Div by_rep, by_q_len, by_p_tokens;             // of heads below 2^23 by up to 128, of tokens below 2^14 by up to 16 and 128
     float sc;                                      // log2(e) * scale
     float* part_o;                                 // [partial row][head_dim], the prefix's first
     float2* part_ml;                               // [partial row] {m, sum}

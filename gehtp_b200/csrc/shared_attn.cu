@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
     // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
     if (!beside) pdl_wait();
     pdl_release();
-    // A CTA that comes up when all items have been handed out has nothing left to work out: the first one left their number.
-    if (beside) {
+    // A CTA that comes up when all items have been handed out has nothing left to work out: an earlier one left their number. The first
+    // goes on all the same, since it writes the plan.
+    if (beside && blockIdx.x) {
         if (threadIdx.x == 0) {
             const uint32_t all = *(volatile uint32_t*)(A.next + 1), out = *(volatile uint32_t*)A.next;
             s_k = all && out >= all - 1;
@@ -574,8 +575,8 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     *why = "attn shared: head_dim is 64 or 128";
     if (hd != 64 && hd != 128) return false;
     a.rep = n_heads / a.kv_heads;
-    *why = "attn shared: up to 1024 sequences, 16 new tokens and 128 rows (q_len * n_heads / kv_heads) to a key head, 65536 (sequence, key head) pairs";
-    if (a.batch > MAX_BATCH || a.q_len > MAX_Q || (size_t)a.q_len * a.rep > MAX_ROWS || (size_t)a.batch * a.kv_heads > 65536) return false;
+    *why = "attn shared: up to 1024 sequences, 16 new tokens and 128 rows (q_len * n_heads / kv_heads) to a key head, 65535 (sequence, key head) pairs";
+    if (a.batch > MAX_BATCH || a.q_len > MAX_Q || (size_t)a.q_len * a.rep > MAX_ROWS || (size_t)a.batch * a.kv_heads > 65535) return false;
     *why = "attn shared: up to 2^30 prefix positions and 2^24 slots";
     if (a.n_prefix > (1u << 30) || a.nslots > (1u << 24)) return false;
     *why = "attn shared: weights of tails that have no slots";

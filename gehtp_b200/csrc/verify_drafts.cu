@@ -67,12 +67,13 @@ __device__ __forceinline__ void unpack_logits(const uint4& v, float (&x)[E::V]) 
         for (int i = 0; i < 4; i++) { x[2 * i] = E::f((typename E::T)(w[i] & 0xffffu)); x[2 * i + 1] = E::f((typename E::T)(w[i] >> 16)); }
     }
 }
+// (ordinary loads: a read-only one could be moved ahead of the wait for the kernel that writes the logits)
 // V logits from place e on: in one load where they lie in the row and on a boundary; places outside the row are -inf
 template <class E>
 __device__ __forceinline__ void load_logits(const typename E::T* row, int64_t e, int64_t end, float (&x)[E::V]) {
     const typename E::T* p = row + e;
     if (e >= 0 && e + E::V <= end && ((uintptr_t)p & 15u) == 0) {
-        unpack_logits<E>(__ldg((const uint4*)p), x);
+        unpack_logits<E>(__ldcg((const uint4*)p), x);
     } else {
 #pragma unroll
         for (int i = 0; i < E::V; i++) x[i] = e + i >= 0 && e + i < end ? E::f(p[i]) : -INFINITY;
@@ -179,7 +180,7 @@ __device__ __forceinline__ float2 part_of_row(const typename E::T* p, int64_t fi
         uint4 w[AHEAD];
         float x[AHEAD * E::V];
 #pragma unroll
-        for (int u2 = 0; u2 < AHEAD; u2++) w[u2] = __ldg((const uint4*)(p + e + u2 * STEP));
+        for (int u2 = 0; u2 < AHEAD; u2++) w[u2] = __ldcg((const uint4*)(p + e + u2 * STEP));
 #pragma unroll
         for (int u2 = 0; u2 < AHEAD; u2++) {
             float y[E::V];

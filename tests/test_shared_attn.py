@@ -142,6 +142,7 @@ CASES = [
     (12, 3, 28, 4, 64, 3000, 40, [(7 * i) % 41 for i in range(12)]),         # 18 tokens of seven heads to a row tile
     (4, 12, 10, 1, 128, 257, 150, [150, 13, 12, 11]),       # 120 rows to a tail
     (16, 1, 8, 1, 128, 513, 33, [33 - i for i in range(16)]),                # 128 rows that meet few positions: with the tails
+    (1024, 1, 1, 1, 64, 5, 3, [i % 4 for i in range(1024)]),                 # the most sequences
     (130, 1, 2, 2, 64, 40, 300, [300 if i == 77 else 2 for i in range(130)]),
 ]
 
@@ -228,7 +229,7 @@ def test_workspace_refuses_what_the_call_refuses(cuda):
     assert ws(2, 1, 16, 8, 128, 512, 64, 1) > ws(2, 1, 16, 8, 128, 512, 64, 0) > 0
     for bad in ((0, 1, 16, 8, 128, 512, 64, 0), (2, 0, 16, 8, 128, 512, 64, 0), (2, 1, 15, 8, 128, 512, 64, 0), (2, 1, 16, 0, 128, 512, 64, 0),
                 (2, 1, 16, 8, 96, 512, 64, 0), (1025, 1, 16, 8, 128, 512, 64, 0), (2, 17, 16, 8, 128, 512, 64, 0), (2, 16, 9, 1, 128, 512, 64, 0),
-                (2, 1, 16, 8, 128, 512, 0, 1), (2, 1, 16, 8, 128, (1 << 30) + 1, 64, 0), (2, 1, 16, 8, 128, 0, (1 << 24) + 1, 0), (1024, 1, 65, 65, 64, 1, 0, 0)):
+                (2, 1, 16, 8, 128, 512, 0, 1), (2, 1, 16, 8, 128, (1 << 30) + 1, 64, 0), (2, 1, 16, 8, 128, 0, (1 << 24) + 1, 0), (1024, 1, 64, 64, 64, 1, 0, 0)):
         assert ws(*bad) == 0 and b"attn shared" in cuda.gehtp_cuda_last_error()
 
 
