@@ -237,14 +237,16 @@ __device__ __forceinline__ bool sound(float2 x) { return x.y > 0.0f && isfinite(
 // Sums over the CTA: of all threads, and of those in front of each.
 struct BlockScan {
     double warp[WARPS];
-    __device__ __forceinline__ double sum(double v) {
-        v = warp_sum_d(v);
+    double2 pair[WARPS];
+    __device__ __forceinline__ double2 sums(double2 v) {
+        v.x = warp_sum_d(v.x);
+        v.y = warp_sum_d(v.y);
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) warp[threadIdx.x >> 5] = v;
+        if ((threadIdx.x & 31) == 0) pair[threadIdx.x >> 5] = v;
         __syncthreads();
-        double t = 0.0;
+        double2 t = make_double2(0.0, 0.0);
 #pragma unroll
-        for (int i = 0; i < WARPS; i++) t += warp[i];
+        for (int i = 0; i < WARPS; i++) { t.x += pair[i].x; t.y += pair[i].y; }
         return t;
     }
     __device__ __forceinline__ double before(double v, double* total) {
@@ -341,39 +343,42 @@ __device__ __forceinline__ void draw(const VerifyArgs& A, uint32_t b, const type
     bool less = q != nullptr;                                 // the weights are p - q
     // e_p - c e_q with the product rounded on its own: equal rows leave 0
     auto rest = [&](float x, float y) { return fmax(ep(x) - __dmul_rn(c, eq(y)), 0.0); };
+    double total, front, tp = 0.0;
     if (less) {
-        const double tp = S.scan.sum(v[0].x + v[1].x), tq = S.scan.sum(v[0].y + v[1].y);
-        c = tp / tq;
+        const double2 t = S.scan.sums(make_double2(v[0].x + v[1].x, v[0].y + v[1].y));
+        tp = t.x;
+        c = t.x / t.y;
 #pragma unroll
         for (int i = 0; i < 2; i++) w[i] = fmax(fma(c0 - c, v[i].w, v[i].z), 0.0);
-        if (S.scan.sum(w[0] + w[1]) < 0x1p-10 * tp) {         // p and q nearly alike: once more with the true c
-            __shared__ double again[MAX_SPLITS * WARPS];
-            for (uint32_t at = warp; at < stretches; at += WARPS) {
-                const int64_t from = vecs * at / stretches, to = vecs * (at + 1) / stretches;
-                double r = 0.0;
-                for (int64_t j = from + lane; j < to; j += 32) {
-                    const int64_t e = j * E::V - p_lead;
-                    float x[E::V], y[E::V];
-                    load_logits<E>(p, e, vocab, x);
-                    load_logits<E>(q, e, vocab, y);
+    }
+    front = S.scan.before(w[0] + w[1], &total);
+    if (less && total < 0x1p-10 * tp) {                       // p and q nearly alike: once more with the true c
+        __shared__ double again[MAX_SPLITS * WARPS];
+        for (uint32_t at = warp; at < stretches; at += WARPS) {
+            const int64_t from = vecs * at / stretches, to = vecs * (at + 1) / stretches;
+            double r = 0.0;
+            for (int64_t j = from + lane; j < to; j += 32) {
+                const int64_t e = j * E::V - p_lead;
+                float x[E::V], y[E::V];
+                load_logits<E>(p, e, vocab, x);
+                load_logits<E>(q, e, vocab, y);
 #pragma unroll
-                    for (int i = 0; i < E::V; i++) r += rest(x[i], y[i]);
-                }
-                r = warp_sum_d(r);
-                if (lane == 0) again[at] = r;
+                for (int i = 0; i < E::V; i++) r += rest(x[i], y[i]);
             }
-            __syncthreads();
+            r = warp_sum_d(r);
+            if (lane == 0) again[at] = r;
+        }
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 2; i++) w[i] = threadIdx.x * 2 + i < stretches ? again[threadIdx.x * 2 + i] : 0.0;
-            // below: what the roundings of two sums leave of equal rows
-            if (S.scan.sum(w[0] + w[1]) <= 1e-12 * tp) {
-                less = false;
-                w[0] = v[0].x; w[1] = v[1].x;
-            }
+        for (int i = 0; i < 2; i++) w[i] = threadIdx.x * 2 + i < stretches ? again[threadIdx.x * 2 + i] : 0.0;
+        front = S.scan.before(w[0] + w[1], &total);
+        if (total <= 1e-12 * tp) {                            // what the roundings of two sums leave of equal rows
+            less = false;
+            w[0] = v[0].x; w[1] = v[1].x;
+            front = S.scan.before(w[0] + w[1], &total);
         }
     }
-    double total;
-    const double front = S.scan.before(w[0] + w[1], &total), goal = fmax(u * total, 0.0);
+    const double goal = fmax(u * total, 0.0);
     // the first stretch whose end is above the goal; a draw of 1 and above ends in the last that has a weight
     if (threadIdx.x == 0) S.last = -1;
     __syncthreads();
@@ -439,7 +444,7 @@ template <class E, bool GREEDY>
 __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A) {
     __shared__ DrawShared shared;
     __shared__ uint8_t pass[MAX_DRAFTS];
-    __shared__ float2 s_row[2];
+    __shared__ float2 rows[MAX_DRAFTS + 1][2];                    // {maximum, sum} of target and draft rows
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
     pdl_wait();
     pdl_release();
@@ -448,27 +453,31 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
     const typename E::T *target = (const typename E::T*)A.target + (size_t)b * (A.n + 1) * A.t_stride, *draft = (const typename E::T*)A.draft + (size_t)b * A.n * A.d_stride;
     const double k = A.inv * 1.4426950408889634;
     const float2 *t_part = A.part + (size_t)b * (A.n + 1) * A.pieces, *d_part = A.part + ((size_t)A.batch * (A.n + 1) + (size_t)b * A.n) * A.pieces;
-    // ---- which drafts pass
-    for (uint32_t i = warp; i < nd; i += WARPS) {
-        const int x = A.tokens[(size_t)b * A.n + i];
+    // ---- which drafts pass; the row behind the last one is looked at beside them
+    for (uint32_t i = warp; i <= nd; i += WARPS) {
+        const int x = i < nd ? A.tokens[(size_t)b * A.n + i] : -1;
         const bool in = x >= 0 && (uint32_t)x < A.vocab;
         const double lp = !GREEDY && in ? (double)E::f(target[i * A.t_stride + x]) : 0.0, lq = !GREEDY && in && A.draft ? (double)E::f(draft[i * A.d_stride + x]) : 0.0;
         const float2 p = whole_row<GREEDY>(t_part + (size_t)i * A.pieces, A.pieces, (float)k);
-        bool ok;
+        float2 q = make_float2(NAN, NAN);
+        bool ok = i < nd;
         if (GREEDY) {
-            ok = isfinite(p.x) && x == __float_as_int(p.y);
-        } else {
+            ok = ok && isfinite(p.x) && x == __float_as_int(p.y);
+        } else if (ok) {
             double px = 0.0, qx = 1.0;
             ok = sound(p);
             if (ok && in) px = exp2((lp - p.x) * k) / p.y;
             if (A.draft) {
-                const float2 q = whole_row<false>(d_part + (size_t)i * A.pieces, A.pieces, (float)k);
+                q = whole_row<false>(d_part + (size_t)i * A.pieces, A.pieces, (float)k);
                 ok = ok && sound(q);
                 qx = ok && in ? exp2((lq - q.x) * k) / q.y : 0.0;
             }
             ok = ok && (double)A.uniforms[(size_t)b * (A.n + 1) + i] * qx < px;
         }
-        if (lane == 0) pass[i] = ok;
+        if (lane == 0) {
+            if (i < nd) pass[i] = ok;
+            rows[i][0] = p; rows[i][1] = q;
+        }
     }
     __syncthreads();
     uint32_t a = 0;
@@ -477,23 +486,17 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
     int32_t* token = A.out + (size_t)b * (A.n + 1) + a;
     if (blockIdx.x == 0) write_accepted(A, b, a);
     // ---- the row behind the accepted ones
-    if (warp < 2) {
-        float2 x = make_float2(NAN, NAN);
-        if (warp == 0) x = whole_row<GREEDY>(t_part + (size_t)a * A.pieces, A.pieces, (float)k);
-        else if (!GREEDY && rejected && A.draft) x = whole_row<false>(d_part + (size_t)a * A.pieces, A.pieces, (float)k);
-        if (lane == 0) s_row[warp] = x;
-    }
-    __syncthreads();
+    const float2 rp = rows[a][0], rq = rows[a][1];
     if constexpr (GREEDY) {
-        if (threadIdx.x == 0) *token = isfinite(s_row[0].x) ? __float_as_int(s_row[0].y) : -1;
+        if (threadIdx.x == 0) *token = isfinite(rp.x) ? __float_as_int(rp.y) : -1;
     } else {
-        if (!sound(s_row[0])) {                                   // a row without a distribution, for all CTAs of the sequence
+        if (!sound(rp)) {                                   // a row without a distribution, for all CTAs of the sequence
             if (blockIdx.x == 0 && threadIdx.x == 0) *token = -1;
             return;
         }
         const int away = rejected && !A.draft ? A.tokens[(size_t)b * A.n + a] : -1;
-        const typename E::T *p = target + a * A.t_stride, *q = sound(s_row[1]) ? draft + a * A.d_stride : nullptr;   // a draft row without one takes nothing away
-        draw<E>(A, b, p, q, s_row[0], s_row[1], k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], away, shared, token);
+        const typename E::T *p = target + a * A.t_stride, *q = sound(rq) ? draft + a * A.d_stride : nullptr;   // a draft row without one takes nothing away
+        draw<E>(A, b, p, q, rp, rq, k, (double)A.uniforms[(size_t)b * (A.n + 1) + A.n], away, shared, token);
     }
 }
 
