@@ -583,6 +583,9 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     if (with_weights && !a.nslots) return false;
     const size_t tokens = (size_t)a.batch * a.q_len, rows = tokens * a.rep;
     l.t_rt = row_tiles((size_t)a.q_len * a.rep);
+    // slices of the tails: three to a group of warps that one row tile makes, one or two where more do (32 sequences with weights: 24 an SM 85 us, 12 90;
+    // 64 sequences x 8 tokens: 6 an SM 165 us, 12 170)
+    a.t_slices = std::max(1u, (l.t_rt == 1 ? 24 : std::max(3u, 12 / l.t_rt)) * SMS / a.kv_heads);
     // The prefix goes with the tails, in their launch, while its rows fit into their row tile, or are in few tiles of 16 and meet few
     // positions; else on tcgen05. 8 heads of 128, 32 rows: 512 positions 11.2 us with the tails, 13.3 on tcgen05; 2048 15.0 and
     // 14.9; 8192 24.9 and 20.1. 64 rows: 512 12.2 and 13.8; 2048 20.6 and 19.9. 128 rows: 512 13.4 and 14.4.
@@ -593,19 +596,25 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     a.p_slices = a.p_len = 0;
     if (tiles) {
         const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * 8 / l.t_rt;
-        uint32_t best = l.umma ? 1 : std::min(tiles, std::max(1u, fit / groups));
-        size_t least = SIZE_MAX;
-        // rounds over the SMs of slices and about three tiles' time to begin and end one
-        for (uint32_t s = 1; l.umma && s <= std::min(tiles, fit); s++) {
-            const size_t cost = ((size_t)groups * s + fit - 1) / fit * ((tiles + s - 1) / s + 3);
-            if (cost < least) { least = cost; best = s; }
+        uint32_t best = std::min(tiles, std::max(1u, fit / groups));
+        if (l.umma) {
+            // What a number of slices costs, in us: a CTA takes about 7 and 2.6 a tile of two row tiles (1.6 of one). SMs that have none
+            // work on the tails meanwhile, 43 KB a us each, 30 while slices are one tile; what is left of those behind the prefix begins
+            // 4 us later. The tails are taken as half full. 8 sequences behind 8192 positions: 16 slices, which fill the SMs best, 32.8 us,
+            // this way 26.6 (replayed, L2 cold); 64 behind 32768: 18 slices 95.4, 84.6; 32 with 2048 slots behind 16384: 67.3, 63.1.
+            const bool short_ones = (size_t)a.batch * a.nslots / 2 / TILE <= a.t_slices;
+            const double per = a.p_tiles > 1 ? 2.6 : 1.6, work = (double)a.batch * a.kv_heads * a.nslots * hd * 4 / 2 / (short_ones ? 30e3 : 43e3);
+            double least = 1e30;
+            for (uint32_t s = 1; s <= std::min(tiles, fit); s++) {
+                const uint32_t ctas = groups * s, rounds = (ctas + SMS - 1) / SMS;
+                const double t = rounds * (7.0 + per * ((tiles + s - 1) / s)), left = work - (rounds == 1 ? (SMS - ctas) * t : 0.0);
+                const double cost = t + (left > 0.0 ? left / SMS + 4.0 : 0.0);
+                if (cost < least) { least = cost; best = s; }
+            }
         }
         a.p_len = (tiles + best - 1) / best * unit;
         a.p_slices = (a.n_prefix + a.p_len - 1) / a.p_len;
     }
-    // slices: three to a group of warps that one row tile makes, one or two where more do (32 sequences with weights: 24 an SM 85 us, 12 90;
-    // 64 sequences x 8 tokens: 6 an SM 165 us, 12 170)
-    a.t_slices = std::max(1u, (l.t_rt == 1 ? 24 : std::max(3u, 12 / l.t_rt)) * SMS / a.kv_heads);
     const size_t t_rows = a.nslots ? ((size_t)a.t_slices + a.batch) * a.kv_heads * a.q_len * a.rep : 0, parts = a.p_rows() + t_rows;
     *why = "attn shared: 2^31 partial results at most";
     if (parts >= (1ull << 31)) return false;
