@@ -7,7 +7,7 @@
 //   T = 0: x_i is accepted while it is the lowest place of the largest logit, and the token behind is that place
 //
 // verify_rows_kernel: maximum and sum of 2^((x - maximum) k), k = log2(e) / T, of pieces of the rows, a warp to a piece, in fp32: within some
-// 2^-20, which is what the tests of acceptance go by.
+// 2^-20, which is what the tests of acceptance go by. Rows that are there are counted first, and cut so that every warp has a like share.
 // verify_choose_kernel: several CTAs per sequence decide, each for itself, how many are accepted, and draw the token behind them. A draw
 // that ends next to the border of two tokens has to go to the right one, and there are as many borders as tokens: this one row
 // is taken in 64 bits. Every warp has a stretch of the vocabulary; the CTA that comes last sees from the stretches' sums in which
@@ -42,13 +42,15 @@ struct VerifyArgs {
     const int32_t *tokens, *n_drafts;
     const float* uniforms;
     int32_t *accepted, *out;
-    uint32_t batch, n, vocab, pieces, piece;        // pieces of `piece` logits to a row
+    uint32_t batch, n, vocab;
     size_t t_stride, d_stride;
     double inv;                             // 1 / T
     uint32_t splits;                        // CTAs that share a sequence's draw
     uint32_t* done;                         // [batch] of them that are through; zeros when the second kernel starts
     double4* sums;                          // [batch][splits * WARPS] of the stretches
-    float2* part;                           // [target rows | draft rows][pieces] {maximum, sum}; T = 0: {maximum, its place}
+    uint32_t* base;                         // where n_drafts is given: [batch] first row of every sequence, behind them the pieces of a row
+    uint32_t pieces;                        // where it is not
+    float2* part;                           // [rows that are there][pieces] {maximum, sum}; T = 0: {maximum, its place}
 };
 
 struct El32 { typedef float T; static constexpr int V = 4; static __device__ float f(float x) { return x; } };
@@ -170,12 +172,31 @@ __device__ __forceinline__ float2 part_of_row(const typename E::T* p, int64_t fi
         }
     };
     int64_t e = first + lane * E::V;
-    if (e < 0 && end > 0) {                                          // in front of the row's first boundary
-        float x[E::V];
-        load_logits<E>(p, e, end, x);
+    auto edge = [&] {                                                // what may have ends of the row among it
+        uint4 w[AHEAD];
+        float x[AHEAD * E::V];
+#pragma unroll
+        for (int u2 = 0; u2 < AHEAD; u2++) {                         // whole vectors first, all of them under way together
+            const int64_t at = e + u2 * STEP;
+            w[u2] = make_uint4(0u, 0u, 0u, 0u);
+            if (at >= 0 && at + E::V <= end) w[u2] = __ldcg((const uint4*)(p + at));
+        }
+#pragma unroll
+        for (int u2 = 0; u2 < AHEAD; u2++) {
+            const int64_t at = e + u2 * STEP;
+            float y[E::V];
+            unpack_logits<E>(w[u2], y);
+            if (at < 0 || at + E::V > end) {
+#pragma unroll
+                for (int i = 0; i < E::V; i++) y[i] = at + i >= 0 && at + i < end ? E::f(p[at + i]) : -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < E::V; j++) x[u2 * E::V + j] = y[j];
+        }
         take(x, e);
-        e += STEP;
-    }
+        e += AHEAD * STEP;
+    };
+    if (first < 0 && end > 0) edge();
     for (; e + (AHEAD - 1) * STEP + E::V <= end; e += AHEAD * STEP) {
         uint4 w[AHEAD];
         float x[AHEAD * E::V];
@@ -190,11 +211,7 @@ __device__ __forceinline__ float2 part_of_row(const typename E::T* p, int64_t fi
         }
         take(x, e);
     }
-    for (; e < end; e += STEP) {
-        float x[E::V];
-        load_logits<E>(p, e, end, x);
-        take(x, e);
-    }
+    while (e < end) edge();
     __syncwarp();
     if (GREEDY) {
         if (odd) { best.x = NAN; place = 0; }
@@ -203,25 +220,83 @@ __device__ __forceinline__ float2 part_of_row(const typename E::T* p, int64_t fi
     return join_lanes<GREEDY, 32>(best, k);
 }
 
-// A warp to a piece of a row, CTAs that stay. Rows in the order of their drafts, so that all CTAs have like shares of the ones that are there.
+// Rows that are there, sequence by sequence: its target rows, then its draft rows.
+__device__ __forceinline__ uint32_t rows_of(const VerifyArgs& A, uint32_t drafts) { return drafts * (A.draft ? 2 : 1) + 1; }
+
+// Pieces of a row, `length` logits each but for what lies between a boundary and the row's start: 1024 at least; one to a warp of four
+// CTAs an SM where that makes eight pieces or more, else 16 to 24, so that the last turn of the warps is a small part of all. (64 sequences
+// with up to 7 drafts, 151936 tokens: 35 us; pieces of 8192 for whatever rows there are 42.5.)
+struct Cut { uint32_t pieces, length; };
+constexpr uint32_t ROW_WARPS = 148 * 4 * (RT / 32), MIN_PIECE = 1024, MOST_PIECES = 24;
+__host__ __device__ inline Cut cut_rows(uint32_t vocab, uint32_t rows) {
+    const uint32_t places = vocab + 7;                             // up to seven in front of the first boundary
+    uint32_t pieces = ROW_WARPS / rows;
+    if (pieces < 8) {
+        pieces = (16 * rows + ROW_WARPS - 1) / ROW_WARPS * ROW_WARPS / rows;
+        pieces = pieces < MOST_PIECES ? pieces : MOST_PIECES;
+    }
+    Cut c;
+    c.length = ((places + pieces - 1) / pieces + 255) & ~255u;
+    c.length = c.length > MIN_PIECE ? c.length : MIN_PIECE;
+    c.pieces = (places + c.length - 1) / c.length;
+    return c;
+}
+
+// A warp to a piece, in turns where there are more.
 template <class E, bool GREEDY>
-__global__ void __launch_bounds__(RT) verify_rows_kernel(const VerifyArgs A) {
+__global__ void __launch_bounds__(RT, 4) verify_rows_kernel(const VerifyArgs A) {
+    extern __shared__ uint32_t base[];                               // [batch + 1] where n_drafts is given
+    __shared__ uint32_t ends[RT / 32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, every = rows_of(A, A.n);
     pdl_wait();
     pdl_release();
-    const uint32_t kinds = A.draft ? 2 : 1, rows = A.batch * (A.n * kinds + 1);
-    const uint64_t items = (uint64_t)rows * A.pieces;
-    const float k = (float)(A.inv * 1.4426950408889634);
+    if (A.n_drafts) {
+        const uint32_t per = (A.batch + RT - 1) / RT, from = min(A.batch, threadIdx.x * per), to = min(A.batch, from + per);
+        uint32_t mine = 0, x;
+        for (uint32_t b = from; b < to; b++) mine += rows_of(A, drafts_of(A, b));
+        x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        if (lane == 31) ends[warp] = x;
+        __syncthreads();
+        for (uint32_t w = 0; w < warp; w++) x += ends[w];
+        if (threadIdx.x == RT - 1) base[A.batch] = x;
+        x -= mine;
+        for (uint32_t b = from; b < to; b++) { base[b] = x; x += rows_of(A, drafts_of(A, b)); }
+        __syncthreads();
+        if (blockIdx.x == 0)
+            for (uint32_t b = threadIdx.x; b <= A.batch; b += RT) A.base[b] = b < A.batch ? base[b] : cut_rows(A.vocab, base[b]).pieces;
+    }
     if (!GREEDY && blockIdx.x == 0)
         for (uint32_t b = threadIdx.x; b < A.batch; b += RT) A.done[b] = 0;
-    for (uint64_t it = (uint64_t)blockIdx.x * (RT / 32) + threadIdx.x / 32; it < items; it += (uint64_t)gridDim.x * (RT / 32)) {
-        const uint32_t piece = (uint32_t)(it % A.pieces), u = (uint32_t)(it / A.pieces), i = u / (A.batch * kinds), v = u % (A.batch * kinds), b = v % A.batch;
-        const bool target = v < A.batch;
-        if (i >= drafts_of(A, b) + (target ? 1 : 0)) continue;
-        const size_t row = target ? (size_t)b * (A.n + 1) + i : (size_t)b * A.n + i;
-        const typename E::T* p = target ? (const typename E::T*)A.target + row * A.t_stride : (const typename E::T*)A.draft + row * A.d_stride;
-        const int64_t first = (int64_t)piece * A.piece - lead<E>(p);
-        const float2 best = part_of_row<E, GREEDY>(p, first, piece + 1 == A.pieces ? (int64_t)A.vocab : min((int64_t)A.vocab, first + A.piece), k);
-        if ((threadIdx.x & 31) == 0) A.part[(row + (target ? 0 : (size_t)A.batch * (A.n + 1))) * A.pieces + piece] = best;
+    const uint32_t rows = A.n_drafts ? base[A.batch] : A.batch * every;
+    const Cut cut = cut_rows(A.vocab, rows);
+    const float k = (float)(A.inv * 1.4426950408889634);
+    for (uint32_t it = blockIdx.x * (RT / 32) + warp; it < rows * cut.pieces; it += gridDim.x * (RT / 32)) {
+        const uint32_t r = it / cut.pieces, piece = it % cut.pieces;
+        uint32_t b = 0, first_row, next;
+        if (A.n_drafts) {
+            for (uint32_t n = A.batch; n > 1;) {                     // the last sequence that begins at r or in front of it
+                const uint32_t half = n / 2;
+                if (base[b + half] <= r) b += half;
+                n -= half;
+            }
+            first_row = base[b];
+            next = base[b + 1];
+        } else {
+            b = r / every;
+            first_row = b * every;
+            next = first_row + every;
+        }
+        const uint32_t targets = A.draft ? (next - first_row + 1) / 2 : next - first_row, i = r - first_row;
+        const typename E::T* p = i < targets ? (const typename E::T*)A.target + ((size_t)b * (A.n + 1) + i) * A.t_stride
+                                             : (const typename E::T*)A.draft + ((size_t)b * A.n + i - targets) * A.d_stride;
+        const int64_t from = (int64_t)piece * cut.length - lead<E>(p);
+        const float2 best = part_of_row<E, GREEDY>(p, from, min((int64_t)A.vocab, from + cut.length), k);
+        if (lane == 0) A.part[it] = best;
     }
 }
 
@@ -452,13 +527,15 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
     if (!GREEDY && threadIdx.x < 32) shared.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
     const typename E::T *target = (const typename E::T*)A.target + (size_t)b * (A.n + 1) * A.t_stride, *draft = (const typename E::T*)A.draft + (size_t)b * A.n * A.d_stride;
     const double k = A.inv * 1.4426950408889634;
-    const float2 *t_part = A.part + (size_t)b * (A.n + 1) * A.pieces, *d_part = A.part + ((size_t)A.batch * (A.n + 1) + (size_t)b * A.n) * A.pieces;
+    const uint32_t base = A.n_drafts ? A.base[b] : b * rows_of(A, A.n);
+    const uint32_t pieces = A.n_drafts ? A.base[A.batch] : A.pieces;
+    const float2* part = A.part + (size_t)base * pieces;
     // ---- which drafts pass; the row behind the last one is looked at beside them
     for (uint32_t i = warp; i <= nd; i += WARPS) {
         const int x = i < nd ? A.tokens[(size_t)b * A.n + i] : -1;
         const bool in = x >= 0 && (uint32_t)x < A.vocab;
         const double lp = !GREEDY && in ? (double)E::f(target[i * A.t_stride + x]) : 0.0, lq = !GREEDY && in && A.draft ? (double)E::f(draft[i * A.d_stride + x]) : 0.0;
-        const float2 p = whole_row<GREEDY>(t_part + (size_t)i * A.pieces, A.pieces, (float)k);
+        const float2 p = whole_row<GREEDY>(part + (size_t)i * pieces, pieces, (float)k);
         float2 q = make_float2(NAN, NAN);
         bool ok = i < nd;
         if (GREEDY) {
@@ -468,7 +545,7 @@ __global__ void __launch_bounds__(CT, 4) verify_choose_kernel(const VerifyArgs A
             ok = sound(p);
             if (ok && in) px = exp2((lp - p.x) * k) / p.y;
             if (A.draft) {
-                q = whole_row<false>(d_part + (size_t)i * A.pieces, A.pieces, (float)k);
+                q = whole_row<false>(part + (size_t)(nd + 1 + i) * pieces, pieces, (float)k);
                 ok = ok && sound(q);
                 qx = ok && in ? exp2((lq - q.x) * k) / q.y : 0.0;
             }
@@ -541,29 +618,20 @@ const char* verify_refuses(uint32_t batch, uint32_t n, uint32_t vocab) {
     return nullptr;
 }
 
-// Pieces of a row, a warp's each: of 1024 to 8192 logits, some 64 warps an SM over all rows
-void cut_rows(uint32_t batch, uint32_t n, uint32_t vocab, uint32_t* piece, uint32_t* pieces) {
-    const size_t total = (size_t)batch * (2 * n + 1) * vocab;
-    uint32_t p = 1024;
-    while (p < 8192 && (size_t)p * 148 * 64 < total) p *= 2;
-    *piece = p;
-    *pieces = (uint32_t)(((size_t)vocab + 7 + p - 1) / p);    // up to seven logits in front of the first boundary
-}
-
 // CTAs to a sequence's draw: four an SM over all sequences, while every thread has a vector of logits
 uint32_t cut_draw(uint32_t batch, uint32_t vocab) {
     return std::max(1u, std::min({MAX_SPLITS, 148 * 4 / batch, vocab / (CT * 8)}));
 }
 
-struct Layout { size_t sums, part, total; };
+struct Layout { size_t sums, base, part, total; };
 Layout lay_out(uint32_t batch, uint32_t n, uint32_t vocab) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    uint32_t piece, pieces;
-    cut_rows(batch, n, vocab, &piece, &pieces);
     Layout l;
     l.sums = up((size_t)batch * 4);
-    l.part = l.sums + up((size_t)batch * cut_draw(batch, vocab) * WARPS * sizeof(double4));
-    l.total = l.part + up((size_t)batch * (2 * n + 1) * pieces * 8);
+    l.base = l.sums + up((size_t)batch * cut_draw(batch, vocab) * WARPS * sizeof(double4));
+    l.part = l.base + up((size_t)(batch + 1) * 4);
+    // at most: one piece to a warp, or few to a row
+    l.total = l.part + up((ROW_WARPS + (size_t)batch * (2 * n + 1) * std::min(MOST_PIECES, vocab / MIN_PIECE + 2)) * 8);
     return l;
 }
 
@@ -576,9 +644,9 @@ bool launch_verify(cudaStream_t st, const VerifyArgs& a) {
         g_launches++;
         return launch_pdl_cluster(verify_greedy_kernel<E>, cfg, dim3(CL, 1, 1), a) == cudaSuccess;
     }
-    const uint64_t items = ((uint64_t)a.batch * (a.n * (a.draft ? 2 : 1) + 1)) * a.pieces;
+    const uint64_t most = (uint64_t)a.batch * (a.n * (a.draft ? 2 : 1) + 1) * (a.vocab / MIN_PIECE + 1), warps = std::min<uint64_t>(most, ROW_WARPS);
     g_launches += 2;
-    if (launch_pdl(verify_rows_kernel<E, GREEDY>, dim3((uint32_t)std::min<uint64_t>((items + RT / 32 - 1) / (RT / 32), 148 * 6)), dim3(RT), 0, st, a) != cudaSuccess) return false;
+    if (launch_pdl(verify_rows_kernel<E, GREEDY>, dim3((uint32_t)((warps + RT / 32 - 1) / (RT / 32))), dim3(RT), a.n_drafts ? (a.batch + 1) * 4 : 0, st, a) != cudaSuccess) return false;
     return launch_pdl(verify_choose_kernel<E, GREEDY>, dim3(GREEDY ? 1 : a.splits, a.batch), dim3(CT), 0, st, a) == cudaSuccess;
 }
 
@@ -637,12 +705,12 @@ extern "C" int gehtp_verify_drafts(const void* target_dev, const void* draft_dev
     VerifyArgs a{};
     a.target = target_dev; a.draft = draft; a.tokens = tokens_dev; a.n_drafts = n_drafts_dev; a.uniforms = uniforms_dev;
     a.accepted = accepted_dev; a.out = out_dev; a.batch = batch; a.n = n_drafts; a.vocab = vocab;
-    cut_rows(batch, n_drafts, vocab, &a.piece, &a.pieces);
+    a.pieces = cut_rows(vocab, batch * (n_drafts * (draft ? 2 : 1) + 1)).pieces;
     a.t_stride = target_stride; a.d_stride = draft_stride;
     a.inv = greedy ? 0.0 : 1.0 / temperature;
     unsigned char* ws = (unsigned char*)workspace_dev;
     a.splits = cut_draw(batch, vocab);
-    a.done = (uint32_t*)ws; a.sums = (double4*)(ws + l.sums); a.part = (float2*)(ws + l.part);
+    a.done = (uint32_t*)ws; a.sums = (double4*)(ws + l.sums); a.base = (uint32_t*)(ws + l.base); a.part = (float2*)(ws + l.part);
     if (!k_verify_drafts((cudaStream_t)stream, a, dtype, greedy)) {
         const cudaError_t e = cudaGetLastError();
         return fail(e == cudaSuccess ? "verify drafts: launch refused" : cudaGetErrorString(e));
