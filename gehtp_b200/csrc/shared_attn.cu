@@ -51,20 +51,21 @@ __device__ __forceinline__ uint32_t tail_length(const SharedArgs& A, uint32_t b)
 // tail positions that all rows of a sequence see
 __device__ __forceinline__ uint32_t common_length(const SharedArgs& A, uint32_t n) { return n + 1 > A.q_len ? n + 1 - A.q_len : 0; }
 
-// Slices in front of each sequence's (cum[batch]: all of them) and tiles to a slice, by one warp. Slices are as long as cuts
-// the tails together into about t_slices; a sequence with any position has one at least.
+// Slices in front of each sequence's (cum[batch]: all of them) and positions to a slice, by one warp. Slices are as long as cuts
+// the tails together into about t_slices, 64 positions at least and then in steps of 16 where one warp has an item; a sequence with any
+// position has one at least.
 __device__ uint32_t cut_tails(const SharedArgs& A, uint32_t* cum) {
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = threadIdx.x & 31, cut = A.q_len * A.rep <= 16 ? 16 : TILE;
     uint32_t tiles = 0;
-    for (uint32_t b = lane; b < A.batch; b += 32) tiles += (common_length(A, tail_length(A, b)) + TILE - 1) / TILE;
+    for (uint32_t b = lane; b < A.batch; b += 32) tiles += (common_length(A, tail_length(A, b)) + cut - 1) / cut;
     for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-    const uint32_t k = max(1u, (tiles + A.t_slices - 1) / A.t_slices);
+    const uint32_t k = max(TILE / cut, (tiles + A.t_slices - 1) / A.t_slices);
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < A.batch; b0 += 32) {
         const uint32_t b = b0 + lane;
         uint32_t s = 0;
         if (b < A.batch) {
-            const uint32_t n = tail_length(A, b), t = (common_length(A, n) + TILE - 1) / TILE;
+            const uint32_t n = tail_length(A, b), t = (common_length(A, n) + cut - 1) / cut;
             s = n ? max(1u, (t + k - 1) / k) : 0;
         }
         uint32_t x = s;
@@ -76,7 +77,7 @@ __device__ uint32_t cut_tails(const SharedArgs& A, uint32_t* cum) {
         before += __shfl_sync(0xffffffffu, x, 31);
     }
     if (lane == 0) cum[A.batch] = before;
-    return k;
+    return k * cut;
 }
 
 // What an item has to do: rows against keys, and the place of its partial results.
@@ -117,9 +118,9 @@ __device__ __forceinline__ Item item_of(const SharedArgs& A, const uint32_t* cum
         I.c = common_length(A, I.n);
         I.token0 = b * A.q_len;
         I.rows = A.q_len * A.rep;
-        I.from = (u - cum[b]) * k * TILE;
+        I.from = (u - cum[b]) * k;
         I.last = u + 1 == cum[b + 1];
-        I.to = I.last ? I.n : I.from + k * TILE;
+        I.to = I.last ? I.n : I.from + k;
         I.v_off = (size_t)A.batch * A.kv_heads * HD;
         I.kbase = A.tail + ((size_t)b * A.kv_heads + I.h) * HD;
         I.out = A.p_rows() + ((size_t)u * A.kv_heads + I.h) * I.rows;
@@ -127,28 +128,177 @@ __device__ __forceinline__ Item item_of(const SharedArgs& A, const uint32_t* cum
     return I;
 }
 
-// RT warps share an item, 16 rows each (RT: 1, 2, 4 or 8), and the tiles of 16 RT positions that they bring in by cp.async. They meet once a
+// 8x8 words of 16 bits, a row's pairs over four lanes, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// At most 8 rows against 16 positions at a time: the positions are the products' 16 rows and the item's rows their 8 columns, where rows as
+// rows would leave half of every product, exponential and register to nobody. A lane has the rows 2 (lane % 4) and 1 more, at
+// positions lane / 4 and 8 further. 32 sequences of 32 heads, tails of up to 2048 alone: 42.5 us, rows as rows 47.7; 16 of up to 1024 16.2 and 20.0.
+template <bool BF, int HD>
+struct Few {
+    uint32_t q[HD / 16][2];
+    float o[HD / 16][4], m[2], l[2];
+    int lim[2];                                                       // the first position that a row does not see
+
+    __device__ __forceinline__ void begin(const SharedArgs& A, const Item& I, uint32_t lane) {
+        const uint32_t r = lane >> 2, q4 = lane & 3;
+        const bool in = r < I.rows;
+        const uint16_t* qp = A.q + (in ? (size_t)(I.token0 + r / A.rep) * A.q_stride + (size_t)(I.h * A.rep + r % A.rep) * HD : 0) + q4 * 2;
+#pragma unroll
+        for (int x = 0; x < HD / 16; x++) {
+            q[x][0] = in ? *(const uint32_t*)(qp + x * 16) : 0u;
+            q[x][1] = in ? *(const uint32_t*)(qp + x * 16 + 8) : 0u;
+            o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            lim[e] = I.last ? min((int)I.to, (int)(I.n + (q4 * 2 + e) / A.rep + 1) - (int)A.q_len) : (int)I.to;
+            m[e] = -INFINITY;
+            l[e] = 0.0f;
+        }
+    }
+
+    // kt, vt: shared addresses of 16 keys and their values; v: the values once more
+    __device__ __forceinline__ void step(const SharedArgs& A, const Item& I, uint32_t p0, uint32_t kt, uint32_t vt, const unsigned char* v, uint32_t lane) {
+        constexpr uint32_t ROW = HD * 2;
+        const uint32_t g8 = lane >> 2, q4 = lane & 3;
+        float s[4] = {};                                              // position g8 + 8 (e / 2), row 2 q4 + e % 2
+        {
+            const uint32_t r = (lane & 7) + ((lane >> 3) & 1) * 8;
+            float s2[4] = {};
+#pragma unroll
+            for (int x = 0; x < HD / 16; x++) {
+                uint32_t f[4];
+                ldsm4(f, kt + r * ROW + (((2 * x + ((lane >> 4) & 1)) ^ (r & 7)) * 16));
+                mma16<BF>(x & 1 ? s2 : s, f, q[x][0], q[x][1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] += s2[e];
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            s[e] = (int)(p0 + g8 + (e >> 1) * 8) < lim[e & 1] ? s[e] * A.sc : -INFINITY;
+            mx[e & 1] = fmaxf(mx[e & 1], s[e]);
+        }
+        if (I.tail && A.scores) {
+            float* sp = A.scores + (((size_t)I.b * A.kv_heads + I.h) * I.rows + q4 * 2) * A.nslots + p0 + g8;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (q4 * 2 + (e & 1) < I.rows && p0 + g8 + (e >> 1) * 8 < I.to) sp[(size_t)(e & 1) * A.nslots + (e >> 1) * 8] = s[e];
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+                const float mn = fmaxf(m[e], mx[e]), f = mn > m[e] ? (m[e] == -INFINITY ? 0.0f : sm100::ex2(m[e] - mn)) : 1.0f;
+                m[e] = mn;
+                l[e] *= f;
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++) { o[j][e] *= f; o[j][2 + e] *= f; }
+            }
+        }
+        const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            s[e] = sm100::ex2(s[e] - off[e & 1]);
+            l[e & 1] += s[e];
+        }
+        // as below: values that are no numbers, at positions that only some rows see
+        bool odd = false;
+        if (I.last && p0 + 16 > I.c && I.n > I.c) {
+            constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u;
+#pragma unroll 1
+            for (uint32_t e = lane; e < 2 * HD; e += 32)
+                for (uint32_t u = 0; u < 4; u++) {
+                    const uint32_t x = ((const uint32_t*)v)[e * 4 + u];
+                    odd |= (x & EXP & 0xffffu) == (EXP & 0xffffu) || (x & EXP & 0xffff0000u) == (EXP & 0xffff0000u);
+                }
+            odd = __any_sync(0xffffffffu, odd);
+        }
+        if (odd) {
+#pragma unroll 1
+            for (uint32_t col = 0; col < 16; col++) {
+                float p[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) p[e] = __shfl_sync(0xffffffffu, col < 8 ? s[e] : s[2 + e], (int)((col % 8) * 4 + q4));
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) {
+                    const float x = unpack2<BF>(*(const uint16_t*)(v + col * ROW + ((j ^ (col & 7)) * 16) + g8 * 2)).x;
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        if ((int)(p0 + col) < lim[e]) o[j / 2][j % 2 * 2 + e] = fmaf(p[e], x, o[j / 2][j % 2 * 2 + e]);
+                }
+            }
+            return;
+        }
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t w = pack2<BF>(s[2 * half], s[2 * half + 1]);
+            hi[half] = transposed(w);
+            // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
+            if (BF) {
+                const float2 u = unpack2<BF>(w);
+                lo[half] = transposed(pack2<BF>(s[2 * half] - u.x, s[2 * half + 1] - u.y));
+            }
+        }
+        const uint32_t r = (lane & 7) + ((lane >> 4) & 1) * 8;
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++) {
+            uint32_t f[4];
+            ldsm4_t(f, vt + r * ROW + (((2 * j + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+            mma16<BF>(o[j], f, hi[0], hi[1]);
+            if (BF) mma16<BF>(o[j], f, lo[0], lo[1]);
+        }
+    }
+
+    __device__ __forceinline__ void write(const SharedArgs& A, const Item& I, uint32_t lane) {
+        const uint32_t g8 = lane >> 2, q4 = lane & 3;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t r = q4 * 2 + e;
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+            if (r < I.rows) {
+                if (g8 == 0) A.part_ml[I.out + r] = make_float2(m[e], l[e]);
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) A.part_o[(I.out + r) * HD + j * 8 + g8] = o[j / 2][j % 2 * 2 + e];
+            }
+        }
+    }
+};
+
+// RT warps share an item, 16 rows each (RT: 1, 2, 4 or 8; 0: one warp and at most 8 rows), and the tiles of 16 RT positions that they bring in by cp.async. They meet once a
 // tile among themselves and with nobody else, so that what an item costs to begin and to end is other groups' time: eight warps an
-// SM, 24 KB of tiles each. A CTA to an item, with 64 positions split over its warps, took 93 us where this takes 89 (32 sequences,
+// SM, 24 KB of tiles each (twelve of 16 KB where rows are at most 8). A CTA to an item, with 64 positions split over its warps, took 93 us where this takes 89 (32 sequences,
 // tails of 1024 to 4096).
-template <int HD>
-__host__ __device__ constexpr int warp_stages() { return HD == 128 ? 3 : 6; }
+template <int HD, int RT>
+__host__ __device__ constexpr int warp_stages() { return (HD == 128 ? 1 : 2) * (RT ? 3 : 2); }
 template <int RT>
 __host__ __device__ constexpr int warps_of() { return RT == 8 ? 8 : 4; }
 template <int HD, int RT>
-__host__ __device__ constexpr size_t parts_smem() { return (size_t)warps_of<RT>() * warp_stages<HD>() * 64 * HD + (MAX_BATCH + 4) * 4; }
+__host__ __device__ constexpr size_t parts_smem() { return (size_t)warps_of<RT>() * warp_stages<HD, RT>() * 64 * HD + (MAX_BATCH + 4) * 4; }
+
+template <int RT>
+__host__ __device__ constexpr int parts_ctas() { return RT == 8 ? 1 : RT ? 2 : 3; }
 
 template <bool BF, int HD, int RT>
-__global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
-    constexpr uint32_t ST = warp_stages<HD>(), ROW = HD * 2, TP = 16 * RT, HALF = TP * ROW, NT = warps_of<RT>() * 32, GROUPS = warps_of<RT>() / RT;
+__global__ void __launch_bounds__(warps_of<RT>() * 32, parts_ctas<RT>()) shared_parts_kernel(const SharedArgs A, uint32_t prefix_items, uint32_t with_tails, uint32_t beside) {
+    constexpr uint32_t W = RT ? RT : 1, ST = warp_stages<HD, RT>(), ROW = HD * 2, TP = 16 * W, HALF = TP * ROW, NT = warps_of<RT>() * 32, GROUPS = warps_of<RT>() / W;
     extern __shared__ __align__(128) unsigned char smem[];
     uint32_t* cum = (uint32_t*)(smem + GROUPS * ST * 2 * HALF);
     __shared__ uint32_t s_k, s_next[GROUPS][2];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3, group = warp / RT, part = warp % RT;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3, group = warp / W, part = warp % W;
     const uint32_t base = smem_addr(smem), ring = base + group * ST * 2 * HALF;
     auto meet = [&] {
-        if (RT == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(RT * 32) : "memory");
+        if (W == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(W * 32) : "memory");
     };
     // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait: all that was there before the
     // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
@@ -195,7 +345,7 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
                 const uint32_t st = ring + (i % ST) * 2 * HALF;
 #pragma unroll
                 for (uint32_t u = 0; u < HD / 16; u++) {
-                    const uint32_t e = u * (RT * 32) + part * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), pos = I.from + i * TP + r;
+                    const uint32_t e = u * (W * 32) + part * 32 + lane, r = e / (HD / 8), ch = e % (HD / 8), pos = I.from + i * TP + r;
                     const bool in = pos < I.to;                     // rows past the end: zeros, whatever the cache holds there
                     const uint16_t* src = I.kbase + (in ? (size_t)pos * pitch + ch * 8 : 0);
                     const uint32_t dst = st + r * ROW + ((ch ^ (r & 7)) * 16);
@@ -207,6 +357,23 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, RT == 8 ? 1 : 2) shared_p
         };
 #pragma unroll
         for (uint32_t i = 0; i < ST - 1; i++) load(i);
+        if constexpr (RT == 0) {
+            Few<BF, HD> rows;
+            rows.begin(A, I, lane);
+            for (uint32_t i = 0; i < tiles; i++) {
+                cp_wait<ST - 2>();
+                meet();
+                load(i + ST - 1);                                     // over the tile before, which all lanes have read
+                const uint32_t kt = (i % ST) * 2 * HALF + (ring - base);
+                rows.step(A, I, I.from + i * TP, base + kt, base + kt + HALF, smem + kt + HALF, lane);
+            }
+            cp_wait<0>();
+            if (lane == 0) s_next[group][turn] = ahead;
+            meet();                                                // the next item's tiles go over the ones just read
+            w = s_next[group][turn];
+            rows.write(A, I, lane);
+            continue;
+        }
         uint32_t qf[HD / 16][4];
         int lim[2];                                                   // the first position that a row does not see
 #pragma unroll
@@ -540,12 +707,13 @@ bool launch_parts(cudaStream_t st, const SharedArgs& a, uint32_t prefix_items, b
     const size_t items = prefix_items + (tails ? ((size_t)a.t_slices + a.batch) * a.kv_heads : 0);
     if (!items) return true;
     g_launches++;
-    return launch_pdl(shared_parts_kernel<BF, HD, RT>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * (RT == 8 ? 1 : 2))), dim3(warps_of<RT>() * 32),
+    return launch_pdl(shared_parts_kernel<BF, HD, RT>, dim3((uint32_t)std::min<size_t>(items, (size_t)SMS * parts_ctas<RT>())), dim3(warps_of<RT>() * 32),
                       parts_smem<HD, RT>(), st, a, prefix_items, tails ? 1u : 0u, beside ? 1u : 0u) == cudaSuccess;
 }
 template <bool BF, int HD>
 bool launch_parts_rt(cudaStream_t st, const SharedArgs& a, uint32_t rt, uint32_t prefix_items, bool tails, bool beside) {
     switch (rt) {
+        case 0: return launch_parts<BF, HD, 0>(st, a, prefix_items, tails, beside);
         case 1: return launch_parts<BF, HD, 1>(st, a, prefix_items, tails, beside);
         case 2: return launch_parts<BF, HD, 2>(st, a, prefix_items, tails, beside);
         case 4: return launch_parts<BF, HD, 4>(st, a, prefix_items, tails, beside);
@@ -582,20 +750,22 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     *why = "attn shared: weights of tails that have no slots";
     if (with_weights && !a.nslots) return false;
     const size_t tokens = (size_t)a.batch * a.q_len, rows = tokens * a.rep;
-    l.t_rt = row_tiles((size_t)a.q_len * a.rep);
-    // slices of the tails: three to a group of warps that one row tile makes, one or two where more do (32 sequences with weights: 24 an SM 85 us, 12 90;
-    // 64 sequences x 8 tokens: 6 an SM 165 us, 12 170)
-    a.t_slices = std::max(1u, (l.t_rt == 1 ? 24 : std::max(3u, 12 / l.t_rt)) * SMS / a.kv_heads);
+    const uint32_t tail_rows = a.q_len * a.rep, t_rt = row_tiles(tail_rows);
+    // slices of the tails: three to a group of warps that one row tile makes, one or two where more do (64 sequences x 8 tokens: 6 an SM 165 us,
+    // 12 170), somewhat less than two to a warp of at most 8 rows (32 sequences with weights: 23 an SM 74.7 us, 16 78.8, 27 79.7)
+    a.t_slices = std::max(1u, (tail_rows <= 8 ? 23 : t_rt == 1 ? 24 : std::max(3u, 12 / t_rt)) * SMS / a.kv_heads);
     // The prefix goes with the tails, in their launch, while its rows fit into their row tile, or are in few tiles of 16 and meet few
     // positions; else on tcgen05. 8 heads of 128, 32 rows: 512 positions 11.2 us with the tails, 13.3 on tcgen05; 2048 15.0 and
     // 14.9; 8192 24.9 and 20.1. 64 rows: 512 12.2 and 13.8; 2048 20.6 and 19.9. 128 rows: 512 13.4 and 14.4.
-    l.umma = rows > l.t_rt * 16 && !(l.t_rt == 1 && rows * a.n_prefix <= 65536);
-    a.p_tokens = (uint32_t)std::min<size_t>(tokens, (l.umma ? 128 : l.t_rt * 16) / a.rep);
+    l.t_rt = t_rt;
+    l.umma = rows > t_rt * 16 && !(t_rt == 1 && rows * a.n_prefix <= 65536);
+    a.p_tokens = (uint32_t)std::min<size_t>(tokens, (l.umma ? 128 : t_rt * 16) / a.rep);
     a.p_tiles = (uint32_t)((tokens + a.p_tokens - 1) / a.p_tokens);
+    if (tail_rows <= 8 && (l.umma || rows <= 8 || !a.n_prefix)) l.t_rt = 0;
     const uint32_t unit = l.umma ? 128 : TILE, tiles = (a.n_prefix + unit - 1) / unit;
     a.p_slices = a.p_len = 0;
     if (tiles) {
-        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * 8 / l.t_rt;
+        const uint32_t groups = (l.umma && a.p_tiles > 1 ? (a.p_tiles + 1) / 2 : a.p_tiles) * a.kv_heads, fit = l.umma ? SMS : SMS * (l.t_rt ? 8 / t_rt : 12);
         uint32_t best = std::min(tiles, std::max(1u, fit / groups));
         if (l.umma) {
             // What a number of slices costs, in us: a CTA takes about 7 and 2.6 a tile of two row tiles (1.6 of one). SMs that have none
