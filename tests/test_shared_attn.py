@@ -144,6 +144,9 @@ CASES = [
     (16, 1, 8, 1, 128, 513, 33, [33 - i for i in range(16)]),                # 128 rows that meet few positions: with the tails
     (1024, 1, 1, 1, 64, 5, 3, [i % 4 for i in range(1024)]),                 # the most sequences
     (130, 1, 2, 2, 64, 40, 300, [300 if i == 77 else 2 for i in range(130)]),
+    (3, 4, 8, 4, 64, 70, 333, [333, 2, 47]),                # 8 rows to a tail
+    (6, 1, 40, 8, 128, 0, 1500, [1500, 17, 0, 1, 16, 963]), # tails alone, slices that end inside 64 positions
+    (50, 2, 9, 3, 128, 1000, 100, [(9 * i) % 101 for i in range(50)]),       # 6 rows to a tail beside the prefix's
 ]
 
 
@@ -195,6 +198,27 @@ def test_a_position_that_is_no_number(cuda, dtype):
     assert fine[1, :3].all() and fine[2, :3].all()
     assert not torch.isfinite(call.out[1, 3:, :4, 5]).any() and fine[1, 3:, 4:].all() and fine[1, 3:, :4, :5].all() and fine[1, 3:, :4, 6:].all()
     assert not torch.isfinite(call.out[2, 3:]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix,d", [(3, 64), (700, 128)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_the_last_position_is_no_number(cuda, prefix, d, dtype):
+    """As above with 8 rows to a tail: what only the last token sees."""
+    import torch
+    call = Call(20, 2, 8, 2, d, prefix, 90, [80, 70, 90] + [60] * 17, getattr(torch, dtype), weights=True)
+    want, _, _, tol = call.expected()
+    tail = call.tail.view(90, 2, 20, 2, d)
+    tail[40, :, 0] = float("nan")
+    tail[69, 1, 1, 0, 5] = float("inf")
+    tail[89, 0, 2] = float("nan")
+    call.run(cuda)
+    torch.cuda.synchronize()
+    assert not torch.isfinite(call.out[0]).any()
+    fine = (call.out.cpu().double() - want).abs() <= tol
+    assert fine[1, 0].all() and fine[2, 0].all() and fine[3:].all()
+    assert not torch.isfinite(call.out[1, 1, :4, 5]).any() and fine[1, 1, 4:].all() and fine[1, 1, :4, :5].all() and fine[1, 1, :4, 6:].all()
+    assert not torch.isfinite(call.out[2, 1]).any()
 
 
 @pytest.mark.gpu
