@@ -112,6 +112,8 @@ CASES = [
     (33, 5, 3001, "float32", 0.0, False, (0, 0), 3), (2, 20, 30000, "bfloat16", 0.0, False, (0, 0), 1), (700, 2, 90, "float16", 0.0, False, (0, 0), 1),
     (700, 2, 90, "float32", 0.9, True, (0, 0), 1),
     (9, 4, 1001, "float32", 0.0, False, (0, 0), 1), (3, 8, 40000, "bfloat16", 0.0, False, (0, 0), 0), (4, 3, 20011, "float16", 0.0, True, (5, 0), 0),
+    # more pieces of rows than warps that take them
+    (700, 2, 5000, "bfloat16", 1.0, True, (0, 8), 0), (120, 7, 30011, "bfloat16", 0.9, True, (0, 0), 1), (1100, 3, 4000, "float32", 0.0, False, (0, 0), 0),
 ]
 
 
