@@ -469,41 +469,54 @@ __device__ __forceinline__ void draw(const VerifyArgs& A, uint32_t b, const type
         }
         lowest(S, (int)threadIdx.x == S.last / 2 ? S.last : INT_MAX, S.last & 1 ? front + w[0] : front);
     }
-    const int at = S.first;
-    const int64_t from = vecs * at / stretches, to = vecs * (at + 1) / stretches;
+    // The token in that stretch. What p - q leaves of like tokens is the rounding of two sums, so a stretch may have a weight and no token with
+    // one (at the ends of the draw, where the goal is 0 or the whole sum): then the next stretch's first token, else one in front of it.
+    const int begin = S.first;
     double upto = S.front;
-    __syncthreads();
-    if (threadIdx.x == 0) S.last = -1;
-    for (int64_t j0 = from; j0 < to; j0 += CT) {
-        const int64_t j = j0 + threadIdx.x, e = j * E::V - p_lead;
-        float x[E::V], y[E::V];
-        double r[E::V], sum = 0.0, all;
-        if (j < to) {
-            load_logits<E>(p, e, vocab, x);
-            if (less) load_logits<E>(q, e, vocab, y);
-        }
-#pragma unroll
-        for (int i = 0; i < E::V; i++) {
-            r[i] = j >= to || e + i == away ? 0.0 : less ? rest(x[i], y[i]) : ep(x[i]);
-            sum += r[i];
-        }
-        double s = upto + S.scan.before(sum, &all);
-        int here = INT_MAX, some = -1;
-#pragma unroll
-        for (int i = 0; i < E::V; i++) {
-            s += r[i];
-            if (r[i] > 0.0) {
-                some = (int)(e + i);
-                if (here == INT_MAX && s > goal) here = some;
+    for (int at = begin, way = 1; ; at += way) {
+        if (at == (int)stretches) { at = begin - 1; way = -1; }
+        if (at < 0) break;                                    // not reached: some token has a weight
+        const int64_t from = vecs * at / stretches, to = vecs * (at + 1) / stretches;
+        const double end = at == begin ? goal : way > 0 ? -1.0 : INFINITY;
+        __syncthreads();
+        if (threadIdx.x == 0) { S.last = -1; S.first = INT_MAX; }
+        for (int64_t j0 = from; j0 < to; j0 += CT) {
+            const int64_t j = j0 + threadIdx.x, e = j * E::V - p_lead;
+            float x[E::V], y[E::V];
+            double r[E::V], sum = 0.0, all;
+            if (j < to) {
+                load_logits<E>(p, e, vocab, x);
+                if (less) load_logits<E>(q, e, vocab, y);
             }
+#pragma unroll
+            for (int i = 0; i < E::V; i++) {
+                r[i] = j >= to || e + i == away ? 0.0 : less ? rest(x[i], y[i]) : ep(x[i]);
+                sum += r[i];
+            }
+            double s = upto + S.scan.before(sum, &all);
+            int here = INT_MAX, some = -1;
+#pragma unroll
+            for (int i = 0; i < E::V; i++) {
+                s += r[i];
+                if (r[i] > 0.0) {
+                    some = (int)(e + i);
+                    if (here == INT_MAX && s > end) here = some;
+                }
+            }
+            if (some >= 0) atomicMax(&S.last, some);
+            lowest(S, here, 0.0);
+            if (S.first != INT_MAX) break;
+            upto += all;
         }
-        if (some >= 0) atomicMax(&S.last, some);
-        lowest(S, here, 0.0);
-        if (S.first != INT_MAX) break;
-        upto += all;
+        __syncthreads();
+        // the stretch's sum was above the goal: its last possible token at the latest
+        const int token = S.first != INT_MAX ? S.first : S.last;
+        if (token >= 0) {
+            if (threadIdx.x == 0) *to_ = token;
+            return;
+        }
     }
-    // the stretch's sum was above the goal: its last possible token at the latest
-    if (threadIdx.x == 0) *to_ = S.first != INT_MAX ? S.first : S.last;
+    if (threadIdx.x == 0) *to_ = -1;
 }
 
 // What a sequence gets: `a` accepted drafts, -1 behind the token that follows them.

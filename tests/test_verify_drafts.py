@@ -251,3 +251,26 @@ def test_captured_and_replayed(cuda, heat):
         graph.replay()
         torch.cuda.synchronize()
         assert np.array_equal(accepted.cpu().numpy(), want) and np.array_equal(out.cpu().numpy(), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [300, 5003, 70001])
+@pytest.mark.parametrize("u", [0.0, 1.0])
+def test_ends_of_a_draw_from_a_few_tokens(cuda, dtype, vocab, u):
+    """Rows that differ in two tokens only: what is left of all others is the rounding of two sums in 64 bits. The ends of the draw yield a token of the vocabulary,
+    with next to nothing of max(p - q, 0) in front of it (behind it)."""
+    import torch
+    for seed in range(6):
+        g = torch.Generator().manual_seed(seed)
+        target = 2.5 * torch.randn(16, 2, vocab, generator=g)
+        target[:, :, vocab // 2], target[:, :, vocab // 2 + 1] = 5.0, 3.0
+        target = target.to(getattr(torch, dtype))
+        draft = target[:, :1].clone()
+        draft[:, :, vocab // 2], draft[:, :, vocab // 2 + 1] = 3.0, 5.0
+        tokens = torch.full((16, 1), -1, dtype=torch.int32)
+        accepted, out = verify(cuda, target, draft, tokens, None, torch.full((16, 2), u), vocab, 0.9)
+        assert (accepted == 0).all() and (out[:, 0] >= 0).all() and (out[:, 0] < vocab).all()
+        for b in range(16):
+            r = np.maximum(chances(target[b, 0].double().numpy(), 0.9) - chances(draft[b, 0].double().numpy(), 0.9), 0.0)
+            assert (r[:out[b, 0]].sum() if u == 0.0 else r[out[b, 0] + 1:].sum()) <= 1e-12
