@@ -85,17 +85,18 @@ __device__ __forceinline__ void load_logits(const typename E::T* row, int64_t e,
 template <class E>
 __device__ __forceinline__ int lead(const typename E::T* row) { return (int)(((uintptr_t)row & 15u) / sizeof(typename E::T)); }
 
-// 2^((x - m) k) in 64 bits: x k - m k split into 32nds and at most half a 32nd; 2^that by a table of the 32 and the interpolation of degree 4 at
+// 2^((x - m) k) in 64 bits: (x - m) k split into 32nds and at most half a 32nd; 2^that by a table of the 32 and the interpolation of degree 4 at
 // the Chebyshev points of [-1/64, 1/64] (within 2^-43): nine 64-bit operations, of which 64 a cycle and SM run, where degree 9 over
-// [-1/2, 1/2] takes thirteen. 0 below 2^-1000 and for -inf.
+// [-1/2, 1/2] takes thirteen. The difference comes first: products of numbers far from 0, as masks leave them, are rounded by more than it is. 0
+// below 2^-1000 (its border rounded up: a number just below that is further down where neighbouring logits are) and for -inf.
 struct Power64 {
     const double* table;                                      // 2^(j / 32)
-    double k, mk;
+    double k, m;
     float floor;
-    __device__ __forceinline__ Power64(const double* table_, double k_, float m) : table(table_), k(k_), mk(-(double)m * k_), floor((float)((double)m - 1000.0 / k_)) {}
+    __device__ __forceinline__ Power64(const double* table_, double k_, float m_) : table(table_), k(k_), m(m_) { floor = __double2float_ru(m - 1000.0 / k); }
     __device__ __forceinline__ double operator()(float x) const {
-        const double t = fma((double)fmaxf(x, floor), k, mk), magic = 211106232532992.0 /* 1.5 * 2^47 */, n = t + magic, f = t - (n - magic);
-        const int i = __double2loint(n);                      // t in 32nds
+        const double d = (double)fmaxf(x, floor) - m, magic = 211106232532992.0 /* 1.5 * 2^47 */, n = fma(d, k, magic), f = fma(d, k, magic - n);
+        const int i = __double2loint(n);                      // d k in 32nds
         double v = 0.009618176115571158;
         v = fma(v, f, 0.055504515573860415);
         v = fma(v, f, 0.24022650695623157);

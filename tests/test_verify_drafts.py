@@ -274,3 +274,38 @@ def test_ends_of_a_draw_from_a_few_tokens(cuda, dtype, vocab, u):
         for b in range(16):
             r = np.maximum(chances(target[b, 0].double().numpy(), 0.9) - chances(draft[b, 0].double().numpy(), 0.9), 0.0)
             assert (r[:out[b, 0]].sum() if u == 0.0 else r[out[b, 0] + 1:].sum()) <= 1e-12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,fill,heat", [("float32", float(np.finfo(np.float32).min), 1.0), ("bfloat16", -3.3895313892515355e38, 0.7), ("float16", -65504.0, 1e-4),
+                                             ("float32", 1e30, 0.8), ("float32", -1e17, 1.0), ("float32", 7e20, 1.0),
+                                             ("float32", -5e21, 0.8), ("float32", 1e23, 1.0)])
+@pytest.mark.parametrize("with_draft", [False, True])
+def test_rows_masked_to_one_value(cuda, dtype, fill, heat, with_draft):
+    """Every logit the same, the type's lowest number among them: each token is as likely as the next. The drafts' rows have only their first third."""
+    import torch
+    batch, vocab = 24, 3001
+    target = torch.full((batch, 2, vocab), fill).to(getattr(torch, dtype))
+    draft = target[:, :1].clone()
+    draft[:, :, 1000:] = -float("inf")
+    for seed in range(20):
+        g = torch.Generator().manual_seed(seed)
+        tokens = torch.randint(0, 1000, (batch, 1), generator=g, dtype=torch.int32)
+        tokens[::3] = -1
+        uniforms = torch.rand(batch, 2, generator=g)
+        accepted, out, near, border = by_rule(target, draft if with_draft else None, tokens, None, uniforms, vocab, heat)
+        if near > 2.0 ** -18 and border > 1e-11:
+            break
+    got = verify(cuda, target, draft if with_draft else None, tokens, None, uniforms, vocab, heat)
+    assert border > 1e-11 and np.array_equal(got[0], accepted) and np.array_equal(got[1], out)
+
+
+@pytest.mark.gpu
+def test_far_logits_at_a_low_temperature(cuda):
+    """Numbers an eighth apart, 1803 powers of two at this temperature: all but the largest weigh nothing."""
+    import torch
+    target = torch.full((4, 1, 3000), 1048586.0 - 0.125)
+    at = torch.tensor([0, 700, 1503, 2999])
+    target[torch.arange(4), 0, at] = 1048586.0
+    accepted, out = verify(cuda, target, None, torch.zeros(4, 0, dtype=torch.int32), None, torch.tensor([[0.0], [0.3], [0.9], [0.5]]), 3000, 1e-4)
+    assert out[:, 0].tolist() == at.tolist()
