@@ -650,6 +650,7 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
         return;
     }
     __shared__ float2 norm[MAX_ROWS];       // {maximum, 1 / sum} of the rows of the key head
+    __shared__ int sees[MAX_ROWS];          // positions of the tail that they see: a sum that is no number is none of the others' matter
     const uint32_t u = blockIdx.x, p0 = (u % chunks) * W_CHUNK, h = (u / chunks) % A.kv_heads, b = u / chunks / A.kv_heads;
     const uint32_t n = tail_length(A, b), rows = A.q_len * A.rep;
     if (p0 >= n) return;
@@ -665,7 +666,8 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
         for (uint32_t r = 0; r < 4; r++) s0[r][i] = in && r < rows ? __ldcg(scores + (size_t)r * A.nslots + i * 256) : -INFINITY;
     }
     for (uint32_t r = warp; r < rows; r += 8) {
-        const RowParts x = row_parts(A, A.plan, b * A.q_len + A.by_rep(r), h * A.rep + r - A.by_rep(r) * A.rep);
+        const uint32_t t = A.by_rep(r);
+        const RowParts x = row_parts(A, A.plan, b * A.q_len + t, h * A.rep + r - t * A.rep);
         const uint32_t count = x.p_count + x.t_count;
         const float2 none = make_float2(-INFINITY, 0.0f), first = lane < count ? __ldcg(&A.part_ml[part_at(x, lane)]) : none;
         float M = first.x;
@@ -677,23 +679,28 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
             L = fmaf(ml.y, part_factor(ml, M), L);
         }
         L = warp_sum(L);
-        if (lane == 0) norm[r] = make_float2(M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L);
+        if (lane == 0) {
+            norm[r] = make_float2(M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L);
+            sees[r] = (int)(n + t + 1) - (int)A.q_len;
+        }
     }
     __syncthreads();
+    const int p = (int)(p0 + threadIdx.x);
     float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (uint32_t r = 0; r < 4; r++)
         if (r < rows) {
             const float2 x = norm[r];
 #pragma unroll
-            for (int i = 0; i < 4; i++) add[i] = fmaf(sm100::ex2(s0[r][i] - x.x), x.y, add[i]);
+            for (int i = 0; i < 4; i++)
+                if (p + i * 256 < sees[r]) add[i] = fmaf(sm100::ex2(s0[r][i] - x.x), x.y, add[i]);
         }
 #pragma unroll 2
     for (uint32_t r = 4; r < rows; r++) {
         const float2 x = norm[r];
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (p0 + i * 256 + threadIdx.x < n) add[i] = fmaf(sm100::ex2(__ldcg(scores + (size_t)r * A.nslots + i * 256) - x.x), x.y, add[i]);
+            if (p + i * 256 < sees[r]) add[i] = fmaf(sm100::ex2(__ldcg(scores + (size_t)r * A.nslots + i * 256) - x.x), x.y, add[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)

@@ -335,3 +335,21 @@ def test_caches_past_four_gigabytes(cuda, batch):
     err = 2.0 ** -8 * want.abs() + (3 * a + 5 * b) / (a + b + rest) * (2.0 ** -16 + 2 * top * 130 * 2.0 ** -23 + 2.0 ** -19 + 2.0 ** -8)
     assert ((got - want[..., None]).abs() <= err[..., None] + 1e-30).all()
     assert cuda.gehtp_attn_shared_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,q_len,heads,prefix", [(2, 3, 4, 0), (3, 4, 8, 60), (33, 2, 16, 700)])
+def test_weights_beside_a_row_that_is_no_number(cuda, batch, q_len, heads, prefix):
+    """The first token's query is no number, and so are the weights of the positions that it sees. Those behind them have theirs from the tokens that see them."""
+    import torch
+    call = Call(batch, q_len, heads, 2, 64, prefix, 90, [90 - i for i in range(batch)], torch.bfloat16, weights=True, seed=batch)
+    _, weights, top, _ = call.expected()
+    call.rows.view(batch, q_len, call.stride)[1, 0, :64] = float("nan")
+    call.run(cuda)
+    torch.cuda.synchronize()
+    n = int(call.n[1])
+    got = (call.w - call.w_in).cpu().double()
+    assert torch.isnan(got[1, 0, :n - q_len + 1]).all()
+    rel = 2 * top.max() * 66 * 2.0 ** -23 + 2.0 ** -19
+    fine = lambda b, h, p: ((got[b, h, p] - weights[b, h, p]).abs() <= weights[b, h, p] * rel + call.w[b, h, p].cpu().abs() * 2.0 ** -22).all()
+    assert fine(1, 0, slice(n - q_len + 1, n)) and fine(1, 1, slice(0, n)) and fine(0, 0, slice(0, int(call.n[0])))
