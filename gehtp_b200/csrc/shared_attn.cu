@@ -47,6 +47,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *(const uint32_t*)&h;
 }
 
+// A score's weight beside a maximum. It meets the values as a word of 16 bits. Where that is fp16 it is made 2^LIFT times as large, which is still below 2^16, so
+// that its 11 bits last down to 2^-29 of the row's largest, and a part of it to 2^-40; without, weights below 2^-25 were gone from the result
+// though their sum was not. Sums and outputs give the factor back when they are written.
+template <bool BF>
+constexpr float LIFT = BF ? 0.0f : 15.0f;
+template <bool BF>
+__device__ __forceinline__ float weight(float s, float m) { return sm100::ex2(BF ? s - m : (s - m) + LIFT<BF>); }
+template <bool BF>
+constexpr float UNLIFT = BF ? 1.0f : 0x1p-15f;
+
 __device__ __forceinline__ uint32_t tail_length(const SharedArgs& A, uint32_t b) { return (uint32_t)min(max(A.n_tail[b], 0), (int)A.nslots); }
 // tail positions that all rows of a sequence see
 __device__ __forceinline__ uint32_t common_length(const SharedArgs& A, uint32_t n) { return n + 1 > A.q_len ? n + 1 - A.q_len : 0; }
@@ -206,7 +216,7 @@ struct Few {
         const float off[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            s[e] = sm100::ex2(s[e] - off[e & 1]);
+            s[e] = weight<BF>(s[e], off[e & 1]);
             l[e & 1] += s[e];
         }
         // as below: values that are no numbers, at positions that only some rows see
@@ -242,7 +252,7 @@ struct Few {
         for (int half = 0; half < 2; half++) {
             const uint32_t w = pack2<BF>(s[2 * half], s[2 * half + 1]);
             hi[half] = transposed(w);
-            // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
+            // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result (and see LIFT).
             if (BF) {
                 const float2 u = unpack2<BF>(w);
                 lo[half] = transposed(pack2<BF>(s[2 * half] - u.x, s[2 * half + 1] - u.y));
@@ -266,9 +276,9 @@ struct Few {
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
             if (r < I.rows) {
-                if (g8 == 0) A.part_ml[I.out + r] = make_float2(m[e], l[e]);
+                if (g8 == 0) A.part_ml[I.out + r] = make_float2(m[e], l[e] * UNLIFT<BF>);
 #pragma unroll
-                for (int j = 0; j < HD / 8; j++) A.part_o[(I.out + r) * HD + j * 8 + g8] = o[j / 2][j % 2 * 2 + e];
+                for (int j = 0; j < HD / 8; j++) A.part_o[(I.out + r) * HD + j * 8 + g8] = o[j / 2][j % 2 * 2 + e] * UNLIFT<BF>;
             }
         }
     }
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, parts_ctas<RT>()) shared_
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        s[t][e] = sm100::ex2(s[t][e] - off[e >> 1]);
+                        s[t][e] = weight<BF>(s[t][e], off[e >> 1]);
                         l[e >> 1] += s[t][e];
                     }
                 // Positions that only some rows see have weight 0 for the others, which is 0 times their values: where one of those is no
@@ -495,7 +505,7 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, parts_ctas<RT>()) shared_
                 for (int e = 0; e < 4; e++) {                          // fragment register e: tile e / 2, rows of half e % 2
                     const float a = s[e >> 1][2 * (e & 1)], c2 = s[e >> 1][2 * (e & 1) + 1];
                     hi[e] = pack2<BF>(a, c2);
-                    // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result.
+                    // bf16 keeps 8 bits of a weight: what it loses goes in as a second term. fp16's 11 bits are those of the result (and see LIFT).
                     if (BF) {
                         const float2 u = unpack2<BF>(hi[e]);
                         lo[e] = pack2<BF>(a - u.x, c2 - u.y);
@@ -525,9 +535,9 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, parts_ctas<RT>()) shared_
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
             if (r < I.rows) {
-                if (q4 == 0) A.part_ml[I.out + r] = make_float2(m[half], l[half]);
+                if (q4 == 0) A.part_ml[I.out + r] = make_float2(m[half], l[half] * UNLIFT<BF>);
 #pragma unroll
-                for (int j = 0; j < HD / 8; j++) *(float2*)&A.part_o[(I.out + r) * HD + j * 8 + q4 * 2] = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+                for (int j = 0; j < HD / 8; j++) *(float2*)&A.part_o[(I.out + r) * HD + j * 8 + q4 * 2] = make_float2(o[j][2 * half] * UNLIFT<BF>, o[j][2 * half + 1] * UNLIFT<BF>);
             }
         }
     }

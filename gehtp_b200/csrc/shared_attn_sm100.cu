@@ -10,8 +10,9 @@
 //   P               one thread per row: maximum, 2^(s - m) written over S as matrix operand: fp16, or bf16 as hi + lo pairs (bf16's 8 bits
 //                   are fewer than a result of that type has)
 //   O += P V        tcgen05.mma with P as the A operand from TMEM, V as it lies in memory (MN-major B operand)
-// The maximum that a row's weights are referred to is one of an earlier tile: the exponentials need not wait for the tile's own. It is
-// raised - and O rescaled - when a tile has exceeded it by more than 2^8.
+// The reference of a row's weights is one of an earlier tile while that serves: O is rescaled only where a tile's maximum is well above it. The
+// maximum comes first all the same. (Half of the weights by the old reference while the maximum is found, and again where it turned out too low:
+// 183 us against 178 for 64 x 8 tokens behind 16384 positions, 94 against 93 for 64 behind 32768 in bf16.)
 //
 // Rows of a tile: p_tokens tokens of rep heads, heads fastest (a three-dimensional TMA box over [head_dim][heads][tokens]). Where rep does
 // not divide 128 the last rows of a tile are left over: what lies in their shared memory never reaches another row.
@@ -37,9 +38,11 @@ namespace {
 
 constexpr uint32_t BKV = 128;
 constexpr int NTHREADS = 384;
-// A reference is raised behind a tile that exceeds it by more than 2^8, and before a tile's weights are used where they would exceed 2^14
-// (fp16 ends at 2^16)
-constexpr float kRaise = 8.0f, kMost = 14.0f;
+// A row's weights are 2^(s - reference). The reference lies kLow below the maximum that it was made from, and is made again, O with it, where a tile would have
+// a weight above 2^kMost. fp16 ends at 2^16 and has 11 bits down to 2^-14: 2^-26 of the row's largest weight, and parts of them down to
+// 2^-37. With references at the maximum itself, weights below 2^-25 were gone from O though not from the sum. bf16 has fp32's range.
+template <bool BF> constexpr float kLow = BF ? 0.0f : 12.0f;
+template <bool BF> constexpr float kMost = BF ? 14.0f : 15.5f;
 
 // stages of K and of V tiles: as many as 227 KB hold behind the rows' tiles
 template <int DB, bool PAIR>
@@ -255,7 +258,7 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");    // 256 x 200 + 128 x 104 = 384 x 168, what the CTA was launched with
         const uint32_t t = (warp - 4) >> 2, quarter = warp & 3;
         const uint32_t ts = tmem + ((quarter * 32) << 16) + t * 128, to_ = ts + 256;
-        float m = -INFINITY, top = -INFINITY;                    // reference of the weights; maximum of the last tile
+        float m = -INFINITY;                                     // reference of the weights
         float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         bool ok = true;
         const bool works = t == 0 || (PAIR ? two : n_kt > 1);
@@ -296,9 +299,11 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
                     tmem_st_wait();
                 }
             };
-            if (round == 0) m = max128(v) * A.sc;
-            else if (__any_sync(0xffffffffu, top > m + kRaise)) rescale(top > m + kRaise, top);
-            auto probs = [&](int c, float off) {
+            const float top = max128(v) * A.sc;
+            if (round == 0) m = top - kLow<BF>;
+            else if (__any_sync(0xffffffffu, top > m + kMost<BF>)) rescale(top > m + kMost<BF>, top - kLow<BF>);
+            const float off = m == -INFINITY ? 0.0f : -m;
+            auto probs = [&](int c) {
                 uint32_t w[32];
                 if (BF) {
                     probs32<false>(v[c], w, A.sc, off, 0u, l2);
@@ -308,22 +313,8 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
                     tmem_st16(ts + c * 32, w);
                 }
             };
-            // The first half's weights by the reference known from earlier tiles, while the tile's maximum is found: only where that is more
-            // than 2^14 above the reference they are made again.
-            const float2 l0 = l2[0], l1 = l2[1];
-            float off;
-#pragma unroll 1
-            for (int again = 0; ; again = 1) {
-                off = m == -INFINITY ? 0.0f : -m;
-                probs(0, off);
-                probs(1, off);
-                top = max128(v) * A.sc;
-                if (again || !__any_sync(0xffffffffu, top > m + kMost)) break;
-                l2[0] = l0; l2[1] = l1;
-                rescale(top > m + kMost, top);
-            }
-            probs(2, off);
-            probs(3, off);
+#pragma unroll
+            for (int c = 0; c < 4; c++) probs(c);
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();

@@ -353,3 +353,39 @@ def test_weights_beside_a_row_that_is_no_number(cuda, batch, q_len, heads, prefi
     rel = 2 * top.max() * 66 * 2.0 ** -23 + 2.0 ** -19
     fine = lambda b, h, p: ((got[b, h, p] - weights[b, h, p]).abs() <= weights[b, h, p] * rel + call.w[b, h, p].cpu().abs() * 2.0 ** -22).all()
     assert fine(1, 0, slice(n - q_len + 1, n)) and fine(1, 1, slice(0, n)) and fine(0, 0, slice(0, int(call.n[0])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("case", [
+    (20, 1, 8, 8, 64, 9000, 0),             # a prefix on tcgen05, one row tile to a key head
+    (36, 1, 8, 2, 128, 5000, 0),            # two
+    (2, 1, 4, 2, 128, 0, 6000),             # tails of few rows
+    (2, 4, 6, 1, 64, 0, 6000),              # of more
+    (1, 1, 16, 1, 128, 3000, 3000),         # a prefix in the tails' launch
+], ids=lambda c: "-".join(map(str, c)))
+def test_many_small_weights_beside_a_large_one(cuda, case, dtype):
+    """One position in 1024 has a score 26 bits above the others and the value 0: all of the result comes from weights of 2^-26. In fp16 a weight is off by at most
+    2^-37 of the row's largest, or by its 11 bits: 2^-37 max|v| a position, over the sum of weights."""
+    import torch
+    batch, q_len, heads, kvh, d, prefix, slots = case
+    call = Call(*case, [slots - 5 * i for i in range(batch)] if slots else [0] * batch, getattr(torch, dtype), seed=prefix)
+    call.scale = 0.125
+    call.rows.zero_()
+    call.rows.view(batch * q_len, heads, d)[:, :, 0] = 8.0
+    for cache, n in ((call.prefix, prefix), (call.tail, slots)):
+        dead = torch.isnan(cache)
+        cache[:, 0] = 0.0
+        cache[::1024, 0, :, 0] = 18.0
+        cache[:, 1] = 512.0 * (1.0 + (torch.arange(d, device="cuda") % 4) / 4).to(cache.dtype)
+        cache[::1024, 1] = 0.0
+        cache[dead] = float("nan")
+    call.run(cuda)
+    torch.cuda.synchronize()
+    tail = torch.nan_to_num(call.tail.cpu().double())
+    out, mag, top, _ = formula(call.rows.cpu().double().reshape(batch, q_len, heads, d), call.prefix.cpu().double(), tail, call.n, call.scale)
+    half, eps_p, lost = (2.0 ** -11, 2.0 ** -11, 2.0 ** -37) if dtype == "float16" else (2.0 ** -8, 2.0 ** -16, 0.0)
+    shortest = min(call.n.tolist()) - q_len + 1
+    largest = (prefix + 1023) // 1024 + max(0, shortest + 1023) // 1024          # that every row sees
+    tol = half * out.abs() + mag * (eps_p + 2 * top * (d + 2) * 2.0 ** -23 + 2.0 ** -19) + (prefix + slots) * lost * 896.0 / largest + 1e-30
+    assert ((call.out.cpu().double() - out).abs() <= tol).all() and (out > 100 * (tol - half * out.abs() - mag * 2.0 ** -8)).all()
