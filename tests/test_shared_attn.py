@@ -389,3 +389,33 @@ def test_many_small_weights_beside_a_large_one(cuda, case, dtype):
     largest = (prefix + 1023) // 1024 + max(0, shortest + 1023) // 1024          # that every row sees
     tol = half * out.abs() + mag * (eps_p + 2 * top * (d + 2) * 2.0 ** -23 + 2.0 ** -19) + (prefix + slots) * lost * 896.0 / largest + 1e-30
     assert ((call.out.cpu().double() - out).abs() <= tol).all() and (out > 100 * (tol - half * out.abs() - mag * 2.0 ** -8)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("batch,prefix,slots", [(20, 3000, 0), (60, 3000, 70), (2, 0, 900), (3, 70, 70), (16, 100, 300)])
+@pytest.mark.parametrize("order", ["any", "up", "down"])
+@pytest.mark.parametrize("q", [4.0, 16384.0])
+def test_scores_far_out(cuda, dtype, batch, prefix, slots, order, q):
+    """Scores of up to 2^32, where neighbouring fp32 numbers are a factor of 2^512 apart as weights: the largest one is all of the row. Its weight's word of fp16 may be 2^-11
+    off, beside a sum that is not (in bf16's two words 2^-16), and the result is rounded once more, where the weight is not 2^0 exactly."""
+    import torch
+    call = Call(batch, 2, 8, 2, 128, prefix, slots, [max(2, slots - i) for i in range(batch)] if slots else [0] * batch, getattr(torch, dtype), seed=batch)
+    c = 3000.0 * torch.randn(prefix + slots, 2, generator=torch.Generator().manual_seed(prefix + slots))
+    if order != "any":
+        c = c.sort(0, descending=order == "down")[0]
+    best = prefix // 2 if prefix else 1 if order == "down" else slots // 2     # a position that all rows of all sequences see
+    c[best] = 25000.0
+    call.rows.fill_(q)
+    call.prefix[:, 0] = c[:prefix, :, None].to(call.prefix)
+    dead = torch.isnan(call.tail)
+    call.tail.view(slots, 2, batch, 2, 128)[:, 0] = c[prefix:, None, :, None].to(call.tail)
+    call.tail[dead] = float("nan")
+    call.run(cuda)
+    torch.cuda.synchronize()
+    value = call.prefix[best, 1][None] if prefix else call.tail[best, 1].view(batch, 2, 128)
+    want = value.repeat_interleave(4, 1)[:, None].expand(batch, 2, 8, 128)
+    eps = 2.0 ** -11 if dtype == "float16" else 2.0 ** -8
+    eps += 2.0 ** -11 if dtype == "float16" else 2.0 ** -16
+    got, want = call.out.double(), want.double()
+    assert ((got - want).abs() <= want.abs() * (eps + 2.0 ** -19) + (2.0 ** -25 if dtype == "float16" else 0.0)).all()
