@@ -35,6 +35,9 @@ struct SharedArgs {
     float2* part_ml;                               // [partial row] {m, sum}
     float* scores;                                 // s of every tail position: [sequence][key head][row][nslots], or NULL
     uint32_t* next;                                // where the tails' kernel runs beside the prefix's, which sets both to 0: items handed out; items + 1
+    // Where it does: the prefix's kernel writes `token`, another one for every call, to *start when all in front of the call has been waited for and
+    // `next` is set. Who reads it there (acquire) sees all of that too. The merge takes it away again.
+    uint64_t *start, token;
     uint32_t* plan;                                // written by the first kernel: slices in front of each sequence's, batch + 1 of them
     __host__ __device__ size_t p_rows() const { return (size_t)p_tiles * kv_heads * p_slices * p_tokens * rep; }
 };

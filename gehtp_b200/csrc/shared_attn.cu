@@ -10,6 +10,8 @@
 // from their lengths, which lie on the device: every CTA works that out for itself. S and P stay in registers (mma.sync m16n8k16).
 // shared_parts_kernel: an item to as many warps as it has 16 rows.
 // shared_merge_kernel: partial results of a row together; where asked for, the weights of the tail positions.
+#include <atomic>
+#include <chrono>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -310,19 +312,24 @@ __global__ void __launch_bounds__(warps_of<RT>() * 32, parts_ctas<RT>()) shared_
         if (W == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(W * 32) : "memory");
     };
-    // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait: all that was there before the
-    // call may be read. The merge waits for this kernel alone, so this one does not end before the other.
+    // Beside the prefix's kernel, which lets this one start when all its CTAs are past their own wait. That says when, not what is visible here: the
+    // prefix's token does. A CTA that does not find it waits for the prefix's end. The merge waits for this kernel alone, so this one does not
+    // end before the other.
     if (!beside) pdl_wait();
     pdl_release();
-    // A CTA that comes up when all items have been handed out has nothing left to work out: an earlier one left their number. The first
-    // goes on all the same, since it writes the plan.
-    if (beside && blockIdx.x) {
+    if (beside) {
+        // A CTA that comes up when all items have been handed out has nothing left to work out: an earlier one left their number. The first
+        // goes on all the same, since it writes the plan.
         if (threadIdx.x == 0) {
+            uint64_t token;
+            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(token) : "l"(A.start) : "memory");
             const uint32_t all = *(volatile uint32_t*)(A.next + 1), out = *(volatile uint32_t*)A.next;
-            s_k = all && out >= all - 1;
+            s_k = token != A.token ? 2u : blockIdx.x && all && out >= all - 1 ? 1u : 0u;
         }
         __syncthreads();
-        if (s_k) { pdl_wait(); return; }
+        const uint32_t found = s_k;
+        if (found) pdl_wait();
+        if (found == 1) return;
         __syncthreads();
     }
     if (with_tails) {
@@ -578,6 +585,7 @@ __global__ void __launch_bounds__(256, 3) shared_merge_kernel(const SharedArgs A
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_release();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *A.start = 0;
     if (blockIdx.x >= weight_blocks) {
         __shared__ uint32_t plan[MAX_BATCH + 1];
         if (A.nslots)
@@ -807,7 +815,7 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     if (parts >= (1ull << 31)) return false;
     a.by_rep = Div(a.rep); a.by_q_len = Div(a.q_len); a.by_p_tokens = Div(a.p_tokens);
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    l.ml = up((size_t)(a.batch + 3) * 4);
+    l.ml = up((size_t)(a.batch + 5) * 4);                // next, start, plan
     l.o = l.ml + up(parts * 8);
     l.scores = l.o + up(parts * hd * 4);
     l.total = l.scores + (with_weights ? up((size_t)a.batch * a.kv_heads * a.q_len * a.rep * a.nslots * 4) : 0);
@@ -824,6 +832,13 @@ bool k_shared_parts(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16
 bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16) {
     if (hd == 128) return bf16 ? launch_merge<true, 128>(st, a) : launch_merge<false, 128>(st, a);
     return bf16 ? launch_merge<true, 64>(st, a) : launch_merge<false, 64>(st, a);
+}
+
+// Not 0, and of 2^64 that a workspace may hold: a multiple of an odd number, from a place that the clock gives.
+static uint64_t call_token() {
+    static std::atomic<uint64_t> n{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 2654435761u};
+    const uint64_t t = n.fetch_add(0x9e3779b97f4a7c15ull);
+    return t ? t : 1;
 }
 
 bool on_this_device(const void* p, const char* what) {
@@ -886,7 +901,7 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
     a.weights_in = weights_in_dev; a.weights = weights_dev; a.out = (uint16_t*)out_dev; a.q_stride = q_stride;
     a.sc = scale * 1.4426950408889634f;
     unsigned char* ws = (unsigned char*)workspace_dev;
-    a.next = (uint32_t*)ws; a.plan = a.next + 2; a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
+    a.next = (uint32_t*)ws; a.start = (uint64_t*)(ws + 8); a.plan = a.next + 4; a.token = call_token(); a.part_ml = (float2*)(ws + l.ml); a.part_o = (float*)(ws + l.o);
     a.scores = weights_dev ? (float*)(ws + l.scores) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = dtype == GEHTP_DT_BF16, umma = n_prefix && l.umma;

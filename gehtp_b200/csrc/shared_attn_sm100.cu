@@ -152,10 +152,13 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
     const uint32_t tmem = bars->tmem_base;
     pdl_wait();
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
-        if (threadIdx.x == 0) { atomicExch(A.next, 0u); atomicExch(A.next + 1, 0u); __threadfence(); }
+        if (threadIdx.x == 0) {
+            A.next[0] = A.next[1] = 0;
+            asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(A.start), "l"(A.token) : "memory");
+        }
         __syncthreads();
     }
-    pdl_release();     // behind the wait: the tails' kernel starts beside this one and may read all that was there before the call
+    pdl_release();     // behind the wait: the tails' kernel starts beside this one, and by the token it sees all that this thread does
 
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0) {

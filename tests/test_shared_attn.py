@@ -419,3 +419,32 @@ def test_scores_far_out(cuda, dtype, batch, prefix, slots, order, q):
     eps += 2.0 ** -11 if dtype == "float16" else 2.0 ** -16
     got, want = call.out.double(), want.double()
     assert ((got - want).abs() <= want.abs() * (eps + 2.0 ** -19) + (2.0 ** -25 if dtype == "float16" else 0.0)).all()
+
+
+@pytest.mark.gpu
+def test_one_workspace_and_operands_replaced_before_every_call(cuda):
+    """Calls of different sizes behind one another with the same workspace, each behind the copies that bring its operands."""
+    import torch
+    kinds = [(40, 3, 8, 2, 128, 1500, 150), (6, 1, 32, 8, 64, 4000, 0), (33, 1, 16, 2, 64, 1200, 80), (64, 8, 8, 1, 128, 300, 40), (3, 2, 8, 2, 128, 96, 90)]
+    sets = []
+    for i, kind in enumerate(kinds):
+        calls = [Call(*kind, [(29 * x + 7 * turn) % (kind[6] + 1) for x in range(kind[0])], torch.float16, weights=kind[6] > 0, seed=10 * i + turn) for turn in range(3)]
+        for c in calls:
+            c.run(cuda)
+        torch.cuda.synchronize()
+        sets.append((Call(*kind, [0] * kind[0], torch.float16, weights=kind[6] > 0), calls))
+    ws = torch.full((max(s[0].size(cuda) for s in sets),), 255, dtype=torch.uint8, device="cuda")
+    got = []
+    for turn in range(60):
+        at, calls = sets[(turn * 3) % 5 if turn % 7 else turn % 5]
+        c = calls[turn % 3]
+        at.ws = ws
+        for x, y in ((at.rows, c.rows), (at.prefix, c.prefix), (at.tail, c.tail), (at.n_dev, c.n_dev)):
+            x.copy_(y)
+        if c.w is not None:
+            at.w_in.copy_(c.w_in), at.w.fill_(-5.0)
+        at.run(cuda)
+        got.append((c, at.out.clone(), at.w.clone() if c.w is not None else None))
+    torch.cuda.synchronize()
+    for c, out, w in got:
+        assert torch.equal(out, c.out) and (w is None or torch.equal(w, c.w))
