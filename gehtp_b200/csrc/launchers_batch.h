@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
+#include <initializer_list>
 
 namespace gehtp {
 
@@ -51,6 +52,18 @@ bool k_shared_merge(cudaStream_t st, const SharedArgs& a, uint32_t hd, bool bf16
 inline bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return !a || !b || x + a_bytes <= y || y + b_bytes <= x;
+}
+// Operands of a call: none of `outs` may share memory with another of them or with one of `ins`. What takes no bytes shares none.
+struct Span { const void* p; size_t bytes; };
+inline bool apart(Span a, Span b) { return !a.bytes || !b.bytes || apart(a.p, a.bytes, b.p, b.bytes); }
+inline bool all_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+    for (auto o = outs.begin(); o != outs.end(); o++) {
+        for (auto x = o + 1; x != outs.end(); x++)
+            if (!apart(*o, *x)) return false;
+        for (Span i : ins)
+            if (!apart(*o, i)) return false;
+    }
+    return true;
 }
 // true: `p` is memory of the current device (or managed); else g.last_error says which argument is not
 bool on_this_device(const void* p, const char* what);

@@ -897,6 +897,12 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
         (nslots && (!on_this_device(tail_dev, "attn shared: tail") || !on_this_device(n_tail_dev, "attn shared: n_tail"))) ||
         (weights_dev && !on_this_device(weights_dev, "attn shared: weights")) || (weights_in_dev && !on_this_device(weights_in_dev, "attn shared: weights_in")))
         return -1;
+    // in place, weights_in is an output already
+    const size_t tokens = (size_t)batch * q_len, row = (size_t)n_heads * head_dim, slot = (size_t)kv_heads * head_dim * 4;
+    if (!all_apart({{out_dev, tokens * row * 2}, {weights_dev, weights_dev ? w_bytes : 0}, {workspace_dev, l.total}},
+                   {{q_dev, ((tokens - 1) * q_stride + row) * 2}, {prefix_dev, n_prefix * slot}, {tail_dev, nslots * batch * slot},
+                    {n_tail_dev, nslots ? (size_t)batch * 4 : 0}, {weights_in_dev, weights_in_dev != weights_dev ? w_bytes : 0}}))
+        return fail("attn shared: an output or the workspace overlaps another operand");
     a.q = (const uint16_t*)q_dev; a.prefix = (const uint16_t*)prefix_dev; a.tail = (const uint16_t*)tail_dev; a.n_tail = n_tail_dev;
     a.weights_in = weights_in_dev; a.weights = weights_dev; a.out = (uint16_t*)out_dev; a.q_stride = q_stride;
     a.sc = scale * 1.4426950408889634f;

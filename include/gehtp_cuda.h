@@ -338,7 +338,8 @@ int gehtp_attn_decode_noalloc_status(void);
  * results go to a workspace of the caller, on a 256-byte boundary, of the size that the _workspace function gives for the
  * same sizes (0: sizes the operator does not take, gehtp_cuda_last_error says why). What is in it before a call does not
  * matter and nothing has to be kept of it. Calls that may overlap on the GPU need a workspace each, and so do captured graphs that
- * may be replayed at the same time. Return value: 0, or -1 with gehtp_cuda_last_error; after -1 nothing has been queued unless the
+ * may be replayed at the same time. Outputs and the workspace share no memory with one another or with inputs but where it says so; a call
+ * whose sizes say they would is refused. Return value: 0, or -1 with gehtp_cuda_last_error; after -1 nothing has been queued unless the
  * message is one of the CUDA runtime's. */
 
 /* Element types: WT_DT_F32, WT_DT_BF16 and fp16. */

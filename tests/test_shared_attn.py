@@ -448,3 +448,39 @@ def test_one_workspace_and_operands_replaced_before_every_call(cuda):
     torch.cuda.synchronize()
     for c, out, w in got:
         assert torch.equal(out, c.out) and (w is None or torch.equal(w, c.w))
+
+
+@pytest.mark.gpu
+def test_operands_that_overlap_are_refused(cuda):
+    """Every pair of an output or the workspace with another operand, by one byte at either end; nothing is queued."""
+    import torch
+    shape, prefix, slots = (2, 1, 16, 8, 128), 512, 64
+    ws = cuda.gehtp_attn_shared_workspace(*shape, prefix, slots, 1)
+    size = dict(q=4096 + 128 + 4096, prefix=prefix * 4096, tail=slots * 8192, n=8, w_in=4096, w=4096, out=8192, ws=ws)      # rows of q are 2112 elements apart
+    place, end = {}, 0
+    for name, bytes_ in size.items():
+        place[name] = end
+        end = (end + bytes_ + 255) // 256 * 256
+    buf = torch.zeros(end + 512, dtype=torch.uint8, device="cuda")
+    base = buf.data_ptr()
+    assert base % 256 == 0
+
+    def call(**moved):
+        at = {k: base + v for k, v in place.items()}
+        at.update({k: base + v for k, v in moved.items()})
+        return cuda.gehtp_attn_shared(at["q"], at["prefix"], at["tail"], at["n"], at["w_in"], at["w"], at["out"], *shape, 2112, prefix, slots, DT_F16, 0.1, at["ws"], ws,
+                                      torch.cuda.current_stream().cuda_stream)
+    assert call() == 0, cuda.gehtp_cuda_last_error()
+    assert call(w=place["w_in"]) == 0, cuda.gehtp_cuda_last_error()
+    torch.cuda.synchronize()
+    before = buf.clone()
+    unit = dict(q=16, prefix=16, tail=16, out=16, ws=256)
+    for a in ("out", "w", "ws"):
+        for b in size:
+            if a == b or {a, b} == {"w", "w_in"}:
+                continue
+            u = unit.get(a, 4)
+            for start in (place[b], place[b] + (size[b] - 1) // u * u):
+                assert call(**{a: start}) == -1 and b"overlap" in cuda.gehtp_cuda_last_error(), (a, b, start)
+    torch.cuda.synchronize()
+    assert torch.equal(before, buf)
