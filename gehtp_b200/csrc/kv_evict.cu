@@ -301,6 +301,10 @@ extern "C" int gehtp_kv_evict(const void* ring_dev, void* ring_out_dev, const fl
         !on_this_device(weights_out_dev, "kv evict: weights_out") || !on_this_device(n_dev, "kv evict: n") || !on_this_device(n_out_dev, "kv evict: n_out") ||
         !on_this_device(workspace_dev, "kv evict: workspace") || (kept_dev && !on_this_device(kept_dev, "kv evict: kept")))
         return -1;
+    const size_t ring = heads * nslots * head_dim * 4, w = heads * nslots * 4, n = (size_t)batch * 4;
+    if (!all_apart({{ring_out_dev, ring}, {weights_out_dev, w}, {n_out_dev, n}, {kept_dev, kept_dev ? heads * keep * 4 : 0}, {workspace_dev, need}},
+                   {{ring_dev, ring_dev != ring_out_dev ? ring : 0}, {weights_dev, weights_dev != weights_out_dev ? w : 0}, {n_dev, n_dev != n_out_dev ? n : 0}}))
+        return fail("kv evict: an output or the workspace overlaps another operand");
     EvictArgs a{(const uint16_t*)ring_dev, (uint16_t*)ring_out_dev, weights_dev, weights_out_dev, n_dev, n_out_dev, kept_dev, (int32_t*)workspace_dev,
                 batch, kv_heads, head_dim, nslots, keep, sinks, recent};
     if (!k_kv_evict((cudaStream_t)stream, a)) {

@@ -165,3 +165,38 @@ def test_refusals(cuda, change, message):
     at = lambda k: None if k in change and change[k] is None else base + change.get(k, 0)
     rc = cuda.gehtp_kv_evict(at("ring"), at("out"), at("w"), at("wo"), at("n"), at("no"), at("kept"), 2, 8, 128, 640, 512, 4, 64, at("ws"), change.get("size", 1 << 30), None)
     assert rc == -1 and message in cuda.gehtp_cuda_last_error()
+
+
+@pytest.mark.gpu
+def test_operands_that_overlap_are_refused(cuda):
+    """Every pair of an output or the workspace with another operand but the one that it may be; nothing is queued."""
+    import torch
+    shape = (2, 4, 64, 40, 20, 1, 4)                           # batch, kv_heads, head_dim, slots, keep, sinks, recent
+    ws = cuda.gehtp_kv_evict_workspace(*shape)
+    size = dict(ring=40 * 8 * 64 * 4, ring_out=40 * 8 * 64 * 4, w=8 * 40 * 4, w_out=8 * 40 * 4, n=8, n_out=8, kept=8 * 20 * 4, ws=ws)
+    place, end = {}, 0
+    for name, bytes_ in size.items():
+        place[name] = end
+        end = (end + bytes_ + 255) // 256 * 256
+    buf = torch.zeros(end + 512, dtype=torch.uint8, device="cuda")
+    base = buf.data_ptr()
+    assert base % 256 == 0
+
+    def call(**moved):
+        at = {k: base + v for k, v in place.items()}
+        at.update({k: base + v for k, v in moved.items()})
+        return cuda.gehtp_kv_evict(at["ring"], at["ring_out"], at["w"], at["w_out"], at["n"], at["n_out"], at["kept"], *shape, at["ws"], ws,
+                                   torch.cuda.current_stream().cuda_stream)
+    assert call() == 0 and call(ring_out=place["ring"], w_out=place["w"], n_out=place["n"]) == 0
+    torch.cuda.synchronize()
+    before = buf.clone()
+    unit = dict(ring_out=16, ws=256)
+    for a in ("ring_out", "w_out", "n_out", "kept", "ws"):
+        for b in size:
+            if a == b or a == b + "_out":
+                continue
+            u = unit.get(a, 4)
+            for start in (place[b], place[b] + (size[b] - 1) // u * u):
+                assert call(**{a: start}) == -1 and b"overlap" in cuda.gehtp_cuda_last_error(), (a, b, start)
+    torch.cuda.synchronize()
+    assert torch.equal(before, buf)
