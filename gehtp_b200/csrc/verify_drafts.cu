@@ -716,6 +716,11 @@ extern "C" int gehtp_verify_drafts(const void* target_dev, const void* draft_dev
         (!greedy && !on_this_device(uniforms_dev, "verify drafts: uniforms")) || !on_this_device(accepted_dev, "verify drafts: accepted") ||
         !on_this_device(out_dev, "verify drafts: out") || !on_this_device(workspace_dev, "verify drafts: workspace"))
         return -1;
+    const size_t rows = (size_t)batch * (n_drafts + 1), size = dtype == GEHTP_DT_F32 ? 4 : 2;
+    if (!all_apart({{accepted_dev, each}, {out_dev, rows * 4}, {workspace_dev, l.total}},
+                   {{target_dev, ((rows - 1) * target_stride + vocab) * size}, {draft, draft ? (((size_t)batch * n_drafts - 1) * draft_stride + vocab) * size : 0},
+                    {tokens_dev, all}, {n_drafts_dev, n_drafts_dev ? each : 0}, {uniforms_dev, greedy ? 0 : rows * 4}}))
+        return fail("verify drafts: an output or the workspace overlaps another operand");
     VerifyArgs a{};
     a.target = target_dev; a.draft = draft; a.tokens = tokens_dev; a.n_drafts = n_drafts_dev; a.uniforms = uniforms_dev;
     a.accepted = accepted_dev; a.out = out_dev; a.batch = batch; a.n = n_drafts; a.vocab = vocab;

@@ -309,3 +309,36 @@ def test_far_logits_at_a_low_temperature(cuda):
     target[torch.arange(4), 0, at] = 1048586.0
     accepted, out = verify(cuda, target, None, torch.zeros(4, 0, dtype=torch.int32), None, torch.tensor([[0.0], [0.3], [0.9], [0.5]]), 3000, 1e-4)
     assert out[:, 0].tolist() == at.tolist()
+
+
+@pytest.mark.gpu
+def test_operands_that_overlap_are_refused(cuda):
+    """Every pair of an output or the workspace with another operand; nothing is queued. What a greedy call does not read may lie anywhere."""
+    import torch
+    batch, n, vocab = 3, 2, 1000
+    ws = cuda.gehtp_verify_drafts_workspace(batch, n, vocab)
+    size = dict(target=9 * 1000 * 4, tokens=24, n=12, u=36, accepted=12, out=36, ws=ws, draft=(5 * 1010 + 1000) * 4)
+    place, end = {}, 0
+    for name, bytes_ in size.items():
+        place[name] = end
+        end = (end + bytes_ + 255) // 256 * 256
+    buf = torch.zeros(end + ws, dtype=torch.uint8, device="cuda")
+    base = buf.data_ptr()
+    assert base % 256 == 0
+
+    def call(heat=1.0, **moved):
+        at = {k: base + v for k, v in place.items()}
+        at.update({k: base + v for k, v in moved.items()})
+        return cuda.gehtp_verify_drafts(at["target"], at["draft"], at["tokens"], at["n"], at["u"], at["accepted"], at["out"], batch, n, vocab, 1000, 1010, DT_F32, heat,
+                                        at["ws"], ws, torch.cuda.current_stream().cuda_stream)
+    assert call() == 0 and call(0.0, ws=place["draft"]) == 0
+    torch.cuda.synchronize()
+    before = buf.clone()
+    for a in ("accepted", "out", "ws"):
+        for b in size:
+            if a != b:
+                u = 256 if a == "ws" else 4
+                for start in (place[b], place[b] + (size[b] - 1) // u * u):
+                    assert call(**{a: start}) == -1 and b"overlap" in cuda.gehtp_cuda_last_error(), (a, b, start)
+    torch.cuda.synchronize()
+    assert torch.equal(before, buf)
