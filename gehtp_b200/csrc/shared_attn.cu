@@ -877,7 +877,8 @@ extern "C" int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, cons
     const char* why;
     if (!lay_out(a, n_heads, head_dim, weights_dev != nullptr, l, &why)) return fail(why);
     if (dtype != GEHTP_DT_F16 && dtype != GEHTP_DT_BF16) return fail("attn shared: element type is GEHTP_DT_F16 or GEHTP_DT_BF16");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail("attn shared: scale is a positive number");
+    // the kernels' scale is to the base of 2
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.4426950408889634f)) return fail("attn shared: scale is a positive number below 2^127");
     if (!q_dev || !out_dev || !workspace_dev || (n_prefix && !prefix_dev) || (nslots && (!tail_dev || !n_tail_dev))) return fail("attn shared: null pointer");
     if (weights_in_dev && !weights_dev) return fail("attn shared: weights_in without weights");
     if (q_stride < (size_t)n_heads * head_dim || q_stride % 8) return fail("attn shared: q_stride is a multiple of 8, n_heads * head_dim at least");

@@ -363,7 +363,7 @@ int gehtp_attn_decode_noalloc_status(void);
  * q, prefix, tail and out are of type `dtype` (GEHTP_DT_F16 or GEHTP_DT_BF16), on 16-byte boundaries; out and weights overlap no input
  * otherwise. Scores, softmax and sums are fp32. A softmax weight meets the values as one fp16 word (off by 2^-11 of itself, or by 2^-37 of the row's
  * largest where that is more: positions that weigh less than that count in the sum alone) or as two bf16 words (off by 2^-16). head_dim 64 or 128, batch up to 1024, q_len up to 16, q_len * n_heads / kv_heads up to
- * 128, batch * kv_heads up to 65535, scale > 0. */
+ * 128, batch * kv_heads up to 65535, scale > 0 and below 2^127. */
 size_t gehtp_attn_shared_workspace(uint32_t batch, uint32_t q_len, uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim,
                                    uint32_t n_prefix, uint32_t nslots, int with_weights);
 int gehtp_attn_shared(const void* q_dev, const void* prefix_dev, const void* tail_dev, const int32_t* n_tail_dev,

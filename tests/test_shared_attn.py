@@ -484,3 +484,11 @@ def test_operands_that_overlap_are_refused(cuda):
                 assert call(**{a: start}) == -1 and b"overlap" in cuda.gehtp_cuda_last_error(), (a, b, start)
     torch.cuda.synchronize()
     assert torch.equal(before, buf)
+
+
+@pytest.mark.parametrize("scale,message", [(3e38, b"scale"), (2.0 ** 127, b"no memory of the current device"), (1e-45, b"no memory of the current device")])
+def test_scales_that_have_no_end_to_the_base_of_two(cuda, scale, message):
+    """log2(e) times the scale has to be a number: a score of 0 would be none."""
+    buf = np.zeros(1 << 16, np.uint8)
+    at = (buf.ctypes.data + 255) // 256 * 256
+    assert cuda.gehtp_attn_shared(at, at, at, at, None, None, at, 2, 1, 16, 8, 128, 2048, 512, 64, DT_F16, scale, at, 1 << 40, None) == -1 and message in cuda.gehtp_cuda_last_error()
