@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t mbar_seen(uint64_t* bar, uint32_t parity) {
 
 template <int ST>
 struct __align__(8) PBars {
-    uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[2], p_full[2], o_full, merge;
+    uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[2], p_full[2], o_full, merge, drained;
     uint32_t tmem_base, abort_flag;
 };
 
@@ -136,7 +136,7 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
     if (threadIdx.x == 32)
         for (const CUtensorMap* map : {&tmap_q, &tmap_kv}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     if (threadIdx.x == 0) {
-        mbar_init(&bars->q_full, 1); mbar_init(&bars->o_full, 1); mbar_init(&bars->merge, 8);
+        mbar_init(&bars->q_full, 1); mbar_init(&bars->o_full, 1); mbar_init(&bars->drained, 1); mbar_init(&bars->merge, 8);
         for (int s = 0; s < ST; s++) { mbar_init(&bars->kv_full[s], 1); mbar_init(&bars->kv_empty[s], 1); }
         for (int s = 0; s < 2; s++) { mbar_init(&bars->s_full[s], 1); mbar_init(&bars->p_full[s], 4); }
         bars->abort_flag = 0;
@@ -267,8 +267,13 @@ shared_prefix_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __g
                 }
             }
         }
-        if (ok) commit(&bars->o_full);
-        else if (lane == 0) *abort_flag = 1;
+        if (ok) {
+            commit(&bars->o_full);
+        } else {                 // products under way still read shared memory and write the TMEM that the CTA is about to give back
+            if (lane == 0) *abort_flag = 1;
+            commit(&bars->drained);
+            mbar_wait(&bars->drained, 0);
+        }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax and output: one thread per row and group
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");    // 256 x 200 + 128 x 104 = 384 x 168, what the CTA was launched with
