@@ -12,7 +12,8 @@
 // that where there are many: 64 sequences of 512 to 2048 positions cut to 1024 100 us in two launches, 90 in one; and a launch is some 2 us of the
 // host's time: two sequences 13.5 -> 11.8 us call by call.
 // evict_select_kernel, evict_move_kernel: lists that shared memory does not hold, and lengths replaced in place, which no CTA may write
-// before all have read them.
+// before all have read them. In place (rows that stay where they are do not move) 64 sequences of 512 to 2048 cut to 1024 take 79 us in one launch and 77 in
+// two, two sequences 9.0 and 11.9.
 #include <cstdio>
 #include <algorithm>
 #include "engine.h"

@@ -8,10 +8,6 @@
 
 namespace gehtp {
 
-// Attention over a shared prefix and own tails. A row is one query head of one token; the rows that meet a key head's
-// prefix together are those of p_tokens tokens (a row tile), those that meet a tail are the q_len * rep of its sequence.
-// Every (row tile, key head, slice of the prefix) and every (sequence, key head, slice of its tail) leaves a partial result per
-// row: the sum of 2^(s - m) v, the sum of 2^(s - m) and the maximum m, with s = log2(e) * scale * q.k.
 // n / d by a product, for n * d < 2^32
 struct Div {
     uint64_t m;
@@ -20,6 +16,11 @@ struct Div {
     __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((n * m) >> 32); }
 };
 
+// Attention over a shared prefix and own tails. A row is one query head of one token; the rows that meet a key head's
+// prefix together are those of p_tokens tokens (a row tile), those that meet a tail are the q_len * rep of its sequence.
+// Every (row tile, key head, slice of the prefix) and every (sequence, key head, slice of its tail) leaves a partial result per
+// row: the sum of 2^(s - m) v, the sum of 2^(s - m) and the reference m, with s = log2(e) * scale * q.k. m is a maximum, or what the prefix's
+// kernel took in its place.
 struct SharedArgs {
     const uint16_t *q, *prefix, *tail;
     const int32_t* n_tail;

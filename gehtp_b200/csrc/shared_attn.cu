@@ -288,8 +288,8 @@ struct Few {
 
 // RT warps share an item, 16 rows each (RT: 1, 2, 4 or 8; 0: one warp and at most 8 rows), and the tiles of 16 RT positions that they bring in by cp.async. They meet once a
 // tile among themselves and with nobody else, so that what an item costs to begin and to end is other groups' time: eight warps an
-// SM, 24 KB of tiles each (twelve of 16 KB where rows are at most 8). A CTA to an item, with 64 positions split over its warps, took 93 us where this takes 89 (32 sequences,
-// tails of 1024 to 4096).
+// SM, 24 KB of tiles each (twelve of 16 KB where rows are at most 8). A CTA to an item, with 64 positions split over its warps, took 93 us where a group to an item
+// of whatever few rows took 89 (32 sequences, tails of 1024 to 4096, before rows of at most 8 had their own form, which takes 74).
 template <int HD, int RT>
 __host__ __device__ constexpr int warp_stages() { return (HD == 128 ? 1 : 2) * (RT ? 3 : 2); }
 template <int RT>
@@ -777,7 +777,8 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
     const size_t tokens = (size_t)a.batch * a.q_len, rows = tokens * a.rep;
     const uint32_t tail_rows = a.q_len * a.rep, t_rt = row_tiles(tail_rows);
     // slices of the tails: three to a group of warps that one row tile makes, one or two where more do (64 sequences x 8 tokens: 6 an SM 165 us,
-    // 12 170), somewhat less than two to a warp of at most 8 rows (32 sequences with weights: 23 an SM 74.7 us, 16 78.8, 27 79.7)
+    // 12 170), 23 an SM, which has twelve warps, for rows of at most 8: the best of
+    // three at one size (32 sequences with weights: 23 an SM 74.7 us, 16 78.8, 27 79.7)
     a.t_slices = std::max(1u, (tail_rows <= 8 ? 23 : t_rt == 1 ? 24 : std::max(3u, 12 / t_rt)) * SMS / a.kv_heads);
     // The prefix goes with the tails, in their launch, while its rows fit into their row tile, or are in few tiles of 16 and meet few
     // positions; else on tcgen05. 8 heads of 128, 32 rows: 512 positions 11.2 us with the tails, 13.3 on tcgen05; 2048 15.0 and
@@ -795,7 +796,8 @@ bool lay_out(SharedArgs& a, uint32_t n_heads, uint32_t hd, bool with_weights, La
         if (l.umma) {
             // What a number of slices costs, in us: a CTA takes about 7 and 2.6 a tile of two row tiles (1.6 of one). SMs that have none
             // work on the tails meanwhile, 43 KB a us each, 30 while slices are one tile; what is left of those behind the prefix begins
-            // 4 us later. The tails are taken as half full. 8 sequences behind 8192 positions: 16 slices, which fill the SMs best, 32.8 us,
+            // 4 us later. The tails are taken as half full. (Heads of 128; those of 64 go by the same prices, which were
+            // not measured for them.) 8 sequences behind 8192 positions: 16 slices, which fill the SMs best, 32.8 us,
             // this way 26.6 (replayed, L2 cold); 64 behind 32768: 18 slices 95.4, 84.6; 32 with 2048 slots behind 16384: 67.3, 63.1.
             const bool short_ones = (size_t)a.batch * a.nslots / 2 / TILE <= a.t_slices;
             const double per = a.p_tiles > 1 ? 2.6 : 1.6, work = (double)a.batch * a.kv_heads * a.nslots * hd * 4 / 2 / (short_ones ? 30e3 : 43e3);

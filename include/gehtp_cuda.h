@@ -340,7 +340,9 @@ int gehtp_attn_decode_noalloc_status(void);
  * matter and nothing has to be kept of it. Calls that may overlap on the GPU need a workspace each, and so do captured graphs that
  * may be replayed at the same time. Outputs and the workspace share no memory with one another or with inputs but where it says so; a call
  * whose sizes say they would is refused. Return value: 0, or -1 with gehtp_cuda_last_error; after -1 nothing has been queued unless the
- * message is one of the CUDA runtime's. */
+ * message is one of the CUDA runtime's. As everywhere in this interface the caller is one thread.
+ * Caches are the caller's: the states of the engine above have no device address here, so a prompt that a runlist has prefilled comes to `prefix`
+ * by gehtp_cuda_state_read and a copy. Logits that a runlist leaves in a temp can be verified where they are (gehtp_cuda_temp_dev). */
 
 /* Element types: WT_DT_F32, WT_DT_BF16 and fp16. */
 #define GEHTP_DT_F32   0u
@@ -358,10 +360,11 @@ int gehtp_attn_decode_noalloc_status(void);
  *            What lies in slots from n_tail on is never read.
  *   weights  NULL, or fp32 [batch][kv_heads][nslots]: position p < n_tail gets weights_in[p] + the softmax weight that the key head's
  *            q_len * n_heads / kv_heads rows give it, positions from n_tail on are left as they are. weights_in: NULL stands for zeros;
- *            may be `weights` itself, but not overlap it otherwise
+ *            may be `weights` itself, but not overlap it otherwise. All q_len new tokens give their weights, drafts that are then
+ *            refused among them: what those gave to positions that stay is not taken back
  *   out      [batch][q_len][n_heads][head_dim]; a row that sees no position at all is zeros
  * q, prefix, tail and out are of type `dtype` (GEHTP_DT_F16 or GEHTP_DT_BF16), on 16-byte boundaries; out and weights overlap no input
- * otherwise. Scores, softmax and sums are fp32. A softmax weight meets the values as one fp16 word (off by 2^-11 of itself, or by 2^-37 of the row's
+ * otherwise. A row whose every score is -inf is zeros too. Scores, softmax and sums are fp32. A softmax weight meets the values as one fp16 word (off by 2^-11 of itself, or by 2^-37 of the row's
  * largest where that is more: positions that weigh less than that count in the sum alone) or as two bf16 words (off by 2^-16). head_dim 64 or 128, batch up to 1024, q_len up to 16, q_len * n_heads / kv_heads up to
  * 128, batch * kv_heads up to 65535, scale > 0 and below 2^127. */
 size_t gehtp_attn_shared_workspace(uint32_t batch, uint32_t q_len, uint32_t n_heads, uint32_t kv_heads, uint32_t head_dim,
@@ -400,7 +403,7 @@ int gehtp_kv_evict(const void* ring_dev, void* ring_out_dev, const float* weight
  * p_i = softmax(target_i / temperature), q_i = softmax(draft_i / temperature). Draft i of a sequence is accepted while
  * uniforms[i] * q_i(token_i) < p_i(token_i). At the first place that is not accepted the token is drawn from max(p_i - q_i, 0) (from p_i
  * where its sum is below 1e-12: rows that are alike), behind n accepted ones from p_n: the first token whose cumulated share is above
- * uniforms[n_drafts]. temperature 0: draft i is accepted while it is the lowest place of target_i's largest logit, and the token behind
+ * uniforms[n_drafts]. Acceptance goes by sums in fp32, off by some 2^-20 of a probability; the draw by 64 bits. temperature 0: draft i is accepted while it is the lowest place of target_i's largest logit, and the token behind
  * the accepted ones is that place; draft and uniforms are not read.
  *   target   [batch][n_drafts + 1] rows of `vocab` logits, target_stride elements apart: row i is what follows draft i - 1
  *   draft    [batch][n_drafts] rows, draft_stride apart, or NULL: drafts without probabilities (found by lookup, or chosen greedily),
